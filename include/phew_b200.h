@@ -308,6 +308,82 @@ int phew_dequantize(const void* wq, const void* scales, const void* biases, void
 int phew_quantize(const void* w, void* wq, void* scales, void* biases, int64_t rows,
                   int64_t cols, int group_size, int bits, int dtype, void* stream);
 
+/* ---- quantised key/value cache ------------------------------------------- */
+
+/* Keys and values in the affine group-wise layout above, in pages of token
+ * rows, written and read in place:
+ *   codes  [pages][kv_heads][page_size][head_dim * bits / 32] uint32
+ *   scales, biases  [pages][kv_heads][page_size][head_dim / group_size], `dtype`
+ * bits 4 or 8; head_dim 64, 128 or 256; group_size 32, 64 or 128, dividing
+ * head_dim.  All arrays contiguous and 16-byte aligned.
+ * Position p of sequence b lies in page block_table[b][p / page_size]
+ * (int32, rows `table_stride` entries apart, `columns` entries each) at row
+ * p % page_size; with block_table NULL, in page b.  Lengths, offsets and the
+ * table live on the device, so that a captured graph replays with new ones;
+ * table entries behind a sequence's last page are not read.  A position
+ * outside a sequence's pages or a table entry that is no page of the cache
+ * is not accessed: it sets *error_flag (device int) to PHEW_ERR_INVALID. */
+typedef struct phew_kv_cache {
+  void* k_codes;
+  void* k_scales;
+  void* k_biases;
+  void* v_codes;
+  void* v_scales;
+  void* v_biases;
+  int64_t pages;
+  int64_t page_size;
+  int kv_heads;
+  int head_dim;
+  int group_size;
+  int bits;
+  int dtype;
+} phew_kv_cache;
+
+/* Quantises tokens [0, counts[b]) of k[b], v[b] ([batch][kv_heads][tokens]
+ * [head_dim] views of the cache's dtype; strides {token, head, batch} in
+ * elements, multiples of 16 bytes) into positions offsets[b] + token, with the
+ * arithmetic of phew_quantize; counts NULL = all tokens.  Other rows of the
+ * cache stay as they were.  With k_out / v_out (contiguous) it also writes
+ * the values the cache now stands for (phew_dequantize's), zero for tokens
+ * behind counts[b].  Two tokens of one call must not name the same row.
+ * The cache side of mx.fast.quantized_scaled_dot_product_attention
+ * (emit/codegen.py:428-449), written a step at a time. */
+int phew_kv_update(const phew_kv_cache* cache, const void* k, const void* v, const int64_t* k_strides,
+                   const int64_t* v_strides, int64_t batch, int64_t tokens, const int* offsets,
+                   const int* counts, const int* block_table, int64_t table_stride, int64_t columns,
+                   void* k_out, void* v_out, int* error_flag, void* stream);
+
+/* Values of positions [0, min(lengths[b], out_len)) of every sequence as
+ * dense [batch][kv_heads][out_len][head_dim] arrays of the cache's dtype
+ * (phew_dequantize's values), zero behind a sequence's length.  The dense k
+ * and v that phew_sdpa or phew_gemm take. */
+int phew_kv_fetch(const phew_kv_cache* cache, void* k_out, void* v_out, int64_t batch, int64_t out_len,
+                  const int* lengths, const int* block_table, int64_t table_stride, int64_t columns,
+                  int* error_flag, void* stream);
+
+/* Bytes of device scratch phew_kv_attention needs on the current device. */
+size_t phew_kv_attention_workspace(const phew_kv_cache* cache, int64_t batch, int64_t heads,
+                                   int64_t tokens);
+
+/* o = softmax(scale * q k^T) v over a 4-bit cache: q [batch][heads][tokens]
+ * [head_dim] of the cache's dtype (strides {token, head, batch} in elements,
+ * multiples of 16 bytes), o contiguous, heads a multiple of kv_heads (query
+ * head h reads cache head h / (heads / kv_heads)).  Sequence b has
+ * lengths[b] keys and counts[b] query tokens (NULL = all).  causal = 1: the
+ * last query token sits at the last key, token i sees keys
+ * j <= lengths[b] - counts[b] + i.  Rows that see no key, and rows behind
+ * counts[b], are zero.  Scores, softmax statistics and sums are fp32.
+ * `workspace`: caller-owned scratch of phew_kv_attention_workspace bytes,
+ * 16-byte aligned; calls that may overlap need one each.
+ * Replaces mx.fast.quantized_scaled_dot_product_attention
+ * (emit/codegen.py:428-449; FastQuantizedScaledDotProductAttention
+ * ir/ops.py:191-200) where k and v are kept between calls. */
+int phew_kv_attention(const phew_kv_cache* cache, const void* q, const int64_t* q_strides, void* o,
+                      int64_t batch, int64_t heads, int64_t tokens, const int* lengths,
+                      const int* counts, const int* block_table, int64_t table_stride,
+                      int64_t columns, float scale, int causal, void* workspace,
+                      size_t workspace_bytes, int* error_flag, void* stream);
+
 /* ---- seeded inputs for the verification sweep -------------------------- */
 
 #define PHEW_FILL_NORMAL 0       /* N(0, 1) * scale (Box-Muller)           */

@@ -52,6 +52,10 @@ EXPORTED_SYMBOLS = (
     "phew_reduce_var",
     "phew_dequantize",
     "phew_quantize",
+    "phew_kv_update",
+    "phew_kv_fetch",
+    "phew_kv_attention_workspace",
+    "phew_kv_attention",
     "phew_copy_strided_to",
     "phew_reduce",
     "phew_copy_strided",
@@ -109,6 +113,24 @@ class CompareStats(ctypes.Structure):
     ]
 
 
+class KVCache(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p),
+        ("k_scales", ctypes.c_void_p),
+        ("k_biases", ctypes.c_void_p),
+        ("v_codes", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("v_biases", ctypes.c_void_p),
+        ("pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("group_size", ctypes.c_int),
+        ("bits", ctypes.c_int),
+        ("dtype", ctypes.c_int),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -146,6 +168,21 @@ _SIGNATURES = {
     "phew_softmax": ([_vp, _vp, _i64, _i64, _int, _vp], _int),
     "phew_reduce_var": ([_vp, _vp, _i64, _i64, _i64, _int, _int, _vp], _int),
     "phew_dequantize": ([_vp, _vp, _vp, _vp, _i64, _i64, _int, _int, _int, _vp], _int),
+    "phew_kv_update": (
+        [ctypes.POINTER(KVCache), _vp, _vp, ctypes.POINTER(_i64), ctypes.POINTER(_i64), _i64, _i64, _vp, _vp,
+         _vp, _i64, _i64, _vp, _vp, _vp, _vp],
+        _int,
+    ),
+    "phew_kv_fetch": (
+        [ctypes.POINTER(KVCache), _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp],
+        _int,
+    ),
+    "phew_kv_attention_workspace": ([ctypes.POINTER(KVCache), _i64, _i64, _i64], ctypes.c_size_t),
+    "phew_kv_attention": (
+        [ctypes.POINTER(KVCache), _vp, ctypes.POINTER(_i64), _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64,
+         ctypes.c_float, _int, _vp, ctypes.c_size_t, _vp, _vp],
+        _int,
+    ),
     "phew_copy_strided_to": (
         [_vp, _vp, _int, ctypes.POINTER(_i64), ctypes.POINTER(_i64), ctypes.POINTER(_i64), _int, _vp],
         _int,

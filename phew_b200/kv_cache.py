@@ -1,0 +1,301 @@
+"""A quantised key/value cache: tokens written into pages, read back, attended to.
+
+The k and v that ``mx.fast.quantized_scaled_dot_product_attention`` takes
+(phew ``emit/codegen.py:428-449``), kept between calls: the affine group-wise
+codes of ``mx.quantize``, in pages, written one step at a time and read in
+place.  Lengths, offsets and block tables are int32 arrays on the device, so
+a step captured into a CUDA graph replays with new ones.
+"""
+
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import torch
+
+from . import _native
+from . import dtypes as dt
+
+_error_flags: dict[int, torch.Tensor] = {}
+
+
+def _core():
+    from .mx import core
+
+    return core
+
+
+def _on(device: torch.device):
+    """Makes `device` current when it is not (kernels launch on the current one)."""
+    if torch.cuda.current_device() == device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def cache_error_flag(device: torch.device) -> torch.Tensor:
+    """Device int that the cache's kernels set when a position or a page lies
+    outside the cache (0 = clean)."""
+    f = _error_flags.get(device.index)
+    if f is None:
+        f = torch.zeros(1, dtype=torch.int32, device=device)
+        _error_flags[device.index] = f
+    return f
+
+
+def check_cache_errors() -> None:
+    """Raise if a kernel of the cache met a position outside a sequence's
+    pages or a block table entry that is no page (synchronises)."""
+    for f in _error_flags.values():
+        code = int(f.item())
+        if code:
+            f.zero_()
+            raise _native.PhewError(
+                code, "quantised cache: a length or offset outside a sequence's pages, or a block "
+                      "table entry that is no page of the cache")
+
+
+class QuantizedKVCache:
+    """Keys and values in pages of token rows, ``(codes, scales, biases)`` each:
+
+    * codes ``[pages, kv_heads, page_size, head_dim * bits / 32]`` uint32 (or
+      int32), packed as by ``mx.quantize`` along the head dimension;
+    * scales, biases ``[pages, kv_heads, page_size, head_dim / group_size]`` in
+      the cache's dtype (float32, float16 or bfloat16).
+
+    ``bits`` 4 or 8 (attention reads 4), ``head_dim`` 64, 128 or 256,
+    ``group_size`` 32, 64 or 128.  The arrays are the caller's: ``update``
+    writes into them.  A block table ``[batch, columns]`` names each sequence's
+    pages in order; without one page b belongs to sequence b.
+    """
+
+    __slots__ = ("keys", "values", "pages", "kv_heads", "page_size", "head_dim", "group_size", "bits",
+                 "dtype", "device", "_struct", "_workspaces")
+
+    def __init__(self, keys, values, *, group_size: int = 64, bits: int = 4) -> None:
+        core = _core()
+        if len(keys) != 3 or len(values) != 3:
+            raise ValueError("QuantizedKVCache: keys and values are (codes, scales, biases) each")
+        parts = [a if isinstance(a, core.array) else core.array(a) for a in (*keys, *values)]
+        g, nb = int(group_size), int(bits)
+        if nb not in (4, 8):
+            raise ValueError(f"QuantizedKVCache: bits must be 4 or 8, got {bits}")
+        if g not in (32, 64, 128):
+            raise ValueError(f"QuantizedKVCache: group_size must be 32, 64 or 128, got {group_size}")
+        codes, scales = parts[0], parts[1]
+        if codes.ndim != 4:
+            raise ValueError(f"QuantizedKVCache: codes must be [pages, kv_heads, page_size, words], got {codes.shape}")
+        dim = codes.shape[-1] * 32 // nb
+        if dim not in (64, 128, 256) or dim % g:
+            raise ValueError(f"QuantizedKVCache: head_dim must be 64, 128 or 256 and a multiple of group_size, "
+                             f"got {dim} at group_size {g}")
+        if scales.dtype.code is None:
+            raise TypeError(f"QuantizedKVCache: unsupported scale dtype {scales.dtype.name}")
+        want = codes.shape[:-1] + (dim // g,)
+        for i, a in enumerate(parts):
+            name = ("key ", "value ")[i // 3] + ("codes", "scales", "biases")[i % 3]
+            if i % 3 == 0:
+                if a.dtype.name not in ("uint32", "int32"):
+                    raise TypeError(f"QuantizedKVCache: {name} must be uint32, got {a.dtype.name}")
+                if a.shape != codes.shape:
+                    raise ValueError(f"QuantizedKVCache: {name} shape {a.shape} != {codes.shape}")
+            else:
+                if a.dtype is not scales.dtype:
+                    raise TypeError(f"QuantizedKVCache: {name} must be {scales.dtype.name}, got {a.dtype.name}")
+                if a.shape != want:
+                    raise ValueError(f"QuantizedKVCache: {name} shape {a.shape} != {want}")
+            if not a._t.is_contiguous() or a._t.data_ptr() % 16:
+                raise ValueError(f"QuantizedKVCache: {name} must be contiguous and 16-byte aligned "
+                                 "(the cache is written in place)")
+            if a._t.device != codes._t.device:
+                raise ValueError(f"QuantizedKVCache: {name} lies on another device")
+        if codes.size == 0:
+            raise ValueError("QuantizedKVCache: empty cache")
+        self.keys, self.values = tuple(parts[:3]), tuple(parts[3:])
+        self.pages, self.kv_heads, self.page_size = codes.shape[:3]
+        self.head_dim, self.group_size, self.bits, self.dtype = dim, g, nb, scales.dtype
+        self.device = codes._t.device
+        self._struct = _native.KVCache(*(ctypes.c_void_p(a._t.data_ptr()) for a in parts), self.pages,
+                                       self.page_size, self.kv_heads, dim, g, nb, self.dtype.code)
+        self._workspaces: dict[tuple, int] = {}
+
+    @classmethod
+    def zeros(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, dtype="bfloat16", *,
+              group_size: int = 64, bits: int = 4) -> "QuantizedKVCache":
+        """A cache of its own arrays, all zero."""
+        core = _core()
+        if int(bits) not in (4, 8) or int(group_size) not in (32, 64, 128):
+            raise ValueError("QuantizedKVCache: bits must be 4 or 8, group_size 32, 64 or 128")
+        d, rows = dt.from_any(dtype), (int(pages), int(kv_heads), int(page_size))
+
+        def side():
+            codes = torch.zeros(rows + (head_dim * int(bits) // 32,), dtype=torch.int32, device=core.device())
+            sb = [torch.zeros(rows + (head_dim // int(group_size),), dtype=d.torch, device=core.device())
+                  for _ in range(2)]
+            return tuple(core.array(t) for t in (codes, *sb))
+
+        return cls(side(), side(), group_size=group_size, bits=bits)
+
+
+def _ints(x, shape, what: str, cache: QuantizedKVCache) -> torch.Tensor:
+    """An int32 device array of `shape` (a host sequence is copied in)."""
+    core = _core()
+    a = x if isinstance(x, core.array) else core.array(x, None if isinstance(x, torch.Tensor) else core.int32)
+    t = a._t
+    if t.dtype != torch.int32:
+        raise TypeError(f"{what} must be int32, got {a.dtype.name}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{what} shape {tuple(t.shape)} != {shape}")
+    if t.device != cache.device:
+        raise ValueError(f"{what} lies on another device than the cache")
+    return t if t.is_contiguous() else core.contiguous_copy(a)._t
+
+
+def _table(block_table, batch: int, what: str, cache: QuantizedKVCache):
+    """(tensor that holds the table or None, pointer, row stride, columns)."""
+    if block_table is None:
+        if batch > cache.pages:
+            raise ValueError(f"{what}: without a block_table the cache needs a page for each of the {batch} "
+                             f"sequences, it has {cache.pages}")
+        return None, None, 0, 1
+    core = _core()
+    a = block_table
+    if not isinstance(a, core.array):
+        a = core.array(a, None if isinstance(a, torch.Tensor) else core.int32)
+    t = a._t
+    if t.dtype != torch.int32:
+        raise TypeError(f"{what}: block_table must be int32, got {a.dtype.name}")
+    if t.dim() != 2 or t.shape[0] != batch or t.shape[1] == 0:
+        raise ValueError(f"{what}: block_table shape {tuple(t.shape)} is not [{batch}, columns]")
+    if t.device != cache.device:
+        raise ValueError(f"{what}: block_table lies on another device than the cache")
+    if t.stride(1) != 1 and t.shape[1] > 1 or t.stride(0) < 0:
+        t = core.contiguous_copy(a)._t
+    return t, t.data_ptr(), t.stride(0), t.shape[1]
+
+
+def _rows(x, shape, what: str, cache: QuantizedKVCache):
+    """(tensor, strides {token, head, batch}) of a [batch, heads, tokens, head_dim]
+    view that the kernels read in place: unit stride along the head dimension
+    and 16-byte aligned rows; anything else is copied first."""
+    core = _core()
+    a = core.asarray_device(x, contiguous=False)
+    if a.dtype is not cache.dtype:
+        raise TypeError(f"{what} must be {cache.dtype.name} like the cache, got {a.dtype.name}")
+    t = a._t
+    if t.dim() != 4 or any(w is not None and n != w for n, w in zip(t.shape, shape)):
+        raise ValueError(f"{what} shape {tuple(t.shape)} is not "
+                         f"[{', '.join('*' if w is None else str(w) for w in shape)}]")
+    if t.numel() == 0:
+        raise ValueError(f"{what} is empty")
+    if t.device != cache.device:
+        raise ValueError(f"{what} lies on another device than the cache")
+    unit = 16 // t.element_size()
+    s = t.stride()
+    if s[3] != 1 or s[0] % unit or s[1] % unit or s[2] % unit or t.data_ptr() % 16:
+        t = core.contiguous_copy(core.array._wrap(t))._t
+        s = t.stride()
+    return t, (ctypes.c_int64 * 3)(s[2], s[1], s[0])
+
+
+def _call(name: str, cache: QuantizedKVCache, *args) -> None:
+    _native.call(name, cache._struct, *args, cache_error_flag(cache.device).data_ptr(),
+                 torch.cuda.current_stream(cache.device).cuda_stream)
+
+
+def quantized_cache_update(cache: QuantizedKVCache, k, v, offsets, *, block_table=None, counts=None,
+                           fetch: bool = False):
+    """Quantises ``k``, ``v`` ``[batch, kv_heads, tokens, head_dim]`` (the cache's
+    dtype) into the cache at positions ``offsets[b] + token``, in place.
+
+    ``counts`` (int32 ``[batch]``, default all) limits a padded batch to its
+    first tokens; every other row of the cache stays as it was.  A row's codes,
+    scales and biases are those of ``mx.quantize`` on it.  With ``fetch`` the
+    values that the new tokens now stand for are returned as ``(k, v)`` like
+    the inputs (``mx.dequantize``'s, zero behind ``counts``), e.g. for a prompt's
+    own attention.  Two tokens of one call must not land in the same row.
+    A position or page outside the cache is left unwritten and reported by
+    ``ops.check_device_errors``.
+    """
+    k, ks = _rows(k, (None, cache.kv_heads, None, cache.head_dim), "quantized_cache_update: k", cache)
+    v, vs = _rows(v, tuple(k.shape), "quantized_cache_update: v", cache)
+    batch, tokens = k.shape[0], k.shape[2]
+    off = _ints(offsets, (batch,), "quantized_cache_update: offsets", cache)
+    cnt = None if counts is None else _ints(counts, (batch,), "quantized_cache_update: counts", cache)
+    keep, table, stride, columns = _table(block_table, batch, "quantized_cache_update", cache)
+    with _on(cache.device):
+        ko = torch.empty(k.shape, dtype=k.dtype, device=cache.device) if fetch else None
+        vo = torch.empty(k.shape, dtype=k.dtype, device=cache.device) if fetch else None
+        _call("phew_kv_update", cache, k.data_ptr(), v.data_ptr(), ks, vs, batch, tokens, off.data_ptr(),
+              None if cnt is None else cnt.data_ptr(), table, stride, columns,
+              ko.data_ptr() if fetch else None, vo.data_ptr() if fetch else None)
+    del keep
+    if not fetch:
+        return None
+    wrap = _core().array._wrap
+    return wrap(ko), wrap(vo)
+
+
+def quantized_cache_fetch(cache: QuantizedKVCache, lengths, *, block_table=None, max_length: int | None = None):
+    """The first ``lengths[b]`` tokens of every sequence as dense ``(k, v)``
+    ``[batch, kv_heads, max_length, head_dim]`` in the cache's dtype
+    (``mx.dequantize``'s values), zero behind a sequence.  ``max_length``
+    defaults to what a sequence's pages hold; longer sequences are cut there.
+    """
+    core = _core()
+    if not isinstance(lengths, (core.array, torch.Tensor)):
+        lengths = core.array(lengths, core.int32)
+    if len(lengths.shape) != 1 or lengths.shape[0] == 0:
+        raise ValueError(f"quantized_cache_fetch: lengths shape {tuple(lengths.shape)} is not [batch]")
+    batch = lengths.shape[0]
+    n = _ints(lengths, (batch,), "quantized_cache_fetch: lengths", cache)
+    keep, table, stride, columns = _table(block_table, batch, "quantized_cache_fetch", cache)
+    out_len = columns * cache.page_size if max_length is None else int(max_length)
+    if out_len <= 0:
+        raise ValueError(f"quantized_cache_fetch: max_length must be positive, got {max_length}")
+    shape = (batch, cache.kv_heads, out_len, cache.head_dim)
+    with _on(cache.device):
+        k = torch.empty(shape, dtype=cache.dtype.torch, device=cache.device)
+        v = torch.empty(shape, dtype=cache.dtype.torch, device=cache.device)
+        _call("phew_kv_fetch", cache, k.data_ptr(), v.data_ptr(), batch, out_len, n.data_ptr(), table, stride,
+              columns)
+    del keep
+    return core.array._wrap(k), core.array._wrap(v)
+
+
+def quantized_cache_attention(q, cache: QuantizedKVCache, lengths, *, block_table=None, counts=None,
+                              scale: float = 1.0, mask=None):
+    """``softmax(scale * q k^T) v`` over a 4-bit cache -> ``[batch, heads, tokens, head_dim]``.
+
+    ``q`` ``[batch, heads, tokens, head_dim]`` in the cache's dtype, heads a
+    multiple of the cache's (query head h reads cache head h // (heads /
+    kv_heads)); ``lengths`` (int32 ``[batch]``) the keys of each sequence, new
+    tokens included; ``counts`` (int32 ``[batch]``, default all) its query
+    tokens in a padded batch.  ``mask`` None, or ``"causal"``: the last query
+    token sits at the sequence's last key.  Rows that see no key, and rows
+    behind ``counts``, are zero.
+    """
+    if mask is not None and not (isinstance(mask, str) and mask == "causal"):
+        raise ValueError(f"quantized_cache_attention: mask must be None or 'causal', got {mask!r}")
+    if cache.bits != 4:
+        raise ValueError(f"quantized_cache_attention: the cache must hold 4-bit codes, it holds {cache.bits}-bit "
+                         "ones (quantized_cache_fetch reads them back for the dense attention)")
+    q, qs = _rows(q, (None, None, None, cache.head_dim), "quantized_cache_attention: q", cache)
+    batch, heads, tokens = q.shape[:3]
+    if heads % cache.kv_heads:
+        raise ValueError(f"quantized_cache_attention: {heads} query heads over {cache.kv_heads} cache heads")
+    n = _ints(lengths, (batch,), "quantized_cache_attention: lengths", cache)
+    cnt = None if counts is None else _ints(counts, (batch,), "quantized_cache_attention: counts", cache)
+    keep, table, stride, columns = _table(block_table, batch, "quantized_cache_attention", cache)
+    with _on(cache.device):
+        key = (batch, heads, tokens)
+        size = cache._workspaces.get(key)
+        if size is None:
+            size = cache._workspaces[key] = _native.load().phew_kv_attention_workspace(cache._struct, *key)
+        work = torch.empty(size, dtype=torch.uint8, device=cache.device) if size else None
+        o = torch.empty((batch, heads, tokens, cache.head_dim), dtype=q.dtype, device=cache.device)
+        _call("phew_kv_attention", cache, q.data_ptr(), qs, o.data_ptr(), batch, heads, tokens, n.data_ptr(),
+              None if cnt is None else cnt.data_ptr(), table, stride, columns, float(scale),
+              1 if mask is not None else 0, None if work is None else work.data_ptr(), size)
+    del keep, work
+    return _core().array._wrap(o)

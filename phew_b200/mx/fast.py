@@ -7,6 +7,10 @@
   ``emit/codegen.py:413-419``);
 * ``scaled_dot_product_attention`` -> the tcgen05 flash-attention kernel
   (replaces ``mx.fast.scaled_dot_product_attention``, ``emit/codegen.py:421-426``);
+* ``QuantizedKVCache`` with ``quantized_cache_update`` / ``quantized_cache_fetch``
+  / ``quantized_cache_attention`` -> ``phew_kv_*`` (the k and v of
+  ``mx.fast.quantized_scaled_dot_product_attention``, ``emit/codegen.py:428-449``,
+  kept in pages between calls);
 * ``cuda_kernel`` -> :class:`phew_b200.kernel.CudaKernel`, the analogue of
   ``mx.fast.metal_kernel`` (``ir/importer.py:55-94``) and of MLX's own
   ``mx.fast.cuda_kernel`` (listed in phew ``ir/op_registry.py:324-329``).
@@ -18,6 +22,12 @@
 from __future__ import annotations
 
 from ..kernel import CudaKernel
+from ..kv_cache import (  # noqa: F401
+    QuantizedKVCache,
+    quantized_cache_attention,
+    quantized_cache_fetch,
+    quantized_cache_update,
+)
 
 _kernels: dict[tuple, CudaKernel] = {}
 

@@ -216,7 +216,11 @@ def error_flag():
 
 
 def check_device_errors() -> None:
-    """Raise if any kernel reported a timed-out wait (synchronises)."""
+    """Raise if any kernel reported a timed-out wait, or a kernel of the
+    quantised cache a position or page outside the cache (synchronises)."""
+    from .kv_cache import check_cache_errors
+
+    check_cache_errors()
     f = error_flag()
     code = int(f.item())
     if code:
