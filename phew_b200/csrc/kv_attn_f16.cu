@@ -1,0 +1,12 @@
+// Attention of few query rows over a 4-bit cache: the f16 kernels.
+#define PHEW_KV_ATTN_TYPE f16
+#include "kv_attn.cuh"
+
+namespace phew {
+namespace kv {
+
+template size_t attn_bytes<PHEW_KV_ATTN_TYPE>(int, int, int64_t);
+template int run_attn<PHEW_KV_ATTN_TYPE>(const AttnParams&, void*, cudaStream_t);
+
+}  // namespace kv
+}  // namespace phew

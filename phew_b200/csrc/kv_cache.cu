@@ -20,6 +20,39 @@ namespace kv {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int64_t kMaxRows = (1ll << 31) - (1 << 16);  // row numbers of a block past the last one stay 32-bit
+
+// Eight consecutive elements of a token row: one thread's share.
+template <typename T> struct alignas(16) Eight {
+  T v[8];
+};
+
+template <typename T> __device__ __forceinline__ Eight<T> load8(const T* p) {
+  Eight<T> e;
+  const uint4* q = reinterpret_cast<const uint4*>(p);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(&e)[i] = __ldg(q + i);
+  return e;
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const Eight<T>& e) {
+  uint4* q = reinterpret_cast<uint4*>(p);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) q[i] = reinterpret_cast<const uint4*>(&e)[i];
+}
+
+// A row number in [0, 2^31) of a [batch][kv_heads][n] array, taken apart.
+struct RowSplit {
+  FastDiv by_n, by_heads;
+};
+__device__ __forceinline__ void split_row(const RowSplit& s, int row, int& b, int& h, int& i) {
+  const int bh = static_cast<int>(div_by(s.by_n, static_cast<uint32_t>(row)));
+  i = row - bh * static_cast<int>(s.by_n.d);
+  b = static_cast<int>(div_by(s.by_heads, static_cast<uint32_t>(bh)));
+  h = bh - b * static_cast<int>(s.by_heads.d);
+}
+
+// Token rows a thread works on at once: their loads are in flight together.
+constexpr int kRows = 4;
 
 struct UpdateParams {
   Cache c;
@@ -28,55 +61,112 @@ struct UpdateParams {
   void* dense[2];        // values written back, [batch][kv_heads][tokens][D]; null: none
   const int32_t* offsets;
   const int32_t* counts;  // null: all `tokens`
-  int batch, tokens;
+  RowSplit split;
+  int rows, tokens;
   int* error_flag;
 };
 
-// One thread per group of one token row: the simplest right form.
-template <typename T>
+// Codes of eight values.  (x - bias) / scale is taken as a product with the
+// reciprocal, which lies within 3 roundings (q 2^-22.4) of the IEEE quotient:
+// only where that could cross a border between two codes, or is no number,
+// are the eight divided again, so the codes are phew_quantize's bit for bit
+// at a third of the instructions of eight divisions.
+template <int BITS>
+__device__ __forceinline__ void codes8(const float* x, float bi, float sc, float* q) {
+  constexpr float top = (1 << BITS) - 1;
+  constexpr float near = 0.5f - (BITS == 4 ? 1.f / (1 << 17) : 1.f / (1 << 13));  // > 3 roundings of 2 top
+  const float inv = __frcp_rn(sc);
+  bool sure = true;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float v = __fmul_rn(x[e] - bi, inv);
+    const float r = __fadd_rn(__fadd_rn(v, 12582912.f), -12582912.f);  // nearest even, |v| < 2^22
+    sure = sure && fabsf(v - r) < near;
+    q[e] = fminf(fmaxf(r, 0.f), top);
+  }
+  if (!sure) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = fminf(fmaxf(rintf(__fdiv_rn(x[e] - bi, sc)), 0.f), top);
+  }
+}
+
+// Bound by HBM: one 16-byte load of x per eight 16-bit values, 4 or 8 bytes of
+// codes out (and 16 of values).  Eight values to a thread make a code word of
+// one thread and a group of 4, 8 or 16 neighbouring lanes.
+template <typename T, int BITS, int G>
 __global__ void __launch_bounds__(kThreads) update_kernel(const UpdateParams p) {
-  const int g = p.c.group, ng = p.c.head_dim / g, per = 32 / p.c.bits, top = (1 << p.c.bits) - 1;
-  const int64_t rows = static_cast<int64_t>(p.batch) * p.c.map.kv_heads * p.tokens;
-  const int64_t total = 2 * rows * ng;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int side = i >= rows * ng;
-    const int64_t j = i - side * rows * ng;
-    const int64_t row = j / ng;
-    const int grp = static_cast<int>(j % ng);
-    const int tok = static_cast<int>(row % p.tokens);
-    const int h = static_cast<int>(row / p.tokens % p.c.map.kv_heads);
-    const int b = static_cast<int>(row / p.tokens / p.c.map.kv_heads);
-    const int count = p.counts ? clamp_count(p.counts[b], p.tokens) : p.tokens;
-    T* dense = p.dense[side] ? static_cast<T*>(p.dense[side]) + row * p.c.head_dim + grp * g : nullptr;
-    if (tok >= count) {
-      if (dense)
-        for (int e = 0; e < g; ++e) dense[e] = from_f32<T>(0.f);
+  constexpr int LG = G / 8;
+  constexpr float top = (1 << BITS) - 1;
+  const int side = blockIdx.y;
+  const int lanes = p.c.head_dim / 8;                  // threads to a row
+  const int per_pass = kThreads / lanes;               // rows to a pass of the block
+  const int c = threadIdx.x & (lanes - 1);             // which eight of the row
+  const int row0 = blockIdx.x * (per_pass * kRows) + static_cast<int>(threadIdx.x) / lanes;
+  const int ng = p.c.head_dim / G;
+  const T* xs = static_cast<const T*>(p.x[side]);
+  Eight<T> in[kRows];
+  int b[kRows], h[kRows], tok[kRows];
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const int row = row0 + u * per_pass;
+    if (row < p.rows) {
+      split_row(p.split, row, b[u], h[u], tok[u]);
+      in[u] = load8(xs + b[u] * p.st[side][2] + h[u] * p.st[side][1] + tok[u] * p.st[side][0] + c * 8);
+    } else {
+      tok[u] = -1;
+      in[u] = Eight<T>{};
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    float x[8], q[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = to_f32(in[u].v[e]);
+    float lo = x[0], hi = x[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) {
+      lo = fminf(lo, x[e]);
+      hi = fmaxf(hi, x[e]);
+    }
+#pragma unroll
+    for (int o = LG / 2; o > 0; o >>= 1) {  // a group's lanes lie side by side
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    if (tok[u] < 0) continue;
+    const int row = row0 + u * per_pass;
+    const int count = p.counts ? clamp_count(__ldg(p.counts + b[u]), p.tokens) : p.tokens;
+    T* dense = p.dense[side] ? static_cast<T*>(p.dense[side]) + static_cast<int64_t>(row) * p.c.head_dim + c * 8 : nullptr;
+    if (tok[u] >= count) {
+      if (dense) store8(dense, Eight<T>{});
       continue;
     }
-    const T* x = static_cast<const T*>(p.x[side]) + b * p.st[side][2] + h * p.st[side][1] + tok * p.st[side][0] + grp * g;
-    float lo = to_f32(x[0]), hi = lo;
-    for (int e = 1; e < g; ++e) {
-      lo = fminf(lo, to_f32(x[e]));
-      hi = fmaxf(hi, to_f32(x[e]));
-    }
-    const float sc = round_to<T>(fmaxf(__fdiv_rn(hi - lo, static_cast<float>(top)), 1e-8f));
+    const float sc = round_to<T>(fmaxf(__fdiv_rn(hi - lo, top), 1e-8f));
     const float bi = round_to<T>(lo);
-    const uint32_t at = row_of(p.c.map, b, h, static_cast<int64_t>(p.offsets[b]) + tok);
-    if (at == kNoRow)
+    codes8<BITS>(x, bi, sc, q);
+    const uint32_t at = row_of(p.c.map, b[u], h[u], static_cast<int64_t>(__ldg(p.offsets + b[u])) + tok[u]);
+    if (at == kNoRow) {
       atomicExch(p.error_flag, PHEW_ERR_INVALID);
-    else {
-      static_cast<T*>(p.c.scales[side])[static_cast<int64_t>(at) * ng + grp] = from_f32<T>(sc);
-      static_cast<T*>(p.c.biases[side])[static_cast<int64_t>(at) * ng + grp] = from_f32<T>(bi);
-    }
-    for (int w = 0; w < g / per; ++w) {
-      uint32_t word = 0;
-      for (int e = 0; e < per; ++e) {
-        const float q = fminf(fmaxf(rintf(__fdiv_rn(to_f32(x[w * per + e]) - bi, sc)), 0.f), static_cast<float>(top));
-        word |= static_cast<uint32_t>(q) << (e * p.c.bits);
-        if (dense) dense[w * per + e] = from_f32<T>(fmaf(sc, q, bi));
+    } else {
+      uint32_t w[BITS / 4] = {};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e * BITS / 32] |= static_cast<uint32_t>(q[e]) << (e * BITS % 32);
+      uint32_t* dst = p.c.codes[side] + (static_cast<int64_t>(at) * lanes + c) * (BITS / 4);
+      if (BITS == 4)
+        dst[0] = w[0];
+      else
+        *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[BITS / 4 - 1]);
+      if ((c & (LG - 1)) == 0) {
+        const int64_t s_at = static_cast<int64_t>(at) * ng + c / LG;
+        static_cast<T*>(p.c.scales[side])[s_at] = from_f32<T>(sc);
+        static_cast<T*>(p.c.biases[side])[s_at] = from_f32<T>(bi);
       }
-      if (at != kNoRow) p.c.codes[side][static_cast<int64_t>(at) * (p.c.head_dim / per) + grp * (g / per) + w] = word;
+    }
+    if (dense) {
+      Eight<T> out;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) out.v[e] = from_f32<T>(fmaf(sc, q[e], bi));
+      store8(dense, out);
     }
   }
 }
@@ -85,48 +175,97 @@ struct FetchParams {
   Cache c;
   void* dense[2];  // [batch][kv_heads][out_len][D]
   const int32_t* lengths;
-  int batch, out_len;
+  RowSplit split;
+  int rows;
   int* error_flag;
 };
 
-// One thread per word of codes.
-template <typename T>
+// Bound by HBM, mostly by the values written: eight codes (one or two words)
+// and their group's scale and bias to a thread, 16 bytes of 16-bit values out.
+template <typename T, int BITS>
 __global__ void __launch_bounds__(kThreads) fetch_kernel(const FetchParams p) {
-  const int per = 32 / p.c.bits, words = p.c.head_dim / per, top = (1 << p.c.bits) - 1;
-  const int ng = p.c.head_dim / p.c.group;
-  const int64_t rows = static_cast<int64_t>(p.batch) * p.c.map.kv_heads * p.out_len;
-  const int64_t total = 2 * rows * words;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int side = i >= rows * words;
-    const int64_t j = i - side * rows * words;
-    const int64_t row = j / words;
-    const int w = static_cast<int>(j % words);
-    const int pos = static_cast<int>(row % p.out_len);
-    const int h = static_cast<int>(row / p.out_len % p.c.map.kv_heads);
-    const int b = static_cast<int>(row / p.out_len / p.c.map.kv_heads);
-    T* dense = static_cast<T*>(p.dense[side]) + row * p.c.head_dim + w * per;
-    uint32_t at = kNoRow;
-    if (pos < p.lengths[b]) {
-      at = row_of(p.c.map, b, h, pos);
-      if (at == kNoRow) atomicExch(p.error_flag, PHEW_ERR_INVALID);
+  const int side = blockIdx.y;
+  const int lanes = p.c.head_dim / 8;
+  const int per_pass = kThreads / lanes;
+  const int c = threadIdx.x & (lanes - 1);
+  const int row0 = blockIdx.x * (per_pass * kRows) + static_cast<int>(threadIdx.x) / lanes;
+  const int ng = p.c.head_dim / p.c.group, grp = c * 8 / p.c.group;
+  uint32_t at[kRows];
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const int row = row0 + u * per_pass;
+    at[u] = kNoRow;
+    if (row < p.rows) {
+      int b, h, pos;
+      split_row(p.split, row, b, h, pos);
+      if (pos < __ldg(p.lengths + b)) {
+        at[u] = row_of(p.c.map, b, h, pos);
+        if (at[u] == kNoRow) atomicExch(p.error_flag, PHEW_ERR_INVALID);
+      }
     }
-    if (at == kNoRow) {
-      for (int e = 0; e < per; ++e) dense[e] = from_f32<T>(0.f);
-      continue;
+  }
+  uint32_t w[kRows][BITS / 4];
+  T sc[kRows], bi[kRows];
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    if (at[u] == kNoRow) continue;
+    const uint32_t* src = p.c.codes[side] + (static_cast<int64_t>(at[u]) * lanes + c) * (BITS / 4);
+    if (BITS == 4) {
+      w[u][0] = __ldg(src);
+    } else {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
+      w[u][0] = v.x;
+      w[u][BITS / 4 - 1] = v.y;
     }
-    const int grp = w * per / p.c.group;
-    const float sc = to_f32(static_cast<const T*>(p.c.scales[side])[static_cast<int64_t>(at) * ng + grp]);
-    const float bi = to_f32(static_cast<const T*>(p.c.biases[side])[static_cast<int64_t>(at) * ng + grp]);
-    const uint32_t word = p.c.codes[side][static_cast<int64_t>(at) * words + w];
-    for (int e = 0; e < per; ++e)
-      dense[e] = from_f32<T>(fmaf(sc, static_cast<float>((word >> (e * p.c.bits)) & top), bi));
+    const int64_t s_at = static_cast<int64_t>(at[u]) * ng + grp;
+    sc[u] = static_cast<const T*>(p.c.scales[side])[s_at];
+    bi[u] = static_cast<const T*>(p.c.biases[side])[s_at];
+  }
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const int row = row0 + u * per_pass;
+    if (row >= p.rows) continue;
+    Eight<T> out{};
+    if (at[u] != kNoRow) {
+      const float s = to_f32(sc[u]), z = to_f32(bi[u]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        out.v[e] = from_f32<T>(fmaf(s, static_cast<float>((w[u][e * BITS / 32] >> (e * BITS % 32)) & ((1 << BITS) - 1)), z));
+    }
+    store8(static_cast<T*>(p.dense[side]) + static_cast<int64_t>(row) * p.c.head_dim + c * 8, out);
   }
 }
 
-unsigned grid_for(int64_t threads) {
-  const int64_t blocks = (threads + kThreads - 1) / kThreads, cap = static_cast<int64_t>(sm_count_current()) * 64;
-  return static_cast<unsigned>(blocks < cap ? blocks : cap);
+// Blocks along x for `rows` token rows of a side.
+dim3 grid_for(int64_t rows, int head_dim) {
+  const int64_t per_block = static_cast<int64_t>(kThreads / (head_dim / 8)) * kRows;
+  return dim3(static_cast<unsigned>((rows + per_block - 1) / per_block), 2);
+}
+
+template <typename T, int BITS> void launch_update(const UpdateParams& p, cudaStream_t st) {
+  const dim3 grid = grid_for(p.rows, p.c.head_dim);
+  switch (p.c.group) {
+    case 32: update_kernel<T, BITS, 32><<<grid, kThreads, 0, st>>>(p); break;
+    case 64: update_kernel<T, BITS, 64><<<grid, kThreads, 0, st>>>(p); break;
+    default: update_kernel<T, BITS, 128><<<grid, kThreads, 0, st>>>(p); break;
+  }
+}
+
+template <typename T> int update_typed(const UpdateParams& p, cudaStream_t st) {
+  if (p.c.bits == 4)
+    launch_update<T, 4>(p, st);
+  else
+    launch_update<T, 8>(p, st);
+  return launch_status("kv update_kernel");
+}
+
+template <typename T> int fetch_typed(const FetchParams& p, cudaStream_t st) {
+  const dim3 grid = grid_for(p.rows, p.c.head_dim);
+  if (p.c.bits == 4)
+    fetch_kernel<T, 4><<<grid, kThreads, 0, st>>>(p);
+  else
+    fetch_kernel<T, 8><<<grid, kThreads, 0, st>>>(p);
+  return launch_status("kv fetch_kernel");
 }
 
 }  // namespace
@@ -187,7 +326,8 @@ extern "C" int phew_kv_update(const phew_kv_cache* cache, const void* k, const v
   if (int s = kv::make_cache(cache, block_table, table_stride, columns, batch, "phew_kv_update", &p.c)) return s;
   PHEW_REQUIRE(k && v && k_strides && v_strides && offsets && error_flag, "phew_kv_update: null pointer");
   PHEW_REQUIRE((k_out == nullptr) == (v_out == nullptr), "phew_kv_update: k_out and v_out go together");
-  PHEW_REQUIRE(tokens > 0 && tokens < (1ll << 31), "phew_kv_update: bad token count");
+  PHEW_REQUIRE(tokens > 0 && tokens < (1ll << 31) && batch * cache->kv_heads < kv::kMaxRows / tokens,
+               "phew_kv_update: bad token count (batch * kv_heads * tokens must stay below 2^31 - 2^16)");
   const int size = dtype_bytes(cache->dtype);
   for (const void* q : {k, v, static_cast<const void*>(k_out), static_cast<const void*>(v_out)})
     PHEW_REQUIRE((reinterpret_cast<uintptr_t>(q) & 15) == 0, "phew_kv_update: pointers must be 16-byte aligned");
@@ -204,17 +344,16 @@ extern "C" int phew_kv_update(const phew_kv_cache* cache, const void* k, const v
   p.dense[1] = v_out;
   p.offsets = offsets;
   p.counts = counts;
-  p.batch = static_cast<int>(batch);
+  p.split = {kv::fast_div(static_cast<uint32_t>(tokens)), kv::fast_div(static_cast<uint32_t>(cache->kv_heads))};
+  p.rows = static_cast<int>(batch * cache->kv_heads * tokens);
   p.tokens = static_cast<int>(tokens);
   p.error_flag = error_flag;
-  const unsigned grid = kv::grid_for(2 * batch * tokens * cache->kv_heads * (cache->head_dim / cache->group_size));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (cache->dtype) {
-    case PHEW_F32: kv::update_kernel<float><<<grid, kv::kThreads, 0, st>>>(p); break;
-    case PHEW_F16: kv::update_kernel<f16><<<grid, kv::kThreads, 0, st>>>(p); break;
-    default: kv::update_kernel<bf16><<<grid, kv::kThreads, 0, st>>>(p); break;
+    case PHEW_F32: return kv::update_typed<float>(p, st);
+    case PHEW_F16: return kv::update_typed<f16>(p, st);
+    default: return kv::update_typed<bf16>(p, st);
   }
-  return launch_status("kv update_kernel");
 }
 
 extern "C" int phew_kv_fetch(const phew_kv_cache* cache, void* k_out, void* v_out, int64_t batch, int64_t out_len,
@@ -223,21 +362,20 @@ extern "C" int phew_kv_fetch(const phew_kv_cache* cache, void* k_out, void* v_ou
   kv::FetchParams p;
   if (int s = kv::make_cache(cache, block_table, table_stride, columns, batch, "phew_kv_fetch", &p.c)) return s;
   PHEW_REQUIRE(k_out && v_out && lengths && error_flag, "phew_kv_fetch: null pointer");
-  PHEW_REQUIRE(out_len > 0 && out_len < (1ll << 31), "phew_kv_fetch: bad output length");
+  PHEW_REQUIRE(out_len > 0 && out_len < (1ll << 31) && batch * cache->kv_heads < kv::kMaxRows / out_len,
+               "phew_kv_fetch: bad output length (batch * kv_heads * length must stay below 2^31 - 2^16)");
   for (const void* q : {k_out, v_out})
     PHEW_REQUIRE((reinterpret_cast<uintptr_t>(q) & 15) == 0, "phew_kv_fetch: pointers must be 16-byte aligned");
   p.dense[0] = k_out;
   p.dense[1] = v_out;
   p.lengths = lengths;
-  p.batch = static_cast<int>(batch);
-  p.out_len = static_cast<int>(out_len);
+  p.split = {kv::fast_div(static_cast<uint32_t>(out_len)), kv::fast_div(static_cast<uint32_t>(cache->kv_heads))};
+  p.rows = static_cast<int>(batch * cache->kv_heads * out_len);
   p.error_flag = error_flag;
-  const unsigned grid = kv::grid_for(2 * batch * out_len * cache->kv_heads * (cache->head_dim * cache->bits / 32));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (cache->dtype) {
-    case PHEW_F32: kv::fetch_kernel<float><<<grid, kv::kThreads, 0, st>>>(p); break;
-    case PHEW_F16: kv::fetch_kernel<f16><<<grid, kv::kThreads, 0, st>>>(p); break;
-    default: kv::fetch_kernel<bf16><<<grid, kv::kThreads, 0, st>>>(p); break;
+    case PHEW_F32: return kv::fetch_typed<float>(p, st);
+    case PHEW_F16: return kv::fetch_typed<f16>(p, st);
+    default: return kv::fetch_typed<bf16>(p, st);
   }
-  return launch_status("kv fetch_kernel");
 }
