@@ -35,6 +35,7 @@
 // the combine kernel joins in a fixed order.
 #pragma once
 
+#include <atomic>
 #include <type_traits>
 
 #include "kv_cache.cuh"
@@ -317,6 +318,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
     if (threadIdx.x < 2) p.meta[2 * blockIdx.x + threadIdx.x] = -1;
     return;
   }
+  asm volatile("griddepcontrol.launch_dependents;");  // the combine kernel may be set up from here on; it waits for this one
   int64_t x = total * blockIdx.x / n;
   const int64_t x_end = total * (blockIdx.x + 1) / n;
   // the entry that tile x belongs to: the first whose tiles, with those before it, pass x / kv_heads
@@ -766,6 +768,7 @@ template <typename S, typename T>
 __global__ void __launch_bounds__(S::D) combine_kernel(const AttnParams p, int n) {
   constexpr int D = S::D, ROWS = S::ROWS;
   const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // attn_kernel is done and its partials are visible
   const int64_t seg = p.meta[2 * c + 1];
   if (seg < 0) return;
   const int kv_heads = p.c.map.kv_heads;
@@ -821,6 +824,18 @@ template <typename S> AttnPlan plan_of() {
   return a;
 }
 
+// Dynamic shared memory of a kernel above 48 KB, allowed once per device (bit d: done on device d).
+using SmemAllowed = std::atomic<uint64_t>;
+template <typename K> int allow_smem(SmemAllowed& done, K* kernel, int bytes) {
+  int dev = 0;
+  PHEW_CHECK_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && (done.load(std::memory_order_relaxed) & bit)) return PHEW_OK;
+  PHEW_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return PHEW_OK;
+}
+
 template <typename S, typename T> int launch_attn(AttnParams p, void* workspace, cudaStream_t st) {
   const AttnPlan a = plan_of<S>();
   const int64_t rows = static_cast<int64_t>(p.tokens) * p.per;
@@ -830,10 +845,21 @@ template <typename S, typename T> int launch_attn(AttnParams p, void* workspace,
   p.meta = static_cast<int64_t*>(workspace);
   p.part = reinterpret_cast<float*>(p.meta + 2 * a.grid);
   p.part_ml = p.part + static_cast<size_t>(a.grid) * 2 * S::ROWS * S::D;
-  PHEW_CHECK_CUDA(cudaFuncSetAttribute(attn_kernel<S, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+  static SmemAllowed allowed;
+  if (int s = allow_smem(allowed, attn_kernel<S, T>, S::SMEM)) return s;
   attn_kernel<S, T><<<a.grid, kWarps * 32, S::SMEM, st>>>(p);
   if (int s = launch_status("kv attn_kernel")) return s;
-  combine_kernel<S, T><<<dim3(a.grid, S::ROWS), S::D, 0, st>>>(p, a.grid);
+  // a programmatic dependent: set up while attn_kernel runs
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.grid, S::ROWS);
+  cfg.blockDim = dim3(S::D);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  PHEW_CHECK_CUDA(cudaLaunchKernelEx(&cfg, combine_kernel<S, T>, p, static_cast<int>(a.grid)));
   return launch_status("kv combine_kernel");
 }
 

@@ -9,28 +9,17 @@ a step captured into a CUDA graph replays with new ones.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 
 import torch
 
 from . import _native
 from . import dtypes as dt
+from .mx import core
 
 _error_flags: dict[int, torch.Tensor] = {}
-
-
-def _core():
-    from .mx import core
-
-    return core
-
-
-def _on(device: torch.device):
-    """Makes `device` current when it is not (kernels launch on the current one)."""
-    if torch.cuda.current_device() == device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+_Strides = ctypes.c_int64 * 3
 
 
 def cache_error_flag(device: torch.device) -> torch.Tensor:
@@ -70,10 +59,9 @@ class QuantizedKVCache:
     """
 
     __slots__ = ("keys", "values", "pages", "kv_heads", "page_size", "head_dim", "group_size", "bits",
-                 "dtype", "device", "_struct", "_workspaces")
+                 "dtype", "device", "_torch_dtype", "_unit", "_struct", "_flag")
 
     def __init__(self, keys, values, *, group_size: int = 64, bits: int = 4) -> None:
-        core = _core()
         if len(keys) != 3 or len(values) != 3:
             raise ValueError("QuantizedKVCache: keys and values are (codes, scales, biases) each")
         parts = [a if isinstance(a, core.array) else core.array(a) for a in (*keys, *values)]
@@ -117,13 +105,13 @@ class QuantizedKVCache:
         self.device = codes._t.device
         self._struct = _native.KVCache(*(ctypes.c_void_p(a._t.data_ptr()) for a in parts), self.pages,
                                        self.page_size, self.kv_heads, dim, g, nb, self.dtype.code)
-        self._workspaces: dict[tuple, int] = {}
+        self._torch_dtype, self._unit = self.dtype.torch, 16 // self.dtype.size
+        self._flag = cache_error_flag(self.device).data_ptr()
 
     @classmethod
     def zeros(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, dtype="bfloat16", *,
               group_size: int = 64, bits: int = 4) -> "QuantizedKVCache":
         """A cache of its own arrays, all zero."""
-        core = _core()
         if int(bits) not in (4, 8) or int(group_size) not in (32, 64, 128):
             raise ValueError("QuantizedKVCache: bits must be 4 or 8, group_size 32, 64 or 128")
         d, rows = dt.from_any(dtype), (int(pages), int(kv_heads), int(page_size))
@@ -137,18 +125,23 @@ class QuantizedKVCache:
         return cls(side(), side(), group_size=group_size, bits=bits)
 
 
-def _ints(x, shape, what: str, cache: QuantizedKVCache) -> torch.Tensor:
-    """An int32 device array of `shape` (a host sequence is copied in)."""
-    core = _core()
-    a = x if isinstance(x, core.array) else core.array(x, None if isinstance(x, torch.Tensor) else core.int32)
-    t = a._t
+def _as_ints(x) -> torch.Tensor:
+    """The tensor of an array, or of a host sequence copied in as int32."""
+    if isinstance(x, core.array):
+        return x._t
+    return core.array(x, None if isinstance(x, torch.Tensor) else core.int32)._t
+
+
+def _ints(x, batch: int, what: str, cache: QuantizedKVCache) -> torch.Tensor:
+    """An int32 [batch] array on the cache's device."""
+    t = _as_ints(x)
     if t.dtype != torch.int32:
-        raise TypeError(f"{what} must be int32, got {a.dtype.name}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{what} shape {tuple(t.shape)} != {shape}")
+        raise TypeError(f"{what} must be int32, got {dt.from_any(t.dtype).name}")
+    if t.shape != (batch,):
+        raise ValueError(f"{what} shape {tuple(t.shape)} != {(batch,)}")
     if t.device != cache.device:
         raise ValueError(f"{what} lies on another device than the cache")
-    return t if t.is_contiguous() else core.contiguous_copy(a)._t
+    return t if t.is_contiguous() else core.contiguous_copy(core.array._wrap(t))._t
 
 
 def _table(block_table, batch: int, what: str, cache: QuantizedKVCache):
@@ -158,49 +151,80 @@ def _table(block_table, batch: int, what: str, cache: QuantizedKVCache):
             raise ValueError(f"{what}: without a block_table the cache needs a page for each of the {batch} "
                              f"sequences, it has {cache.pages}")
         return None, None, 0, 1
-    core = _core()
-    a = block_table
-    if not isinstance(a, core.array):
-        a = core.array(a, None if isinstance(a, torch.Tensor) else core.int32)
-    t = a._t
+    t = _as_ints(block_table)
     if t.dtype != torch.int32:
-        raise TypeError(f"{what}: block_table must be int32, got {a.dtype.name}")
+        raise TypeError(f"{what}: block_table must be int32, got {dt.from_any(t.dtype).name}")
     if t.dim() != 2 or t.shape[0] != batch or t.shape[1] == 0:
         raise ValueError(f"{what}: block_table shape {tuple(t.shape)} is not [{batch}, columns]")
     if t.device != cache.device:
         raise ValueError(f"{what}: block_table lies on another device than the cache")
-    if t.stride(1) != 1 and t.shape[1] > 1 or t.stride(0) < 0:
-        t = core.contiguous_copy(a)._t
-    return t, t.data_ptr(), t.stride(0), t.shape[1]
+    stride, unit = t.stride()
+    if unit != 1 and t.shape[1] > 1:
+        t = core.contiguous_copy(core.array._wrap(t))._t
+        stride = t.shape[1]
+    return t, t.data_ptr(), stride, t.shape[1]
 
 
-def _rows(x, shape, what: str, cache: QuantizedKVCache):
+@functools.lru_cache(maxsize=1024)
+def _strides(token: int, head: int, batch: int):
+    return _Strides(token, head, batch)
+
+
+def _rows(x, what: str, cache: QuantizedKVCache):
     """(tensor, strides {token, head, batch}) of a [batch, heads, tokens, head_dim]
     view that the kernels read in place: unit stride along the head dimension
     and 16-byte aligned rows; anything else is copied first."""
-    core = _core()
-    a = core.asarray_device(x, contiguous=False)
-    if a.dtype is not cache.dtype:
-        raise TypeError(f"{what} must be {cache.dtype.name} like the cache, got {a.dtype.name}")
-    t = a._t
-    if t.dim() != 4 or any(w is not None and n != w for n, w in zip(t.shape, shape)):
-        raise ValueError(f"{what} shape {tuple(t.shape)} is not "
-                         f"[{', '.join('*' if w is None else str(w) for w in shape)}]")
+    t = x._t if isinstance(x, core.array) else core.asarray_device(x, contiguous=False)._t
+    if t.dtype != cache._torch_dtype:
+        raise TypeError(f"{what} must be {cache.dtype.name} like the cache, got {dt.from_any(t.dtype).name}")
+    if t.dim() != 4 or t.shape[3] != cache.head_dim:
+        raise ValueError(f"{what} shape {tuple(t.shape)} is not [batch, heads, tokens, {cache.head_dim}]")
     if t.numel() == 0:
         raise ValueError(f"{what} is empty")
     if t.device != cache.device:
         raise ValueError(f"{what} lies on another device than the cache")
-    unit = 16 // t.element_size()
-    s = t.stride()
-    if s[3] != 1 or s[0] % unit or s[1] % unit or s[2] % unit or t.data_ptr() % 16:
+    b, h, n, unit = t.stride()
+    if unit != 1 or (b | h | n) % cache._unit or t.data_ptr() % 16:
         t = core.contiguous_copy(core.array._wrap(t))._t
-        s = t.stride()
-    return t, (ctypes.c_int64 * 3)(s[2], s[1], s[0])
+        b, h, n, unit = t.stride()
+    return t, _strides(n, h, b)
+
+
+def _stream(cache: QuantizedKVCache) -> int:
+    return torch.cuda.current_stream(cache.device).cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+if _raw_stream is not None:  # the same stream without a Stream object around it
+
+    def _stream(cache: QuantizedKVCache) -> int:  # noqa: F811
+        return _raw_stream(cache.device.index)
+
+
+_functions: dict[str, object] = {}
 
 
 def _call(name: str, cache: QuantizedKVCache, *args) -> None:
-    _native.call(name, cache._struct, *args, cache_error_flag(cache.device).data_ptr(),
-                 torch.cuda.current_stream(cache.device).cuda_stream)
+    """Calls an entry point on the cache's device and current stream there."""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(_native.load(), name)
+    if torch.cuda.current_device() == cache.device.index:
+        status = fn(cache._struct, *args, cache._flag, _stream(cache))
+    else:
+        with torch.cuda.device(cache.device):  # kernels launch on the current device
+            status = fn(cache._struct, *args, cache._flag, _stream(cache))
+    if status:
+        _native.check(status, name)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace(device: int, kv_heads: int, head_dim: int, group_size: int, dtype: int, batch: int, heads: int,
+               tokens: int) -> int:
+    """Scratch bytes of an attention call; they depend on its sizes and the device alone."""
+    c = _native.KVCache(kv_heads=kv_heads, head_dim=head_dim, group_size=group_size, dtype=dtype)
+    with torch.cuda.device(device):
+        return int(_native.load().phew_kv_attention_workspace(c, batch, heads, tokens))
 
 
 def quantized_cache_update(cache: QuantizedKVCache, k, v, offsets, *, block_table=None, counts=None,
@@ -217,23 +241,26 @@ def quantized_cache_update(cache: QuantizedKVCache, k, v, offsets, *, block_tabl
     A position or page outside the cache is left unwritten and reported by
     ``ops.check_device_errors``.
     """
-    k, ks = _rows(k, (None, cache.kv_heads, None, cache.head_dim), "quantized_cache_update: k", cache)
-    v, vs = _rows(v, tuple(k.shape), "quantized_cache_update: v", cache)
-    batch, tokens = k.shape[0], k.shape[2]
-    off = _ints(offsets, (batch,), "quantized_cache_update: offsets", cache)
-    cnt = None if counts is None else _ints(counts, (batch,), "quantized_cache_update: counts", cache)
+    k, ks = _rows(k, "quantized_cache_update: k", cache)
+    v, vs = _rows(v, "quantized_cache_update: v", cache)
+    shape = k.shape
+    batch, heads, tokens, _ = shape
+    if heads != cache.kv_heads:
+        raise ValueError(f"quantized_cache_update: k shape {tuple(shape)} does not have the cache's "
+                         f"{cache.kv_heads} heads")
+    if v.shape != shape:
+        raise ValueError(f"quantized_cache_update: v shape {tuple(v.shape)} != k's {tuple(shape)}")
+    off = _ints(offsets, batch, "quantized_cache_update: offsets", cache)
+    cnt = None if counts is None else _ints(counts, batch, "quantized_cache_update: counts", cache)
     keep, table, stride, columns = _table(block_table, batch, "quantized_cache_update", cache)
-    with _on(cache.device):
-        ko = torch.empty(k.shape, dtype=k.dtype, device=cache.device) if fetch else None
-        vo = torch.empty(k.shape, dtype=k.dtype, device=cache.device) if fetch else None
-        _call("phew_kv_update", cache, k.data_ptr(), v.data_ptr(), ks, vs, batch, tokens, off.data_ptr(),
-              None if cnt is None else cnt.data_ptr(), table, stride, columns,
-              ko.data_ptr() if fetch else None, vo.data_ptr() if fetch else None)
+    out = None
+    if fetch:
+        out = (k.new_empty(shape), k.new_empty(shape))
+    _call("phew_kv_update", cache, k.data_ptr(), v.data_ptr(), ks, vs, batch, tokens, off.data_ptr(),
+          None if cnt is None else cnt.data_ptr(), table, stride, columns,
+          out[0].data_ptr() if fetch else None, out[1].data_ptr() if fetch else None)
     del keep
-    if not fetch:
-        return None
-    wrap = _core().array._wrap
-    return wrap(ko), wrap(vo)
+    return (core.array._wrap(out[0]), core.array._wrap(out[1])) if fetch else None
 
 
 def quantized_cache_fetch(cache: QuantizedKVCache, lengths, *, block_table=None, max_length: int | None = None):
@@ -242,23 +269,19 @@ def quantized_cache_fetch(cache: QuantizedKVCache, lengths, *, block_table=None,
     (``mx.dequantize``'s values), zero behind a sequence.  ``max_length``
     defaults to what a sequence's pages hold; longer sequences are cut there.
     """
-    core = _core()
-    if not isinstance(lengths, (core.array, torch.Tensor)):
-        lengths = core.array(lengths, core.int32)
-    if len(lengths.shape) != 1 or lengths.shape[0] == 0:
-        raise ValueError(f"quantized_cache_fetch: lengths shape {tuple(lengths.shape)} is not [batch]")
-    batch = lengths.shape[0]
-    n = _ints(lengths, (batch,), "quantized_cache_fetch: lengths", cache)
+    n = _as_ints(lengths)
+    if n.dim() != 1 or n.shape[0] == 0:
+        raise ValueError(f"quantized_cache_fetch: lengths shape {tuple(n.shape)} is not [batch]")
+    batch = n.shape[0]
+    n = _ints(n, batch, "quantized_cache_fetch: lengths", cache)
     keep, table, stride, columns = _table(block_table, batch, "quantized_cache_fetch", cache)
     out_len = columns * cache.page_size if max_length is None else int(max_length)
     if out_len <= 0:
         raise ValueError(f"quantized_cache_fetch: max_length must be positive, got {max_length}")
     shape = (batch, cache.kv_heads, out_len, cache.head_dim)
-    with _on(cache.device):
-        k = torch.empty(shape, dtype=cache.dtype.torch, device=cache.device)
-        v = torch.empty(shape, dtype=cache.dtype.torch, device=cache.device)
-        _call("phew_kv_fetch", cache, k.data_ptr(), v.data_ptr(), batch, out_len, n.data_ptr(), table, stride,
-              columns)
+    one = cache.keys[1]._t
+    k, v = one.new_empty(shape), one.new_empty(shape)
+    _call("phew_kv_fetch", cache, k.data_ptr(), v.data_ptr(), batch, out_len, n.data_ptr(), table, stride, columns)
     del keep
     return core.array._wrap(k), core.array._wrap(v)
 
@@ -280,22 +303,20 @@ def quantized_cache_attention(q, cache: QuantizedKVCache, lengths, *, block_tabl
     if cache.bits != 4:
         raise ValueError(f"quantized_cache_attention: the cache must hold 4-bit codes, it holds {cache.bits}-bit "
                          "ones (quantized_cache_fetch reads them back for the dense attention)")
-    q, qs = _rows(q, (None, None, None, cache.head_dim), "quantized_cache_attention: q", cache)
-    batch, heads, tokens = q.shape[:3]
+    q, qs = _rows(q, "quantized_cache_attention: q", cache)
+    shape = q.shape
+    batch, heads, tokens, _ = shape
     if heads % cache.kv_heads:
         raise ValueError(f"quantized_cache_attention: {heads} query heads over {cache.kv_heads} cache heads")
-    n = _ints(lengths, (batch,), "quantized_cache_attention: lengths", cache)
-    cnt = None if counts is None else _ints(counts, (batch,), "quantized_cache_attention: counts", cache)
+    n = _ints(lengths, batch, "quantized_cache_attention: lengths", cache)
+    cnt = None if counts is None else _ints(counts, batch, "quantized_cache_attention: counts", cache)
     keep, table, stride, columns = _table(block_table, batch, "quantized_cache_attention", cache)
-    with _on(cache.device):
-        key = (batch, heads, tokens)
-        size = cache._workspaces.get(key)
-        if size is None:
-            size = cache._workspaces[key] = _native.load().phew_kv_attention_workspace(cache._struct, *key)
-        work = torch.empty(size, dtype=torch.uint8, device=cache.device) if size else None
-        o = torch.empty((batch, heads, tokens, cache.head_dim), dtype=q.dtype, device=cache.device)
-        _call("phew_kv_attention", cache, q.data_ptr(), qs, o.data_ptr(), batch, heads, tokens, n.data_ptr(),
-              None if cnt is None else cnt.data_ptr(), table, stride, columns, float(scale),
-              1 if mask is not None else 0, None if work is None else work.data_ptr(), size)
+    size = _workspace(cache.device.index, cache.kv_heads, cache.head_dim, cache.group_size, cache.dtype.code, batch,
+                      heads, tokens)
+    work = n.new_empty(size // 4)
+    o = q.new_empty(shape)
+    _call("phew_kv_attention", cache, q.data_ptr(), qs, o.data_ptr(), batch, heads, tokens, n.data_ptr(),
+          None if cnt is None else cnt.data_ptr(), table, stride, columns, scale, 0 if mask is None else 1,
+          work.data_ptr(), size)
     del keep, work
-    return _core().array._wrap(o)
+    return core.array._wrap(o)

@@ -22,12 +22,21 @@
 from __future__ import annotations
 
 from ..kernel import CudaKernel
-from ..kv_cache import (  # noqa: F401
-    QuantizedKVCache,
-    quantized_cache_attention,
-    quantized_cache_fetch,
-    quantized_cache_update,
-)
+
+_CACHE_NAMES = ("QuantizedKVCache", "quantized_cache_update", "quantized_cache_fetch", "quantized_cache_attention")
+
+
+def __getattr__(name):
+    """The quantised cache's names, bound here at their first use (its module
+    builds on ``phew_b200.mx`` itself)."""
+    if name not in _CACHE_NAMES:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    from .. import kv_cache
+
+    for n in _CACHE_NAMES:
+        globals()[n] = getattr(kv_cache, n)
+    return globals()[name]
+
 
 _kernels: dict[tuple, CudaKernel] = {}
 
