@@ -12,6 +12,8 @@
 //   value = T(scale * code + bias)                               (fp32 fma)
 // so a written row is bit for bit what phew_quantize gives for it and a read
 // row what phew_dequantize gives.
+#include <type_traits>
+
 #include "common.cuh"
 #include "kv_cache.cuh"
 
@@ -22,23 +24,138 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int64_t kMaxRows = (1ll << 31) - (1 << 16);  // row numbers of a block past the last one stay 32-bit
 
-// Eight consecutive elements of a token row: one thread's share.
-template <typename T> struct alignas(16) Eight {
-  T v[8];
-};
+// Two floats in one 64-bit register, for the packed fp32 instructions (each half rounds like the scalar one).
+__device__ __forceinline__ uint64_t two(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+// max(a, |b|, |c|), NaN when one of them is
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
+  return d;
+}
 
+// Eight consecutive elements of a token row, as they lie in memory.
+template <typename T> struct Eight {
+  uint32_t w[2 * sizeof(T)];
+};
 template <typename T> __device__ __forceinline__ Eight<T> load8(const T* p) {
   Eight<T> e;
-  const uint4* q = reinterpret_cast<const uint4*>(p);
 #pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(&e)[i] = __ldg(q + i);
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    e.w[4 * i] = v.x;
+    e.w[4 * i + 1] = v.y;
+    e.w[4 * i + 2] = v.z;
+    e.w[4 * i + 3] = v.w;
+  }
   return e;
 }
 template <typename T> __device__ __forceinline__ void store8(T* p, const Eight<T>& e) {
-  uint4* q = reinterpret_cast<uint4*>(p);
 #pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) q[i] = reinterpret_cast<const uint4*>(&e)[i];
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+    reinterpret_cast<uint4*>(p)[i] = make_uint4(e.w[4 * i], e.w[4 * i + 1], e.w[4 * i + 2], e.w[4 * i + 3]);
 }
+template <typename T> __device__ __forceinline__ uint32_t pack(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack<bf16>(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+template <> __device__ __forceinline__ uint32_t pack<f16>(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+
+// Elements 2i, 2i + 1 as floats, and back.
+__device__ __forceinline__ uint64_t pair_of(const Eight<float>& e, int i) {
+  return two(__uint_as_float(e.w[2 * i]), __uint_as_float(e.w[2 * i + 1]));
+}
+__device__ __forceinline__ uint64_t pair_of(const Eight<bf16>& e, int i) {
+  return two(__uint_as_float(e.w[i] << 16), __uint_as_float(e.w[i] & 0xffff0000u));
+}
+__device__ __forceinline__ uint64_t pair_of(const Eight<f16>& e, int i) {
+  return two(to_f32(f16{static_cast<uint16_t>(e.w[i])}), to_f32(f16{static_cast<uint16_t>(e.w[i] >> 16)}));
+}
+template <typename T> __device__ __forceinline__ void set_pair(Eight<T>& e, int i, uint64_t v) {
+  if constexpr (sizeof(T) == 4) {
+    e.w[2 * i] = static_cast<uint32_t>(v);
+    e.w[2 * i + 1] = static_cast<uint32_t>(v >> 32);
+  } else {
+    e.w[i] = pack<T>(lo_of(v), hi_of(v));
+  }
+}
+
+// Smallest and largest of the eight.  The 16-bit types keep (min, -max) as one
+// packed pair, so a step across lanes is one shuffle and one packed minimum.
+template <typename T> struct Range {
+  uint32_t p;
+  static __device__ __forceinline__ uint32_t min_of(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if constexpr (std::is_same<T, bf16>::value)
+      asm("min.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else
+      asm("min.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  __device__ __forceinline__ void of(const Eight<T>& e) {
+    constexpr uint32_t neg = 0x80008000u;
+    const uint32_t lo = min_of(min_of(e.w[0], e.w[1]), min_of(e.w[2], e.w[3]));
+    const uint32_t hi = min_of(min_of(e.w[0] ^ neg, e.w[1] ^ neg), min_of(e.w[2] ^ neg, e.w[3] ^ neg));
+    p = min_of(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
+  }
+  __device__ __forceinline__ void with(const Range& o) { p = min_of(p, o.p); }
+  __device__ __forceinline__ void across(int lanes) {
+#pragma unroll
+    for (int o = lanes / 2; o > 0; o >>= 1) p = min_of(p, __shfl_xor_sync(0xffffffffu, p, o));
+  }
+  __device__ __forceinline__ float lo() const { return to_f32(T{static_cast<uint16_t>(p)}); }
+  __device__ __forceinline__ float hi() const { return -to_f32(T{static_cast<uint16_t>(p >> 16)}); }
+};
+template <> struct Range<float> {
+  float a, b;
+  __device__ __forceinline__ void of(const Eight<float>& e) {
+    a = b = __uint_as_float(e.w[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      a = fminf(a, __uint_as_float(e.w[i]));
+      b = fmaxf(b, __uint_as_float(e.w[i]));
+    }
+  }
+  __device__ __forceinline__ void with(const Range& o) {
+    a = fminf(a, o.a);
+    b = fmaxf(b, o.b);
+  }
+  __device__ __forceinline__ void across(int lanes) {
+#pragma unroll
+    for (int o = lanes / 2; o > 0; o >>= 1) {
+      a = fminf(a, __shfl_xor_sync(0xffffffffu, a, o));
+      b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, o));
+    }
+  }
+  __device__ __forceinline__ float lo() const { return a; }
+  __device__ __forceinline__ float hi() const { return b; }
+};
 
 // A row number in [0, 2^31) of a [batch][kv_heads][n] array, taken apart.
 struct RowSplit {
@@ -52,7 +169,11 @@ __device__ __forceinline__ void split_row(const RowSplit& s, int row, int& b, in
 }
 
 // Token rows a thread works on at once: their loads are in flight together.
-constexpr int kRows = 4;
+constexpr int kRows = 2;
+
+// 1.5 2^23: a float in [0, 2^22) added to it leaves the nearest whole number (ties to even) in the low bits.
+constexpr float kRound = 12582912.f;
+constexpr uint32_t kRoundBits = 0x4B400000u;
 
 struct UpdateParams {
   Cache c;
@@ -66,107 +187,144 @@ struct UpdateParams {
   int* error_flag;
 };
 
-// Codes of eight values.  (x - bias) / scale is taken as a product with the
-// reciprocal, which lies within 3 roundings (q 2^-22.4) of the IEEE quotient:
-// only where that could cross a border between two codes, or is no number,
-// are the eight divided again, so the codes are phew_quantize's bit for bit
-// at a third of the instructions of eight divisions.
-template <int BITS>
-__device__ __forceinline__ void codes8(const float* x, float bi, float sc, float* q) {
+// The group's scale and bias, and the reciprocal that codes are taken with.
+struct Affine {
+  float sc, bi, inv;
+  bool plain;  // every quotient lies in [0, top + 1/2): no clamping
+};
+template <typename T, int BITS> __device__ __forceinline__ Affine affine_of(const Range<T>& r) {
   constexpr float top = (1 << BITS) - 1;
-  constexpr float near = 0.5f - (BITS == 4 ? 1.f / (1 << 17) : 1.f / (1 << 13));  // > 3 roundings of 2 top
-  const float inv = __frcp_rn(sc);
-  bool sure = true;
+  Affine a;
+  const float lo = r.lo(), hi = r.hi();
+  a.sc = round_to<T>(fmaxf(__fdiv_rn(hi - lo, top), 1e-8f));
+  a.bi = lo;  // a value of type T
+  a.inv = __frcp_rn(a.sc);
+  a.plain = (hi - lo) * a.inv < top + 0.4999f;
+  return a;
+}
+
+// Codes of eight values: words for the cache, and as floats.  The product
+// with the reciprocal lies within three roundings of the IEEE quotient, so it
+// names the same code unless it falls next to a border between two; only such
+// values (one in a few hundred of bf16 data, whose quotients often hit a
+// border exactly) are divided.  Two values to an instruction throughout.
+template <typename T, int BITS>
+__device__ __forceinline__ void codes8(const Eight<T>& x, const Affine& a, uint32_t* words, uint64_t* q) {
+  constexpr float top = (1 << BITS) - 1;
+  constexpr float sure = 0.5f - (BITS == 4 ? 1.f / (1 << 17) : 1.f / (1 << 13));  // three roundings of 2 top
+  const uint64_t nb = two(-a.bi, -a.bi), inv = two(a.inv, a.inv), up = two(kRound, kRound), down = two(-kRound, -kRound);
+  uint64_t v[4], t[4];
+  float off = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float v = __fmul_rn(x[e] - bi, inv);
-    const float r = __fadd_rn(__fadd_rn(v, 12582912.f), -12582912.f);  // nearest even, |v| < 2^22
-    sure = sure && fabsf(v - r) < near;
-    q[e] = fminf(fmaxf(r, 0.f), top);
+  for (int i = 0; i < 4; ++i) {
+    v[i] = mul2(add2(pair_of(x, i), nb), inv);
+    t[i] = add2(v[i], up);
+    q[i] = add2(t[i], down);
+    v[i] = fma2(q[i], two(-1.f, -1.f), v[i]);
+    off = max_abs(off, lo_of(v[i]), hi_of(v[i]));
   }
-  if (!sure) {
+  if (!(off < sure) || !a.plain) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = fminf(fmaxf(rintf(__fdiv_rn(x[e] - bi, sc)), 0.f), top);
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t xs = pair_of(x, i);
+      float f[2] = {lo_of(q[i]), hi_of(q[i])};
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (!a.plain || !(fabsf(k ? hi_of(v[i]) : lo_of(v[i])) < sure))
+          f[k] = fminf(fmaxf(rintf(__fdiv_rn((k ? hi_of(xs) : lo_of(xs)) - a.bi, a.sc)), 0.f), top);
+      q[i] = two(f[0], f[1]);
+      t[i] = add2(q[i], up);
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < BITS / 4; ++w) {
+    uint32_t sum = 0u - kRoundBits * (BITS == 4 ? 0x11111111u : 0x01010101u);
+#pragma unroll
+    for (int e = 0; e < 32 / BITS; ++e) {
+      const uint64_t p = t[(w * (32 / BITS) + e) / 2];
+      sum += static_cast<uint32_t>(e & 1 ? p >> 32 : p) << (e * BITS);
+    }
+    words[w] = sum;
   }
 }
 
-// Bound by HBM: one 16-byte load of x per eight 16-bit values, 4 or 8 bytes of
-// codes out (and 16 of values).  Eight values to a thread make a code word of
-// one thread and a group of 4, 8 or 16 neighbouring lanes.
-template <typename T, int BITS, int G>
+// Bound by HBM (update of 4 x 32 heads x 8192 tokens of 128 bf16 values with
+// the values written back: 1.22 GB).  A thread takes eight neighbouring values
+// of either half of a row, so that every load and store of a warp is
+// contiguous and the row's address is worked out once for sixteen values; a
+// group is G / 8 neighbouring lanes, or both halves of D / 16.
+template <typename T, int BITS, int D, int G>
 __global__ void __launch_bounds__(kThreads) update_kernel(const UpdateParams p) {
-  constexpr int LG = G / 8;
-  constexpr float top = (1 << BITS) - 1;
+  constexpr int LANES = D / 16;                 // threads to a row
+  constexpr int PER_PASS = kThreads / LANES;    // rows to a pass of the block
+  constexpr int LG = G < D ? G / 8 : LANES;     // lanes of a group
+  constexpr int NG = D / G;
   const int side = blockIdx.y;
-  const int lanes = p.c.head_dim / 8;                  // threads to a row
-  const int per_pass = kThreads / lanes;               // rows to a pass of the block
-  const int c = threadIdx.x & (lanes - 1);             // which eight of the row
-  const int row0 = blockIdx.x * (per_pass * kRows) + static_cast<int>(threadIdx.x) / lanes;
-  const int ng = p.c.head_dim / G;
+  const int c = threadIdx.x % LANES;
+  const int row0 = blockIdx.x * (PER_PASS * kRows) + static_cast<int>(threadIdx.x) / LANES;
   const T* xs = static_cast<const T*>(p.x[side]);
-  Eight<T> in[kRows];
+  Eight<T> in[kRows][2];
   int b[kRows], h[kRows], tok[kRows];
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
-    const int row = row0 + u * per_pass;
+    const int row = row0 + u * PER_PASS;
+    tok[u] = -1;
+    in[u][0] = in[u][1] = Eight<T>{};
     if (row < p.rows) {
       split_row(p.split, row, b[u], h[u], tok[u]);
-      in[u] = load8(xs + b[u] * p.st[side][2] + h[u] * p.st[side][1] + tok[u] * p.st[side][0] + c * 8);
-    } else {
-      tok[u] = -1;
-      in[u] = Eight<T>{};
+      const T* x = xs + b[u] * p.st[side][2] + h[u] * p.st[side][1] + tok[u] * p.st[side][0] + c * 8;
+      in[u][0] = load8(x);
+      in[u][1] = load8(x + D / 2);
     }
   }
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
-    float x[8], q[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = to_f32(in[u].v[e]);
-    float lo = x[0], hi = x[0];
-#pragma unroll
-    for (int e = 1; e < 8; ++e) {
-      lo = fminf(lo, x[e]);
-      hi = fmaxf(hi, x[e]);
-    }
-#pragma unroll
-    for (int o = LG / 2; o > 0; o >>= 1) {  // a group's lanes lie side by side
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
+    Range<T> r[2];
+    r[0].of(in[u][0]);
+    r[1].of(in[u][1]);
+    if (G == D) r[0].with(r[1]);
+    r[0].across(LG);
+    if (G < D)
+      r[1].across(LG);
+    else
+      r[1] = r[0];
     if (tok[u] < 0) continue;
-    const int row = row0 + u * per_pass;
     const int count = p.counts ? clamp_count(__ldg(p.counts + b[u]), p.tokens) : p.tokens;
-    T* dense = p.dense[side] ? static_cast<T*>(p.dense[side]) + static_cast<int64_t>(row) * p.c.head_dim + c * 8 : nullptr;
+    T* dense = nullptr;
+    if (p.dense[side]) dense = static_cast<T*>(p.dense[side]) + static_cast<int64_t>(row0 + u * PER_PASS) * D + c * 8;
     if (tok[u] >= count) {
-      if (dense) store8(dense, Eight<T>{});
+      if (dense) {
+        store8(dense, Eight<T>{});
+        store8(dense + D / 2, Eight<T>{});
+      }
       continue;
     }
-    const float sc = round_to<T>(fmaxf(__fdiv_rn(hi - lo, top), 1e-8f));
-    const float bi = round_to<T>(lo);
-    codes8<BITS>(x, bi, sc, q);
     const uint32_t at = row_of(p.c.map, b[u], h[u], static_cast<int64_t>(__ldg(p.offsets + b[u])) + tok[u]);
-    if (at == kNoRow) {
-      atomicExch(p.error_flag, PHEW_ERR_INVALID);
-    } else {
-      uint32_t w[BITS / 4] = {};
+    if (at == kNoRow) atomicExch(p.error_flag, PHEW_ERR_INVALID);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e * BITS / 32] |= static_cast<uint32_t>(q[e]) << (e * BITS % 32);
-      uint32_t* dst = p.c.codes[side] + (static_cast<int64_t>(at) * lanes + c) * (BITS / 4);
-      if (BITS == 4)
-        dst[0] = w[0];
-      else
-        *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[BITS / 4 - 1]);
-      if ((c & (LG - 1)) == 0) {
-        const int64_t s_at = static_cast<int64_t>(at) * ng + c / LG;
-        static_cast<T*>(p.c.scales[side])[s_at] = from_f32<T>(sc);
-        static_cast<T*>(p.c.biases[side])[s_at] = from_f32<T>(bi);
+    for (int half = 0; half < 2; ++half) {
+      const Affine a = affine_of<T, BITS>(r[half]);
+      uint32_t words[BITS / 4];
+      uint64_t q[4];
+      codes8<T, BITS>(in[u][half], a, words, q);
+      if (at != kNoRow) {
+        uint32_t* dst = p.c.codes[side] + static_cast<int64_t>(at) * (D * BITS / 32) + (half * (D / 16) + c) * (BITS / 4);
+        if (BITS == 4)
+          dst[0] = words[0];
+        else
+          *reinterpret_cast<uint2*>(dst) = make_uint2(words[0], words[BITS / 4 - 1]);
+        if (c % LG == 0 && (G < D || half == 0)) {
+          const int64_t s_at = static_cast<int64_t>(at) * NG + (half * (D / 2) + c * 8) / G;
+          static_cast<T*>(p.c.scales[side])[s_at] = from_f32<T>(a.sc);
+          static_cast<T*>(p.c.biases[side])[s_at] = from_f32<T>(a.bi);
+        }
       }
-    }
-    if (dense) {
-      Eight<T> out;
+      if (dense) {
+        Eight<T> out;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) out.v[e] = from_f32<T>(fmaf(sc, q[e], bi));
-      store8(dense, out);
+        for (int i = 0; i < 4; ++i) set_pair(out, i, fma2(two(a.sc, a.sc), q[i], two(a.bi, a.bi)));
+        store8(dense + half * (D / 2), out);
+      }
     }
   }
 }
@@ -180,20 +338,23 @@ struct FetchParams {
   int* error_flag;
 };
 
-// Bound by HBM, mostly by the values written: eight codes (one or two words)
-// and their group's scale and bias to a thread, 16 bytes of 16-bit values out.
-template <typename T, int BITS>
+// Bound by HBM, mostly by the values written.  Eight codes of either half of
+// a row to a thread, as in update_kernel.  A code becomes a float by a byte
+// permutation into 2^23 + code (conversions run at an eighth of the rate),
+// two values to an instruction from there.
+template <typename T, int BITS, int D>
 __global__ void __launch_bounds__(kThreads) fetch_kernel(const FetchParams p) {
+  constexpr int LANES = D / 16;
+  constexpr int PER_PASS = kThreads / LANES;
+  constexpr int W = BITS / 4;  // words of eight codes
   const int side = blockIdx.y;
-  const int lanes = p.c.head_dim / 8;
-  const int per_pass = kThreads / lanes;
-  const int c = threadIdx.x & (lanes - 1);
-  const int row0 = blockIdx.x * (per_pass * kRows) + static_cast<int>(threadIdx.x) / lanes;
-  const int ng = p.c.head_dim / p.c.group, grp = c * 8 / p.c.group;
+  const int c = threadIdx.x % LANES;
+  const int row0 = blockIdx.x * (PER_PASS * kRows) + static_cast<int>(threadIdx.x) / LANES;
+  const int ng = D / p.c.group, shift = p.c.group == 32 ? 5 : p.c.group == 64 ? 6 : 7;
   uint32_t at[kRows];
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
-    const int row = row0 + u * per_pass;
+    const int row = row0 + u * PER_PASS;
     at[u] = kNoRow;
     if (row < p.rows) {
       int b, h, pos;
@@ -204,51 +365,78 @@ __global__ void __launch_bounds__(kThreads) fetch_kernel(const FetchParams p) {
       }
     }
   }
-  uint32_t w[kRows][BITS / 4];
-  T sc[kRows], bi[kRows];
+  uint32_t w[kRows][2][W];
+  T sc[kRows][2], bi[kRows][2];
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
     if (at[u] == kNoRow) continue;
-    const uint32_t* src = p.c.codes[side] + (static_cast<int64_t>(at[u]) * lanes + c) * (BITS / 4);
-    if (BITS == 4) {
-      w[u][0] = __ldg(src);
-    } else {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
-      w[u][0] = v.x;
-      w[u][BITS / 4 - 1] = v.y;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint32_t* src = p.c.codes[side] + static_cast<int64_t>(at[u]) * (D * BITS / 32) + (half * (D / 16) + c) * W;
+      if (BITS == 4) {
+        w[u][half][0] = __ldg(src);
+      } else {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
+        w[u][half][0] = v.x;
+        w[u][half][W - 1] = v.y;
+      }
+      const int64_t s_at = static_cast<int64_t>(at[u]) * ng + ((half * (D / 2) + c * 8) >> shift);
+      sc[u][half] = static_cast<const T*>(p.c.scales[side])[s_at];
+      bi[u][half] = static_cast<const T*>(p.c.biases[side])[s_at];
     }
-    const int64_t s_at = static_cast<int64_t>(at[u]) * ng + grp;
-    sc[u] = static_cast<const T*>(p.c.scales[side])[s_at];
-    bi[u] = static_cast<const T*>(p.c.biases[side])[s_at];
   }
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
-    const int row = row0 + u * per_pass;
+    const int row = row0 + u * PER_PASS;
     if (row >= p.rows) continue;
-    Eight<T> out{};
-    if (at[u] != kNoRow) {
-      const float s = to_f32(sc[u]), z = to_f32(bi[u]);
+    T* dst = static_cast<T*>(p.dense[side]) + static_cast<int64_t>(row) * D + c * 8;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        out.v[e] = from_f32<T>(fmaf(s, static_cast<float>((w[u][e * BITS / 32] >> (e * BITS % 32)) & ((1 << BITS) - 1)), z));
+    for (int half = 0; half < 2; ++half) {
+      Eight<T> out{};
+      if (at[u] != kNoRow) {
+        const float s = to_f32(sc[u][half]), z = to_f32(bi[u][half]);
+        constexpr uint32_t base = 0x4B000000u;  // 2^23
+        // even and odd codes of 4 bits, or all of 8, a byte each
+        const uint32_t even = BITS == 4 ? w[u][half][0] & 0x0f0f0f0fu : w[u][half][0];
+        const uint32_t odd = BITS == 4 ? (w[u][half][0] >> 4) & 0x0f0f0f0fu : w[u][half][W - 1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t lo, hi;
+          if (BITS == 4) {
+            lo = __byte_perm(even, base, 0x7540 + i);
+            hi = __byte_perm(odd, base, 0x7540 + i);
+          } else {
+            lo = __byte_perm(i < 2 ? even : odd, base, 0x7540 + 2 * (i & 1));
+            hi = __byte_perm(i < 2 ? even : odd, base, 0x7541 + 2 * (i & 1));
+          }
+          const uint64_t n = add2(two(__uint_as_float(lo), __uint_as_float(hi)), two(-8388608.f, -8388608.f));
+          set_pair(out, i, fma2(two(s, s), n, two(z, z)));
+        }
+      }
+      store8(dst + half * (D / 2), out);
     }
-    store8(static_cast<T*>(p.dense[side]) + static_cast<int64_t>(row) * p.c.head_dim + c * 8, out);
   }
 }
 
 // Blocks along x for `rows` token rows of a side.
 dim3 grid_for(int64_t rows, int head_dim) {
-  const int64_t per_block = static_cast<int64_t>(kThreads / (head_dim / 8)) * kRows;
+  const int64_t per_block = static_cast<int64_t>(kThreads / (head_dim / 16)) * kRows;
   return dim3(static_cast<unsigned>((rows + per_block - 1) / per_block), 2);
 }
 
 template <typename T, int BITS> void launch_update(const UpdateParams& p, cudaStream_t st) {
   const dim3 grid = grid_for(p.rows, p.c.head_dim);
-  switch (p.c.group) {
-    case 32: update_kernel<T, BITS, 32><<<grid, kThreads, 0, st>>>(p); break;
-    case 64: update_kernel<T, BITS, 64><<<grid, kThreads, 0, st>>>(p); break;
-    default: update_kernel<T, BITS, 128><<<grid, kThreads, 0, st>>>(p); break;
-  }
+#define PHEW_KV_UPDATE(D, G) \
+  if (p.c.head_dim == D && p.c.group == G) return update_kernel<T, BITS, D, G><<<grid, kThreads, 0, st>>>(p)
+  PHEW_KV_UPDATE(64, 32);
+  PHEW_KV_UPDATE(64, 64);
+  PHEW_KV_UPDATE(128, 32);
+  PHEW_KV_UPDATE(128, 64);
+  PHEW_KV_UPDATE(128, 128);
+  PHEW_KV_UPDATE(256, 32);
+  PHEW_KV_UPDATE(256, 64);
+  PHEW_KV_UPDATE(256, 128);
+#undef PHEW_KV_UPDATE
 }
 
 template <typename T> int update_typed(const UpdateParams& p, cudaStream_t st) {
@@ -259,12 +447,20 @@ template <typename T> int update_typed(const UpdateParams& p, cudaStream_t st) {
   return launch_status("kv update_kernel");
 }
 
-template <typename T> int fetch_typed(const FetchParams& p, cudaStream_t st) {
+template <typename T, int BITS> void launch_fetch(const FetchParams& p, cudaStream_t st) {
   const dim3 grid = grid_for(p.rows, p.c.head_dim);
+  switch (p.c.head_dim) {
+    case 64: fetch_kernel<T, BITS, 64><<<grid, kThreads, 0, st>>>(p); break;
+    case 128: fetch_kernel<T, BITS, 128><<<grid, kThreads, 0, st>>>(p); break;
+    default: fetch_kernel<T, BITS, 256><<<grid, kThreads, 0, st>>>(p); break;
+  }
+}
+
+template <typename T> int fetch_typed(const FetchParams& p, cudaStream_t st) {
   if (p.c.bits == 4)
-    fetch_kernel<T, 4><<<grid, kThreads, 0, st>>>(p);
+    launch_fetch<T, 4>(p, st);
   else
-    fetch_kernel<T, 8><<<grid, kThreads, 0, st>>>(p);
+    launch_fetch<T, 8>(p, st);
   return launch_status("kv fetch_kernel");
 }
 
