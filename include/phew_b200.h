@@ -132,10 +132,11 @@ int phew_event_elapsed_ms(void* start, void* stop, float* ms);
 int phew_event_destroy(void* event);
 
 /* Test hook for the failure path of the tensor-core pipelines, not for
- * production use.  The NEXT phew_gemm or phew_sdpa call on the calling
- * thread that launches a tcgen05 kernel leaves one of its producer's tile
- * loads unissued -- GEMM: ring position `stage` (the stage-th k-block load
- * of each CTA); attention: the V tile of key tile `stage` -- and bounds
+ * production use.  The NEXT phew_gemm, phew_sdpa or phew_kv_attention call on
+ * the calling thread that launches a tcgen05 kernel leaves one of its
+ * producer's tile loads unissued -- GEMM: ring position `stage` (the stage-th
+ * k-block load of each CTA); attention: the V tile of key tile `stage` (of
+ * the cache's, the word that it is there) -- and bounds
  * each of its pipeline waits by `wait_limit_ns` (0 < limit <= 1 s) instead
  * of 1 s.  The consumers' waits then run out: the kernel sets the caller's
  * error flag to PHEW_ERR_TIMEOUT, lets the loads and MMAs it did issue land,
@@ -322,7 +323,9 @@ int phew_quantize(const void* w, void* wq, void* scales, void* biases, int64_t r
  * table live on the device, so that a captured graph replays with new ones;
  * table entries behind a sequence's last page are not read.  A position
  * outside a sequence's pages or a table entry that is no page of the cache
- * is not accessed: it sets *error_flag (device int) to PHEW_ERR_INVALID. */
+ * is not accessed: it sets error_flag[0] to PHEW_ERR_INVALID.  error_flag is
+ * two device ints; a pipeline wait of phew_kv_attention that runs out sets
+ * error_flag[1] to PHEW_ERR_TIMEOUT. */
 typedef struct phew_kv_cache {
   void* k_codes;
   void* k_scales;
@@ -361,9 +364,10 @@ int phew_kv_fetch(const phew_kv_cache* cache, void* k_out, void* v_out, int64_t 
                   const int* lengths, const int* block_table, int64_t table_stride, int64_t columns,
                   int* error_flag, void* stream);
 
-/* Bytes of device scratch phew_kv_attention needs on the current device. */
+/* Bytes of device scratch phew_kv_attention needs on the current device
+ * (columns as there, 1 without a block table). */
 size_t phew_kv_attention_workspace(const phew_kv_cache* cache, int64_t batch, int64_t heads,
-                                   int64_t tokens);
+                                   int64_t tokens, int64_t columns);
 
 /* o = softmax(scale * q k^T) v over a 4-bit cache: q [batch][heads][tokens]
  * [head_dim] of the cache's dtype (strides {token, head, batch} in elements,

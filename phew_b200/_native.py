@@ -177,7 +177,7 @@ _SIGNATURES = {
         [ctypes.POINTER(KVCache), _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp],
         _int,
     ),
-    "phew_kv_attention_workspace": ([ctypes.POINTER(KVCache), _i64, _i64, _i64], ctypes.c_size_t),
+    "phew_kv_attention_workspace": ([ctypes.POINTER(KVCache), _i64, _i64, _i64, _i64], ctypes.c_size_t),
     "phew_kv_attention": (
         [ctypes.POINTER(KVCache), _vp, ctypes.POINTER(_i64), _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64,
          ctypes.c_float, _int, _vp, ctypes.c_size_t, _vp, _vp],

@@ -6,19 +6,39 @@
 // over the keys j < lengths[b] that token i sees, k and v the values
 // scale * code + bias of the cache.  The serving form of
 // mx.fast.quantized_scaled_dot_product_attention (phew emit/codegen.py:428-449).
-#include "kv_attn.cuh"
+#include "kv_attn_tc.cuh"
+
+namespace phew {
+namespace kv {
+namespace {
+
+// Query rows to a cache head from which the tcgen05 kernel takes over: below, the mma.sync kernel's one or
+// two passes over the cache cost less than a 256-row tile that is mostly empty.
+constexpr int64_t kTcMinRows = 64;
+
+bool takes_tc(int dtype, int head_dim, int64_t rows) {
+  return dtype != PHEW_F32 && head_dim <= 128 && rows >= kTcMinRows;
+}
+
+}  // namespace
+}  // namespace kv
+}  // namespace phew
 
 using namespace phew;
 
 extern "C" size_t phew_kv_attention_workspace(const phew_kv_cache* cache, int64_t batch, int64_t heads,
-                                              int64_t tokens) {
-  if (!cache || cache->kv_heads <= 0) return 0;
+                                              int64_t tokens, int64_t columns) {
+  if (!cache || cache->kv_heads <= 0 || batch <= 0 || heads <= 0 || tokens <= 0 || columns <= 0) return 0;
   const int64_t rows = tokens * (heads / cache->kv_heads);
+  size_t few = 0, many = 0;
   switch (cache->dtype) {
-    case PHEW_F32: return kv::attn_bytes<float>(cache->head_dim, cache->group_size, rows);
-    case PHEW_F16: return kv::attn_bytes<f16>(cache->head_dim, cache->group_size, rows);
-    default: return kv::attn_bytes<bf16>(cache->head_dim, cache->group_size, rows);
+    case PHEW_F32: few = kv::attn_bytes<float>(cache->head_dim, cache->group_size, rows); break;
+    case PHEW_F16: few = kv::attn_bytes<f16>(cache->head_dim, cache->group_size, rows); break;
+    default: few = kv::attn_bytes<bf16>(cache->head_dim, cache->group_size, rows);
   }
+  if (kv::takes_tc(cache->dtype, cache->head_dim, rows))
+    many = kv::tc_bytes(batch, cache->kv_heads, cache->head_dim, rows, columns * cache->page_size);
+  return few > many ? few : many;
 }
 
 extern "C" int phew_kv_attention(const phew_kv_cache* cache, const void* q, const int64_t* q_strides, void* o,
@@ -40,7 +60,7 @@ extern "C" int phew_kv_attention(const phew_kv_cache* cache, const void* q, cons
                  "phew_kv_attention: strides must be multiples of 16 bytes");
   PHEW_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
                "phew_kv_attention: pointers must be 16-byte aligned");
-  PHEW_REQUIRE(workspace_bytes >= phew_kv_attention_workspace(cache, batch, heads, tokens) &&
+  PHEW_REQUIRE(workspace_bytes >= phew_kv_attention_workspace(cache, batch, heads, tokens, block_table ? columns : 1) &&
                    (workspace || workspace_bytes == 0),
                "phew_kv_attention: the workspace is too small");
   p.q = q;
@@ -57,6 +77,9 @@ extern "C" int phew_kv_attention(const phew_kv_cache* cache, const void* q, cons
   p.causal = causal != 0;
   p.error_flag = error_flag;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // (the tcgen05 kernel takes its maxima over unscaled scores)
+  if (kv::takes_tc(cache->dtype, cache->head_dim, static_cast<int64_t>(p.tokens) * p.per) && p.scale_log2 > 0.f)
+    return kv::run_attn_tc(p, cache->dtype == PHEW_BF16, workspace, st);
   switch (cache->dtype) {
     case PHEW_F32: return kv::run_attn<float>(p, workspace, st);
     case PHEW_F16: return kv::run_attn<f16>(p, workspace, st);

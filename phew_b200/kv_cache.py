@@ -23,22 +23,26 @@ _Strides = ctypes.c_int64 * 3
 
 
 def cache_error_flag(device: torch.device) -> torch.Tensor:
-    """Device int that the cache's kernels set when a position or a page lies
-    outside the cache (0 = clean)."""
+    """Two device ints (0 = clean): [0] set when a position or a page lies
+    outside the cache, [1] when a bounded wait ran out."""
     f = _error_flags.get(device.index)
     if f is None:
-        f = torch.zeros(1, dtype=torch.int32, device=device)
+        f = torch.zeros(2, dtype=torch.int32, device=device)
         _error_flags[device.index] = f
     return f
 
 
 def check_cache_errors() -> None:
     """Raise if a kernel of the cache met a position outside a sequence's
-    pages or a block table entry that is no page (synchronises)."""
+    pages or a block table entry that is no page, or gave up a wait
+    (synchronises)."""
     for f in _error_flags.values():
-        code = int(f.item())
-        if code:
+        code, waited = f.tolist()
+        if code or waited:
             f.zero_()
+        if waited:
+            raise _native.PhewError(waited, "quantised cache: a device-side wait timed out (pipeline stalled)")
+        if code:
             raise _native.PhewError(
                 code, "quantised cache: a length or offset outside a sequence's pages, or a block "
                       "table entry that is no page of the cache")
@@ -219,12 +223,12 @@ def _call(name: str, cache: QuantizedKVCache, *args) -> None:
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace(device: int, kv_heads: int, head_dim: int, group_size: int, dtype: int, batch: int, heads: int,
-               tokens: int) -> int:
+def _workspace(device: int, page_size: int, kv_heads: int, head_dim: int, group_size: int, dtype: int, batch: int,
+               heads: int, tokens: int, columns: int) -> int:
     """Scratch bytes of an attention call; they depend on its sizes and the device alone."""
-    c = _native.KVCache(kv_heads=kv_heads, head_dim=head_dim, group_size=group_size, dtype=dtype)
+    c = _native.KVCache(page_size=page_size, kv_heads=kv_heads, head_dim=head_dim, group_size=group_size, dtype=dtype)
     with torch.cuda.device(device):
-        return int(_native.load().phew_kv_attention_workspace(c, batch, heads, tokens))
+        return int(_native.load().phew_kv_attention_workspace(c, batch, heads, tokens, columns))
 
 
 def quantized_cache_update(cache: QuantizedKVCache, k, v, offsets, *, block_table=None, counts=None,
@@ -311,8 +315,8 @@ def quantized_cache_attention(q, cache: QuantizedKVCache, lengths, *, block_tabl
     n = _ints(lengths, batch, "quantized_cache_attention: lengths", cache)
     cnt = None if counts is None else _ints(counts, batch, "quantized_cache_attention: counts", cache)
     keep, table, stride, columns = _table(block_table, batch, "quantized_cache_attention", cache)
-    size = _workspace(cache.device.index, cache.kv_heads, cache.head_dim, cache.group_size, cache.dtype.code, batch,
-                      heads, tokens)
+    size = _workspace(cache.device.index, cache.page_size, cache.kv_heads, cache.head_dim, cache.group_size,
+                      cache.dtype.code, batch, heads, tokens, columns)
     work = n.new_empty(size // 4)
     o = q.new_empty(shape)
     _call("phew_kv_attention", cache, q.data_ptr(), qs, o.data_ptr(), batch, heads, tokens, n.data_ptr(),
