@@ -32,9 +32,9 @@ extern "C" size_t phew_kv_attention_workspace(const phew_kv_cache* cache, int64_
   const int64_t rows = tokens * (heads / cache->kv_heads);
   size_t few = 0, many = 0;
   switch (cache->dtype) {
-    case PHEW_F32: few = kv::attn_bytes<float>(cache->head_dim, cache->group_size, rows); break;
-    case PHEW_F16: few = kv::attn_bytes<f16>(cache->head_dim, cache->group_size, rows); break;
-    default: few = kv::attn_bytes<bf16>(cache->head_dim, cache->group_size, rows);
+    case PHEW_F32: few = kv::attn_bytes<float>(batch, cache->kv_heads, cache->head_dim, cache->group_size, rows); break;
+    case PHEW_F16: few = kv::attn_bytes<f16>(batch, cache->kv_heads, cache->head_dim, cache->group_size, rows); break;
+    default: few = kv::attn_bytes<bf16>(batch, cache->kv_heads, cache->head_dim, cache->group_size, rows);
   }
   if (kv::takes_tc(cache->dtype, cache->head_dim, rows))
     many = kv::tc_bytes(batch, cache->kv_heads, cache->head_dim, rows, columns * cache->page_size);

@@ -1,38 +1,49 @@
 // Attention of few query rows over a 4-bit cache (decode, drafted tokens).
 //
-//   s_rj = scale * sum_g sk[j,g] (q_r . c_j)_g + (zk[j,g] + 8 sk[j,g]) sum(q_r)_g
-//   o_r  = sum_j p_rj (sum_g sv[j,g] c_j + (zv[j,g] + 8 sv[j,g])) / sum_j p_rj
+//   s_rj = scale * sum_g sk[j,g] (q_r . n_j)_g + zk[j,g] sum(q_r)_g
+//   o_r  = sum_j p_rj (sum_g sv[j,g] n_j + zv[j,g]) / sum_j p_rj
 //
-// with c = code - 8, a whole number that bf16 and f16 hold exactly: scales and
-// biases never touch a code, they act on the small score tile (keys) and on
-// the softmax weights (values).  A cache head's `per` query heads and the
-// query tokens are the rows r = token * per + head, eight or sixteen to a
-// block, so keys and values are read once for all of them.
+// with n the codes as they lie in the cache: scales and biases never touch a
+// code, they act on the small score tile (keys) and on the softmax weights
+// (values).  A cache head's `per` query heads and the query tokens are the
+// rows r = token * per + head, eight or sixteen to a block, so keys and values
+// are read once for all of them.
 //
 // Bound by HBM (a packed row of 128 with groups of 64 is 72 bytes): at 6.5
-// TB/s an SM gets 41 codes a clock, which leaves about three instruction
-// lanes for each.  So
+// TB/s an SM gets 41 codes a clock, which leaves 1.6 integer instructions (two
+// warp instructions a clock, measured) and 3 of any kind for each 32.  So
 //  * both products run on mma.sync m16n8k16 with keys (scores) and head
-//    dimension (output) along m and the few query rows along n: no padding
-//    of eight rows to sixteen, and codes go from packed words to fragments in
-//    registers with one shift and one logic operation per pair.  (tcgen05
-//    would need the codes as 16-bit tiles in shared memory: four times the
-//    bytes, written and read once more than the 128 bytes a clock an SM has.)
+//    dimension (output) along m and the few query rows along n: no padding of
+//    eight rows to sixteen.  (tcgen05 would need the codes as 16-bit tiles in
+//    shared memory: four times the bytes, written and read once more than the
+//    128 bytes a clock an SM has.)
+//  * codes need no conversion: sixteen bits that hold n in 0 .. 15 are the f16
+//    subnormal n 2^-24, and n one digit up is 16 n 2^-24, so one logic operation
+//    makes a pair of operands, `w & 0x000f000f` or `w & 0x00f000f0`, and one
+//    shift by eight brings the word's other half under the same masks: 5
+//    instructions for eight codes.  The 16 goes into the query (keys) or out of
+//    the sum (values), exactly.  (e4m3, which holds a nibble in a byte as it
+//    is, was tried: mma.sync on that type is expanded into conversions here,
+//    11 instructions each.)
+//  * queries and weights are f16 after a power of two: a row's largest query
+//    element goes to [2^14, 2^15); weights, at most 2^kGrow, times a value scale
+//    kept at most 2^7 by a power of two that follows the largest scale met.
+//    What falls below f16's range is then under 2^-38 of the largest.  f32
+//    queries and weights are two f16 terms (22 bits);
 //  * a word's eight codes stay with the thread that loads it: the order of
 //    the head dimension inside a product is free, so queries are arranged to
-//    match (pairs i, i + 4 of a word) and nothing is shuffled;
-//  * weights move from the score fragment (key-major) to the operand of the
-//    second product by movmatrix, in registers;
-//  * every warp walks its own 32 of each 128 keys with its own running
-//    maximum and sum and its own ring of cp.async stages: no block barrier in
-//    the loop; warps join in shared memory once per segment.
+//    match and nothing is shuffled; weights move from the score fragment
+//    (key-major) to the operand of the second product by movmatrix;
+//  * every warp walks keys of its own with its own running maximum and sum
+//    and its own ring of cp.async stages: no block barrier anywhere, so the
+//    latencies at a segment's begin and end are hidden by the SM's other warps.
 //
 // Work split: the (sequence, row block, cache head) segments of all
-// sequences, cut into tiles of 128 keys, are one line of W tiles; block c of n
-// takes tiles [cW/n, (c+1)W/n), so any mix of lengths loads the SMs evenly and
-// no host ever needs the lengths.  A segment that lies in one block is
-// finished there; a cut one leaves partial sums (maximum, sum, output) that
-// the combine kernel joins in a fixed order.
+// sequences, cut into tiles of 32 keys, are one line of W units (a segment's
+// begin counts as kBegin tiles); warp c of n takes units [cW/n, (c+1)W/n), so
+// any mix of lengths loads the SMs evenly and no host ever needs the lengths.
+// A segment that lies in one warp is finished there; a cut one leaves partial
+// sums (maximum, sum, output) that the combine kernel joins in a fixed order.
 #pragma once
 
 #include <atomic>
@@ -43,9 +54,10 @@
 namespace phew {
 namespace kv {
 
-constexpr int kWarps = 4;
-constexpr int kStageKeys = 32;                  // keys of one warp's stage
-constexpr int kTile = kWarps * kStageKeys;      // keys of one block step
+constexpr int kWarps = 4;       // of a block; they share nothing
+constexpr int kTile = 32;       // keys of a tile: one warp's stage
+constexpr int kBegin = 2;       // tiles that the latencies of a segment's begin are worth
+constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;  // codes of a word as pairs of f16
 constexpr float kGrow = 8.0f;                   // log2 units a score may pass the running maximum by
 constexpr float kFloor = -1.0e38f;              // running maximum before the first key
 
@@ -58,12 +70,16 @@ struct AttnParams {
   const int32_t* counts;  // null: all `tokens`
   int batch, heads, tokens, per;  // per: query heads to a cache head
   int blocks;                     // row blocks of a sequence's tokens * per rows
+  int step_col, step_row;         // kTile tokens in pages and rows
+  uint32_t page_rows;             // kv_heads * page_size
+  bool eights;                    // pages hold whole eights of rows
   FastDiv by_per, by_blocks;
   float scale_log2;
   bool causal;
-  float* part;   // [n][2][rows][D] partial outputs, then [n][2][rows][2] (maximum, sum)
-  float* part_ml;
-  int64_t* meta;  // [n][2]: segment of partial 0 (begun by an earlier block) and 1 (left to later ones); -1: none
+  // scratch: of every warp two partials, 0 of a segment that an earlier warp began and 1 of one that it leaves
+  float* part;     // [warp][2][rows][D] outputs
+  float* part_ml;  // [warp][2][rows][2] maximum and sum
+  int2* span;      // [segment] first and last warp; equal where one warp finished it
   int* error_flag;
 };
 
@@ -72,7 +88,7 @@ struct Entry {
   int b, block;
   int length, count;
   int end;    // keys [0, end) that any of its rows sees
-  int tiles;  // at least one, so that some block writes the rows of an empty one
+  int tiles;  // at least one, so that some warp writes the rows of an empty one
 };
 
 __device__ __forceinline__ Entry entry_at(const AttnParams& p, int e, int rows) {
@@ -93,20 +109,24 @@ template <typename T, int D_, int G_, int NT_> struct Shape {
   static constexpr int ROWS = 8 * NT;
   static constexpr int NG = D / G;
   static constexpr bool F32 = sizeof(T) == 4;
-  // terms of a value split into bf16: queries (f32: 24 bits in three; f16 and bf16 as they are) and weights
-  // (bf16 results: one, 2^-9 of a weight; f16: two, 2^-17; f32: three)
-  static constexpr int TQ = F32 ? 3 : 1;
-  static constexpr int TP = F32 ? 3 : std::is_same<T, f16>::value ? 2 : 1;
+  // f16 terms of a query and of a weight: one is exact for 16-bit queries and rounds a weight by 2^-12 of it
+  static constexpr int TERMS = F32 ? 2 : 1;
+  // f16 results see that rounding: it is halved by weighing n - 8 instead of n, the 8 times the sum of the
+  // rounded weights (an accumulator of its own) subtracted at the end
+  static constexpr bool CENTRED = std::is_same<T, f16>::value;
   static constexpr int SB = NG * static_cast<int>(sizeof(T));   // bytes of a key's scales
   static constexpr int SROW = SB < 4 ? 4 : SB;
-  static constexpr int CODE_BYTES = kStageKeys * D / 2;         // one side's codes of a stage
-  static constexpr int STAGE = 2 * CODE_BYTES + 4 * kStageKeys * SROW;
-  static constexpr int STAGES = D == 64 ? 4 : D == 128 ? 3 : 2;
-  static constexpr int RING = STAGE * STAGES;                   // per warp
-  static constexpr int OROW = D + 4;                            // floats of a row when warps join
-  static constexpr int JOIN = kWarps * ROWS * (OROW + 2) * 4;
-  static constexpr int SMEM = RING * kWarps > JOIN ? RING * kWarps : JOIN;
-  static constexpr int CTAS = D == 256 ? (F32 || G == 32 ? 2 : 3) : D == 128 ? (F32 ? 2 : NT == 2 ? 3 : 4) : (F32 || NT == 2 ? 3 : 4);
+  static constexpr int CODE_BYTES = kTile * D / 2;         // one side's codes of a stage
+  static constexpr int STAGE = 2 * CODE_BYTES + 4 * kTile * SROW;
+  static constexpr int AFFINE = kTile * NG * 8;            // scales and biases of a stage's side as float pairs
+  // blocks to an SM (their registers: 65536 / (128 CTAS) to a thread), and as many stages as their share of
+  // the SM's 228 KB holds beside the 1 KB that each block costs
+  static constexpr int CTAS = D == 256 ? 2 : D == 128 ? (F32 || NT == 2 ? 2 : 3) : (F32 || NT == 2 ? 3 : 4);
+  static constexpr int SHARE = (228 / CTAS - 1) * 1024 / kWarps;
+  static constexpr int STAGES = (SHARE - AFFINE) / STAGE < 4 ? (SHARE - AFFINE) / STAGE : 4;
+  static_assert(STAGES >= 2, "a ring needs two stages");
+  static constexpr int RING = STAGE * STAGES + AFFINE;          // per warp
+  static constexpr int SMEM = RING * kWarps;
 };
 
 // ---- small pieces ---------------------------------------------------------
@@ -114,11 +134,15 @@ template <typename T, int D_, int G_, int NT_> struct Shape {
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
-template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int valid) {
+template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
   if constexpr (N == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(valid) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+}
+// four bytes of which `valid` are read, the rest zero
+__device__ __forceinline__ void copy_async_upto4(uint32_t dst, const void* src, int valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -138,48 +162,32 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-
 template <typename T> __device__ __forceinline__ uint32_t pack_out(float lo, float hi) {
   return static_cast<uint32_t>(from_f32<T>(lo).bits) | static_cast<uint32_t>(from_f32<T>(hi).bits) << 16;
 }
 
-// (a & b) | c
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-
-// Codes u and u + 4 of w's two 16-bit halves' (bits 4u and 16 + 4u) as a pair of bf16 code - 8:
-// 0x4300 | n is 128 + n, and 128 + n - 136 is exact.
-template <int U> __device__ __forceinline__ uint32_t pair_bf16(uint32_t w) {
-  uint32_t d;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(and_or(w >> (4 * U), 0x000f000fu, 0x43004300u)), "r"(0x43084308u));
-  return d;
-}
-// The same as f16: with the code one digit further left 0x5400 | n << 4 is 64 + n.
-template <int U> __device__ __forceinline__ uint32_t pair_f16(uint32_t w) {
-  uint32_t d;
-  const uint32_t x = U == 0 ? w << 4 : w >> (U == 0 ? 0 : 4 * U - 4);
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(and_or(x, 0x00f000f0u, 0x54005400u)), "r"(0x54805480u));
-  return d;
-}
-
-template <bool HALF>
+// c += a b and c = a b, f16 with fp32 sums.
 __device__ __forceinline__ void mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  if constexpr (HALF)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_first(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// Two values rounded to f16 (lo in the low half); `rest`: what is left of them.
+template <bool REST> __device__ __forceinline__ uint32_t take_f16(float& lo, float& hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  if constexpr (REST) {
+    lo -= to_f32(f16{static_cast<uint16_t>(d)});
+    hi -= to_f32(f16{static_cast<uint16_t>(d >> 16)});
+  }
+  return d;
 }
 
 // 8 x 8 transpose of 16-bit elements across the warp.
@@ -209,61 +217,91 @@ __device__ __forceinline__ int key_of_slot(int i) { return (i & ~7) | ((i >> 1) 
 // ---- one warp's stage ring --------------------------------------------------
 
 template <typename S, typename T> struct Ring {
+  static constexpr int CH = S::D / 32;  // 16-byte chunks of a row
+  static constexpr int RP = 32 / CH;    // rows that one copy of the warp covers
   const Cache& c;
-  uint32_t base;     // shared address of this warp's stages
-  uint32_t* parity;  // per stage: odd rows (scales of two bytes: which half of the loaded word)
+  uint32_t base;    // shared address of this warp's stages, then of its float pairs
   int lane;
+  uint32_t odd;     // bit s: this lane's row of stage s is odd (two-byte scales: which half of the loaded word)
 
-  // Starts the copy of the 32 rows that the lanes hold into stage `s`.
-  __device__ __forceinline__ void issue(int s, uint32_t row) const {
+  __device__ __forceinline__ uint32_t pairs() const { return base + S::STAGE * S::STAGES; }
+
+  // Starts the copy of the 32 rows that the lanes hold into stage `s`; EIGHTS: rows of eight keys lie side by side.
+  template <bool EIGHTS> __device__ __forceinline__ void issue(int s, uint32_t row) {
     const uint32_t at = base + s * S::STAGE;
-    constexpr int CH = S::D / 32;  // 16-byte chunks of a row
-#pragma unroll
-    for (int side = 0; side < 2; ++side) {
+    const int ch = lane % CH, sub = lane / CH;
+    constexpr uint32_t ROW = S::D / 2;
+    if constexpr (EIGHTS && RP % 8 == 0) {
+      // one row number to RP / 8 eights: the rest of a lane's row is its place among the eight
+      const uint32_t k_off = key_of_slot(sub & 7) * ROW + ch * 16, v_off = (sub & 7) * ROW + ch * 16;
+      const char* k = reinterpret_cast<const char*>(c.codes[0]) + k_off;
+      const char* v = reinterpret_cast<const char*>(c.codes[1]) + v_off;
+      const uint32_t dst = at + sub * ROW + swizzle<S::D>(sub, ch) * 16;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
-        const int id = i * 32 + lane, r = id / CH, ch = id % CH;
-        const uint32_t src = __shfl_sync(0xffffffffu, row, side == 0 ? key_of_slot(r) : r);
-        const bool have = src != kNoRow;
-        copy_async<16>(at + side * S::CODE_BYTES + r * (S::D / 2) + swizzle<S::D>(r, ch) * 16,
-                       c.codes[side] + (have ? static_cast<int64_t>(src) * (S::D / 8) + ch * 4 : 0), have ? 16 : 0);
+        const uint32_t src = __shfl_sync(0xffffffffu, row, i * RP + (RP == 8 ? 0 : sub & ~7));
+        copy_async<16>(dst + i * RP * ROW, k + static_cast<uint64_t>(src) * ROW);
+        copy_async<16>(dst + S::CODE_BYTES + i * RP * ROW, v + static_cast<uint64_t>(src) * ROW);
+      }
+    } else {
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        const char* codes = reinterpret_cast<const char*>(c.codes[side]) + ch * 16;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          const int r = i * RP + sub;
+          const uint32_t src = __shfl_sync(0xffffffffu, row, side == 0 ? key_of_slot(r) : r);
+          copy_async<16>(at + side * S::CODE_BYTES + r * ROW + swizzle<S::D>(r, ch) * 16,
+                         codes + static_cast<uint64_t>(src) * ROW);
+        }
       }
     }
-    const bool have = row != kNoRow;
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
       const char* arr = static_cast<const char*>((a & 1) ? c.biases[a >> 1] : c.scales[a >> 1]);
-      const uint32_t dst = at + 2 * S::CODE_BYTES + (a * kStageKeys + lane) * S::SROW;
+      const uint32_t dst = at + 2 * S::CODE_BYTES + (a * kTile + lane) * S::SROW;
       if constexpr (S::SB == 2) {
         // the aligned word around the two bytes; the array's last row alone has no partner behind it
-        const int64_t off = (static_cast<int64_t>(have ? row : 0) * 2) & ~3ll;
         const uint32_t rows = static_cast<uint32_t>(c.map.pages) * static_cast<uint32_t>(c.map.kv_heads) *
                               static_cast<uint32_t>(c.map.page_size);
-        copy_async<4>(dst, arr + off, !have ? 0 : (row | 1u) < rows ? 4 : 2);
+        copy_async_upto4(dst, arr + static_cast<uint64_t>(row & ~1u) * 2, (row | 1u) < rows ? 4 : 2);
       } else {
         constexpr int N = S::SB < 16 ? S::SB : 16;
 #pragma unroll
-        for (int i = 0; i < S::SB; i += N)
-          copy_async<N>(dst + i, arr + (have ? static_cast<int64_t>(row) * S::SB + i : 0), have ? N : 0);
+        for (int i = 0; i < S::SB; i += N) copy_async<N>(dst + i, arr + static_cast<uint64_t>(row) * S::SB + i);
       }
     }
-    if constexpr (S::SB == 2) {
-      const uint32_t odd = __ballot_sync(0xffffffffu, row & 1);
-      if (lane == 0) parity[s] = odd;
-    }
+    if constexpr (S::SB == 2) odd = (odd & ~(1u << s)) | ((row & 1u) << s);
     copy_commit();
   }
 
-  // Scales (which = 0) or biases (1) of key `key` of stage `s` on one side, as floats.
-  __device__ __forceinline__ void scales(int s, int side, int which, int key, float* out) const {
-    const uint32_t at = base + s * S::STAGE + 2 * S::CODE_BYTES + ((side * 2 + which) * kStageKeys + key) * S::SROW;
+  // Scales and biases of a side of stage `s`, a key to a lane; nothing for a lane without a key.
+  __device__ __forceinline__ void load(int s, int side, bool have, float* sc, float* bi) const {
+    const uint32_t at = base + s * S::STAGE + 2 * S::CODE_BYTES + (side * 2 * kTile + lane) * S::SROW;
+    read(at, s, sc);
+    read(at + kTile * S::SROW, s, bi);
+#pragma unroll
+    for (int g = 0; g < S::NG; ++g)
+      if (!have) sc[g] = bi[g] = 0.f;
+  }
+  // ... for the whole warp to read, as pairs of floats.
+  __device__ __forceinline__ void share(const float* sc, const float* bi) const {
+    const uint32_t dst = pairs() + lane * S::NG * 8;
+    if constexpr (S::NG == 1) {
+      asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(dst), "f"(sc[0]), "f"(bi[0]) : "memory");
+    } else {
+#pragma unroll
+      for (int g = 0; g < S::NG; g += 2)
+        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + g * 8), "f"(sc[g]), "f"(bi[g]),
+                     "f"(sc[g + 1]), "f"(bi[g + 1])
+                     : "memory");
+    }
+  }
+  __device__ __forceinline__ void read(uint32_t at, int s, float* out) const {
     if constexpr (S::SB == 2) {
       uint32_t w;
       load_words<1>(at, &w);
-      if ((parity[s] >> key) & 1) w >>= 16;
-      T t;
-      t.bits = static_cast<uint16_t>(w);
-      out[0] = to_f32(t);
+      out[0] = to_f32(T{static_cast<uint16_t>((odd >> s) & 1 ? w >> 16 : w)});
     } else {
       uint32_t w[S::SB / 4];
       constexpr int N = S::SB < 16 ? S::SB / 4 : 4;
@@ -271,14 +309,24 @@ template <typename S, typename T> struct Ring {
       for (int i = 0; i < S::SB / 4; i += N) load_words<N>(at + i * 4, w + i);
 #pragma unroll
       for (int g = 0; g < S::NG; ++g) {
-        if constexpr (S::F32) {
+        if constexpr (S::F32)
           out[g] = __uint_as_float(w[g]);
-        } else {
-          T t;
-          t.bits = static_cast<uint16_t>(g & 1 ? w[g / 2] >> 16 : w[g / 2] & 0xffff);
-          out[g] = to_f32(t);
-        }
+        else
+          out[g] = to_f32(T{static_cast<uint16_t>(g & 1 ? w[g / 2] >> 16 : w[g / 2])});
       }
+    }
+  }
+  // Scales and biases of key `key` on the side shared last.
+  __device__ __forceinline__ void affine(int key, float* sc, float* bi) const {
+    const uint32_t at = pairs() + key * S::NG * 8;
+    if constexpr (S::NG == 1) {
+      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(sc[0]), "=f"(bi[0]) : "r"(at));
+    } else {
+#pragma unroll
+      for (int g = 0; g < S::NG; g += 2)
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(sc[g]), "=f"(bi[g]), "=f"(sc[g + 1]), "=f"(bi[g + 1])
+                     : "r"(at + g * 8));
     }
   }
 };
@@ -287,25 +335,24 @@ template <typename S, typename T> struct Ring {
 
 template <typename S, typename T>
 __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnParams p) {
-  constexpr int D = S::D, G = S::G, NT = S::NT, NG = S::NG, ROWS = S::ROWS, TQ = S::TQ, TP = S::TP;
+  constexpr int D = S::D, G = S::G, NT = S::NT, NG = S::NG, ROWS = S::ROWS, TERMS = S::TERMS;
   constexpr int WPT = G / 32;   // words of a group that one thread multiplies with the queries
   constexpr int WT = D / 32;    // of a row
-  constexpr bool HALF = std::is_same<T, f16>::value;  // f16 queries: the score product runs in f16
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t s_red[kWarps];
-  __shared__ int64_t s_prefix;
-  __shared__ int s_entry;
-  __shared__ uint32_t s_parity[kWarps][S::STAGES];
+  // (shared memory of its own would cost a block its place on the SM: these come before the ring's use of it)
+  int64_t* s_red = reinterpret_cast<int64_t*>(smem);
+  int64_t* s_prefix = s_red + kWarps;
+  int* s_entry = reinterpret_cast<int*>(s_prefix + kWarps);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r8 = lane >> 2, t4 = lane & 3;
   const int kv_heads = p.c.map.kv_heads;
 
-  // ---- this block's share of the line of tiles ----
+  // ---- this warp's share of the line ----
   const int entries = p.batch * p.blocks;
   int64_t mine = 0;
   for (int e = threadIdx.x; e < entries; e += kWarps * 32) {
     const Entry t = entry_at(p, e, ROWS);
-    mine += t.tiles;
+    mine += t.tiles + kBegin;
     if (blockIdx.x == 0 && t.block == 0 && __ldg(p.lengths + t.b) != t.length) atomicExch(p.error_flag, PHEW_ERR_INVALID);
   }
 #pragma unroll
@@ -313,21 +360,19 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
   if (lane == 0) s_red[warp] = mine;
   __syncthreads();
   const int64_t total = (s_red[0] + s_red[1] + s_red[2] + s_red[3]) * kv_heads;
-  const int64_t n = total < gridDim.x ? total : gridDim.x;
-  if (blockIdx.x >= n) {
-    if (threadIdx.x < 2) p.meta[2 * blockIdx.x + threadIdx.x] = -1;
-    return;
-  }
+  const int64_t all_warps = static_cast<int64_t>(gridDim.x) * kWarps;
+  const int64_t n = total < all_warps ? total : all_warps;
+  // neighbours on the line run on different SMs, and a short line on as many as it can
+  const int self = warp * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x);
   asm volatile("griddepcontrol.launch_dependents;");  // the combine kernel may be set up from here on; it waits for this one
-  int64_t x = total * blockIdx.x / n;
-  const int64_t x_end = total * (blockIdx.x + 1) / n;
-  // the entry that tile x belongs to: the first whose tiles, with those before it, pass x / kv_heads
+  if (blockIdx.x >= n) return;  // no warp of the block has work
+  // the entries that the warps' first units lie in: the first whose units, with those before it, pass them
   {
-    const int64_t target = x / kv_heads;
     int64_t run = 0;
+    const int64_t most = total * (min(static_cast<int64_t>((kWarps - 1) * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x)), n - 1)) / n / kv_heads;
     for (int e0 = 0; e0 < entries; e0 += kWarps * 32) {
       const int e = e0 + static_cast<int>(threadIdx.x);
-      const int64_t own = e < entries ? entry_at(p, e, ROWS).tiles : 0;
+      const int64_t own = e < entries ? entry_at(p, e, ROWS).tiles + kBegin : 0;
       int64_t inc = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -339,33 +384,42 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
       __syncthreads();
       for (int w = 0; w < warp; ++w) inc += s_red[w];
       inc += run;
-      if (inc > target && inc - own <= target) {
-        s_entry = e;
-        s_prefix = inc - own;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const int64_t target = total * (static_cast<int64_t>(w) * gridDim.x + blockIdx.x) / n / kv_heads;
+        if (inc > target && inc - own <= target) {
+          s_entry[w] = e;
+          s_prefix[w] = inc - own;
+        }
       }
       run += s_red[0] + s_red[1] + s_red[2] + s_red[3];
-      if (run > target) break;
+      if (run > most) break;
     }
     __syncthreads();
   }
-  int e = s_entry;
-  int64_t base = s_prefix * kv_heads;
-  int64_t left0 = -1, left1 = -1;  // segments of this block's two partials
+  int e = s_entry[warp];
+  int64_t base = s_prefix[warp] * kv_heads;
+  __syncthreads();  // (the ring takes the shared memory over; the last barrier)
+  if (self >= n) return;
+  int64_t x = total * self / n;
+  const int64_t x_end = total * (self + 1) / n;
 
-  const Ring<S, T> ring{p.c, smem_addr(smem) + warp * S::RING, s_parity[warp], lane};
+  Ring<S, T> ring{p.c, smem_addr(smem) + warp * S::RING, lane, 0u};
 
   while (x < x_end) {
     const Entry ent = entry_at(p, e, ROWS);
-    for (; x < x_end && x < base + static_cast<int64_t>(kv_heads) * ent.tiles;) {
-      const int h = static_cast<int>((x - base) / ent.tiles);
-      const int64_t seg0 = base + static_cast<int64_t>(h) * ent.tiles;
-      const int t0 = static_cast<int>(x - seg0);
-      const int t1 = static_cast<int>((x_end < seg0 + ent.tiles ? x_end : seg0 + ent.tiles) - seg0);
-      x = seg0 + t1;
+    const int units = ent.tiles + kBegin;
+    for (; x < x_end && x < base + static_cast<int64_t>(kv_heads) * units;) {
+      const int h = static_cast<int>((x - base) / units);
+      const int64_t seg0 = base + static_cast<int64_t>(h) * units;
+      const int t0 = max(static_cast<int>(x - seg0) - kBegin, 0);
+      x = min(x_end, seg0 + units);
+      const int t1 = static_cast<int>(x - seg0) - kBegin;
+      if (t1 <= t0) continue;  // units of the begin alone
 
       // ---- queries as the n operand, their group sums, and how far each row sees ----
-      uint32_t qf[NT][TQ][WT][4];
-      float qs[NT][2][NG];
+      uint32_t qf[NT][TERMS][WT][4];
+      float qs[NT][2][NG], unit[NT][2];  // a score is unit times what the product gives
       int lim[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -373,54 +427,57 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
         const int tok = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(r)));
         const bool have = tok < ent.count;
         const T* q = static_cast<const T*>(p.q) + ent.b * p.st[2] + (h * p.per + (r - tok * p.per)) * p.st[1] + tok * p.st[0];
+        float v[WT][8], top = 0.f;
+#pragma unroll
+        for (int w = 0; w < WT; ++w) {
+          uint4 raw[sizeof(T) / 2];
+#pragma unroll
+          for (int k = 0; k < static_cast<int>(sizeof(T)) / 2; ++k)
+            raw[k] = have ? __ldg(reinterpret_cast<const uint4*>(q + (w / WPT) * G + (t4 * WPT + w % WPT) * 8) + k)
+                          : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            v[w][k] = to_f32(reinterpret_cast<const T*>(raw)[k]);
+            top = fmaxf(top, fabsf(v[w][k]));
+          }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // the row's largest magnitude to [2^14, 2^15)
+        const uint32_t e = max(__float_as_uint(top) >> 23, 20u);
+        const float up = __uint_as_float((268u - e) << 23);
+        const float row_unit = p.scale_log2 * __uint_as_float((e - 14u) << 23);  // scale / up
         float sum[NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           sum[g] = 0.f;
 #pragma unroll
-          for (int i = 0; i < WPT; ++i) {
-            float v[8];
-            const T* at = q + g * G + (t4 * WPT + i) * 8;
+          for (int i = 0; i < WPT; ++i)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = 0.f;
-            if (have) {
-              T raw[8];
-#pragma unroll
-              for (int k = 0; k < static_cast<int>(sizeof(T)) / 2; ++k)
-                *reinterpret_cast<uint4*>(raw + k * (16 / sizeof(T))) = __ldg(reinterpret_cast<const uint4*>(at) + k);
-#pragma unroll
-              for (int k = 0; k < 8; ++k) v[k] = to_f32(raw[k]);
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) sum[g] += v[k];
-#pragma unroll
-            for (int tq = 0; tq < TQ; ++tq)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                uint32_t w;
-                if constexpr (HALF) {
-                  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(v[k + 4]), "f"(v[k]));
-                } else {
-                  w = pack_bf16(v[k], v[k + 4]);
-                  if (tq + 1 < TQ) {  // what the next term still has to carry
-                    v[k] -= __uint_as_float(w << 16);
-                    v[k + 4] -= __uint_as_float(w & 0xffff0000u);
-                  }
-                }
-                qf[nt][tq][g * WPT + i][k] = w;
-              }
-          }
+            for (int k = 0; k < 8; ++k) sum[g] += v[g * WPT + i][k];
           sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
           sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+          sum[g] *= up;
+        }
+#pragma unroll
+        for (int w = 0; w < WT; ++w) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[w][k] *= k & 1 ? up * 0.0625f : up;  // odd codes count sixteenfold
+#pragma unroll
+          for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) qf[nt][t][w][k] = take_f16<TERMS == 2>(v[w][k], v[w][k + 4]);
         }
         // rows of the score fragment's columns: 2 t4 and 2 t4 + 1
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
+          const int from = (2 * t4 + cc) * 4;
 #pragma unroll
-          for (int g = 0; g < NG; ++g) qs[nt][cc][g] = __shfl_sync(0xffffffffu, sum[g], (2 * t4 + cc) * 4);
+          for (int g = 0; g < NG; ++g) qs[nt][cc][g] = __shfl_sync(0xffffffffu, sum[g], from);
+          unit[nt][cc] = __shfl_sync(0xffffffffu, row_unit, from);
           const int rr = ent.block * ROWS + nt * 8 + 2 * t4 + cc;
           const int tok_cc = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(rr)));
-          // rows without a query run along unmasked (their weights are finite and never stored)
+          // rows without a query run along unmasked (never stored)
           lim[nt][cc] = tok_cc < ent.count ? seen_end(ent.length, ent.count, tok_cc, p.causal) : 0x7fffffff;
         }
       }
@@ -431,7 +488,12 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
       for (int o = 1; o < 4; o <<= 1) lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, o));
 
       float acc[NT][D / 16][4];
-      float m[NT][2], l[NT][2], bsum[NT][2][NG];
+      // a row's weights are 2^(score - m); m moves when a score passes it by `pass`, which is kGrow once the
+      // row has seen a key and below any score before
+      float m[NT][2], pass[NT][2], l[NT][2], bsum[NT][2][NG];
+      constexpr int SUM_TILES = (NG + 1) / 2;
+      float ones[NT][SUM_TILES][4];  // CENTRED: sums of the rounded weights, two groups to a tile
+      float v_up = 0x1p60f;          // value scales are taken times this
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -439,71 +501,76 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
 #pragma unroll
           for (int k = 0; k < 4; ++k) acc[nt][i][k] = 0.f;
 #pragma unroll
+        for (int g = 0; g < SUM_TILES; ++g)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) ones[nt][g][k] = 0.f;
+#pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
-          m[nt][cc] = kFloor;
+          m[nt][cc] = 0.f;
+          pass[nt][cc] = kFloor;
           l[nt][cc] = 0.f;
 #pragma unroll
           for (int g = 0; g < NG; ++g) bsum[nt][cc][g] = 0.f;
         }
       }
 
-      // ---- the ring: page numbers one stage ahead of the copies, copies STAGES - 1 ahead of the products ----
+      // ---- the ring: page numbers one stage ahead of the copies, copies STAGES - 1 ahead of the products.
+      // A lane without a key copies row 0 of the cache: whatever it holds is masked. ----
       const int steps = t1 - t0;
-      int want_page = -1, want_r = 0;  // -1: no key
+      int key = t0 * kTile + lane;  // of the next look-up
+      int col = static_cast<int>(div_by(p.c.map.by_page, static_cast<uint32_t>(key)));
+      int in_page = key - col * p.c.map.page_size;
+      const int32_t* pages = p.c.map.table ? p.c.map.table + ent.b * p.c.map.table_stride : nullptr;
+      const uint32_t head_row = static_cast<uint32_t>(h) * static_cast<uint32_t>(p.c.map.page_size);
+      const int key_end = min(ent.end, t1 * kTile);
+      int want_page = 0;
+      uint32_t want_r = 0;
       bool want = false;
-      auto look_up = [&](int i) {
-        const int key = (t0 + i) * kTile + warp * kStageKeys + lane;
-        want = i < steps && key < ent.end;
-        if (want) {
-          const int col = static_cast<int>(div_by(p.c.map.by_page, static_cast<uint32_t>(key)));
-          want_r = key - col * p.c.map.page_size;
-          want_page = page_at(p.c.map, ent.b, col);
+      auto look_up = [&]() {
+        want = key < key_end;
+        if (want) want_page = pages ? __ldg(pages + col) : ent.b;
+        want_r = head_row + static_cast<uint32_t>(in_page);
+        key += kTile;
+        in_page += p.step_row;
+        col += p.step_col;
+        if (in_page >= p.c.map.page_size) {
+          in_page -= p.c.map.page_size;
+          ++col;
         }
       };
-      auto start_copy = [&](int i) {
-        uint32_t row = kNoRow;
-        if (want) {
-          if (page_ok(p.c.map, want_page))
-            row = row_at(p.c.map, want_page, h, want_r);
+      int left = steps, st_in = 0, st_out = 0;  // copies still to start, and the stages that come next
+      auto start_copy = [&]() {
+        if (left > 0) {
+          uint32_t row = 0;
+          if (want) {
+            if (page_ok(p.c.map, want_page))
+              row = static_cast<uint32_t>(want_page) * p.page_rows + want_r;
+            else
+              atomicExch(p.error_flag, PHEW_ERR_INVALID);
+          }
+          if (p.eights)
+            ring.template issue<true>(st_in, row);
           else
-            atomicExch(p.error_flag, PHEW_ERR_INVALID);
-        }
-        if (i < steps)
-          ring.issue(i % S::STAGES, row);
-        else
+            ring.template issue<false>(st_in, row);
+          st_in = st_in + 1 == S::STAGES ? 0 : st_in + 1;
+          --left;
+        } else {
           copy_commit();
+        }
       };
-      look_up(0);
-#pragma unroll
-      for (int i = 0; i < S::STAGES - 1; ++i) {
-        start_copy(i);
-        look_up(i + 1);
-      }
-      for (int i = 0; i < steps; ++i) {
-        copy_wait<S::STAGES - 2>();
-        __syncwarp();
-        start_copy(i + S::STAGES - 1);
-        look_up(i + S::STAGES);
-        const int key0 = (t0 + i) * kTile + warp * kStageKeys;
-        if (key0 >= ent.end) continue;
-        const int st = i % S::STAGES;
-        const uint32_t k_at = ring.base + st * S::STAGE, v_at = k_at + S::CODE_BYTES;
+      const int my_key = key_of_slot(r8);
 
+      // One stage of 32 keys; EDGE: some row does not see all of them.
+      auto stage = [&](int st, int key0, auto edge_c) {
+        constexpr bool EDGE = decltype(edge_c)::value;
+        const uint32_t k_at = ring.base + st * S::STAGE, v_at = k_at + S::CODE_BYTES;
         // ---- scores of 2 x 16 keys: rows r8, r8 + 8 of the fragment hold keys key_of_slot(r8), + 8 ----
         float s[2][NT][4];
-        const int my_key = key_of_slot(r8);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-          float sk[2][NG], bk[2][NG];
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            ring.scales(st, 0, 0, kb * 16 + half * 8 + my_key, sk[half]);
-            ring.scales(st, 0, 1, kb * 16 + half * 8 + my_key, bk[half]);
-          }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) s[kb][nt][k] = 0.f;
+          float sk[2][NG], zk[2][NG];
+          ring.affine(kb * 16 + my_key, sk[0], zk[0]);
+          ring.affine(kb * 16 + 8 + my_key, sk[1], zk[1]);
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
             uint32_t wa[WPT], wb[WPT];
@@ -512,43 +579,33 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
             load_words<WPT>(k_at + (r0 + 8) * (D / 2) + swizzle<D>(r0 + 8, word >> 2) * 16 + (word & 3) * 4, wb);
             float d[NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) d[nt][k] = 0.f;
-#pragma unroll
             for (int w = 0; w < WPT; ++w) {
-              uint32_t a[4], b[4];
-              if constexpr (HALF) {
-                a[0] = pair_f16<0>(wa[w]); a[1] = pair_f16<1>(wa[w]); a[2] = pair_f16<2>(wa[w]); a[3] = pair_f16<3>(wa[w]);
-                b[0] = pair_f16<0>(wb[w]); b[1] = pair_f16<1>(wb[w]); b[2] = pair_f16<2>(wb[w]); b[3] = pair_f16<3>(wb[w]);
-              } else {
-                a[0] = pair_bf16<0>(wa[w]); a[1] = pair_bf16<1>(wa[w]); a[2] = pair_bf16<2>(wa[w]); a[3] = pair_bf16<3>(wa[w]);
-                b[0] = pair_bf16<0>(wb[w]); b[1] = pair_bf16<1>(wb[w]); b[2] = pair_bf16<2>(wb[w]); b[3] = pair_bf16<3>(wb[w]);
-              }
+              const uint32_t ya = wa[w] >> 8, yb = wb[w] >> 8;
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int tq = TQ - 1; tq >= 0; --tq) {
-                  const uint32_t* q = qf[nt][tq][g * WPT + w];
-                  mma<HALF>(d[nt], a[0], b[0], a[1], b[1], q[0], q[1]);
-                  mma<HALF>(d[nt], a[2], b[2], a[3], b[3], q[2], q[3]);
+                for (int t = TERMS - 1; t >= 0; --t) {
+                  const uint32_t* q = qf[nt][t][g * WPT + w];
+                  if (w == 0 && t == TERMS - 1)
+                    mma_first(d[nt], wa[w] & kEven, wb[w] & kEven, wa[w] & kOdd, wb[w] & kOdd, q[0], q[1]);
+                  else
+                    mma(d[nt], wa[w] & kEven, wb[w] & kEven, wa[w] & kOdd, wb[w] & kOdd, q[0], q[1]);
+                  mma(d[nt], ya & kEven, yb & kEven, ya & kOdd, yb & kOdd, q[2], q[3]);
                 }
             }
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const float z = fmaf(8.f, sk[half][g], bk[half][g]);
+            for (int half = 0; half < 2; ++half)
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int cc = 0; cc < 2; ++cc) {
                   float& y = s[kb][nt][2 * half + cc];
-                  y = fmaf(sk[half][g], d[nt][2 * half + cc], fmaf(z, qs[nt][cc][g], y));
+                  y = g == 0 ? zk[half][g] * qs[nt][cc][g] : fmaf(zk[half][g], qs[nt][cc][g], y);
+                  y = fmaf(sk[half][g], d[nt][2 * half + cc], y);
                 }
-            }
           }
         }
         // ---- running maximum: moved only when a score passes it by kGrow, so weights stay below 2^kGrow ----
-        const bool edge = key0 + kStageKeys > lim_min;
         bool grow = false;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -557,9 +614,9 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               float& y = s[kb][nt][k];
-              y *= p.scale_log2;
-              if (edge && key0 + kb * 16 + (k >> 1) * 8 + my_key >= lim[nt][k & 1]) y = -INFINITY;
-              grow = grow || y > m[nt][k & 1] + kGrow;
+              y = fmaf(unit[nt][k & 1], y, -m[nt][k & 1]);
+              if (EDGE && key0 + kb * 16 + (k >> 1) * 8 + my_key >= lim[nt][k & 1]) y = -INFINITY;
+              grow = grow || y > pass[nt][k & 1];
             }
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -569,34 +626,80 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
               float top = fmaxf(fmaxf(s[0][nt][cc], s[0][nt][2 + cc]), fmaxf(s[1][nt][cc], s[1][nt][2 + cc]));
 #pragma unroll
               for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-              const float m_new = fmaxf(m[nt][cc], top);
-              const float alpha = exp2_fast(m[nt][cc] - m_new);
-              m[nt][cc] = m_new;
+              const bool move = top > pass[nt][cc];
+              const float by = move ? top : 0.f;
+              const float alpha = exp2_fast(fminf(-by, 0.f));  // (a row's first keys find nothing to scale)
+              if (move) pass[nt][cc] = kGrow;
+              m[nt][cc] += by;
               l[nt][cc] *= alpha;
 #pragma unroll
               for (int g = 0; g < NG; ++g) bsum[nt][cc][g] *= alpha;
+#pragma unroll
+              for (int g = 0; g < SUM_TILES; ++g) {
+                ones[nt][g][cc] *= alpha;
+                ones[nt][g][2 + cc] *= alpha;
+              }
 #pragma unroll
               for (int j = 0; j < D / 16; ++j) {
                 acc[nt][j][cc] *= alpha;
                 acc[nt][j][2 + cc] *= alpha;
               }
+#pragma unroll
+              for (int kb = 0; kb < 2; ++kb) {
+                s[kb][nt][cc] -= by;
+                s[kb][nt][2 + cc] -= by;
+              }
             }
+        }
+        // ---- value scales, at most 2^7 times a power of two that only shrinks ----
+        {
+          float sv[NG], zv[NG];
+          ring.load(st, 1, !EDGE || key0 + lane < ent.end, sv, zv);
+          float top = 0.f;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) top = fmaxf(top, fabsf(sv[g]));
+          if (__any_sync(0xffffffffu, top * v_up > 128.f && top < INFINITY)) {
+            if (!(top < INFINITY)) top = 0.f;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float to = __uint_as_float(min(260u - (__float_as_uint(top) >> 23), 187u) << 23);  // top to [64, 128)
+            const float f = to / v_up;
+            v_up = to;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[nt][i][k] *= f;
+#pragma unroll
+              for (int g = 0; g < SUM_TILES; ++g)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) ones[nt][g][k] *= f;
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            if (S::CENTRED) zv[g] = fmaf(8.f, sv[g], zv[g]);
+            sv[g] *= v_up;
+          }
+          __syncwarp();
+          ring.share(sv, zv);
+          __syncwarp();
         }
         // ---- weights, their sums, and the second product ----
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-          uint32_t pb[NT][NG][TP][2];
+          uint32_t pb[NT][NG][TERMS][2];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            float sv[NG], bv[NG];
-            ring.scales(st, 1, 0, kb * 16 + half * 8 + my_key, sv);
-            ring.scales(st, 1, 1, kb * 16 + half * 8 + my_key, bv);
+            float sv[NG], zv[NG];
+            ring.affine(kb * 16 + half * 8 + my_key, sv, zv);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               float w[2];
 #pragma unroll
               for (int cc = 0; cc < 2; ++cc) {
-                w[cc] = exp2_fast(s[kb][nt][2 * half + cc] - m[nt][cc]);
+                w[cc] = exp2_fast(s[kb][nt][2 * half + cc]);
                 l[nt][cc] += w[cc];
               }
 #pragma unroll
@@ -604,24 +707,28 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
                 float f[2];
 #pragma unroll
                 for (int cc = 0; cc < 2; ++cc) {
-                  f[cc] = w[cc] * sv[g];
-                  float z = w[cc] * fmaf(8.f, sv[g], bv[g]);
-                  if (edge && w[cc] == 0.f) f[cc] = z = 0.f;  // a key this row does not see may hold anything
-                  bsum[nt][cc][g] += z;
+                  // a key that this row does not see may hold anything
+                  const bool none = EDGE && w[cc] == 0.f;
+                  f[cc] = none ? 0.f : w[cc] * sv[g];
+                  bsum[nt][cc][g] = none ? bsum[nt][cc][g] : fmaf(w[cc], zv[g], bsum[nt][cc][g]);
                 }
 #pragma unroll
-                for (int tp = 0; tp < TP; ++tp) {
-                  const uint32_t pk = pack_bf16(f[0], f[1]);
-                  if (tp + 1 < TP) {
-                    f[0] -= __uint_as_float(pk << 16);
-                    f[1] -= __uint_as_float(pk & 0xffff0000u);
-                  }
-                  pb[nt][g][tp][half] = transpose8(pk);
-                }
+                for (int t = 0; t < TERMS; ++t) pb[nt][g][t][half] = transpose8(take_f16<TERMS == 2>(f[0], f[1]));
               }
             }
           }
-          const int key = kb * 16 + t4;  // keys key, + 4, + 8, + 12
+          if constexpr (S::CENTRED) {
+            constexpr uint32_t one = 0x3c003c00u;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int t = TERMS - 1; t >= 0; --t)
+                  mma(ones[nt][g / 2], g & 1 ? 0u : one, g & 1 ? one : 0u, g & 1 ? 0u : one, g & 1 ? one : 0u,
+                      pb[nt][g][t][0], pb[nt][g][t][1]);
+          }
+          const int vk = kb * 16 + t4;  // keys vk, + 4, + 8, + 12
           if constexpr (G >= 64) {
 #pragma unroll
             for (int j = 0; j < D / 64; ++j) {
@@ -629,20 +736,20 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
               uint32_t w[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                load_words<1>(v_at + (key + 4 * k) * (D / 2) + swizzle<D>(key + 4 * k, word >> 2) * 16 + (word & 3) * 4, &w[k]);
+                load_words<1>(v_at + (vk + 4 * k) * (D / 2) + swizzle<D>(vk + 4 * k, word >> 2) * 16 + (word & 3) * 4, &w[k]);
               const uint32_t x0 = __byte_perm(w[0], w[1], 0x5410), x1 = __byte_perm(w[0], w[1], 0x7632);
               const uint32_t y0 = __byte_perm(w[2], w[3], 0x5410), y1 = __byte_perm(w[2], w[3], 0x7632);
               auto tile = [&](int u, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                  for (int tp = TP - 1; tp >= 0; --tp)
-                    mma<false>(acc[nt][j * 4 + u], a0, a1, a2, a3, pb[nt][g][tp][0], pb[nt][g][tp][1]);
+                  for (int t = TERMS - 1; t >= 0; --t)
+                    mma(acc[nt][j * 4 + u], a0, a1, a2, a3, pb[nt][g][t][0], pb[nt][g][t][1]);
               };
-              tile(0, pair_bf16<0>(x0), pair_bf16<0>(x1), pair_bf16<0>(y0), pair_bf16<0>(y1));
-              tile(1, pair_bf16<1>(x0), pair_bf16<1>(x1), pair_bf16<1>(y0), pair_bf16<1>(y1));
-              tile(2, pair_bf16<2>(x0), pair_bf16<2>(x1), pair_bf16<2>(y0), pair_bf16<2>(y1));
-              tile(3, pair_bf16<3>(x0), pair_bf16<3>(x1), pair_bf16<3>(y0), pair_bf16<3>(y1));
+              tile(0, x0 & kEven, x1 & kEven, y0 & kEven, y1 & kEven);
+              tile(1, x0 & kOdd, x1 & kOdd, y0 & kOdd, y1 & kOdd);
+              tile(2, (x0 >> 8) & kEven, (x1 >> 8) & kEven, (y0 >> 8) & kEven, (y1 >> 8) & kEven);
+              tile(3, (x0 >> 8) & kOdd, (x1 >> 8) & kOdd, (y0 >> 8) & kOdd, (y1 >> 8) & kOdd);
             }
           } else {
             // groups of four words: a fragment's eight rows are the two halves of each
@@ -653,175 +760,217 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
               uint32_t w[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                load_words<1>(v_at + (key + 4 * k) * (D / 2) + swizzle<D>(key + 4 * k, word >> 2) * 16 + (word & 3) * 4, &w[k]);
+                load_words<1>(v_at + (vk + 4 * k) * (D / 2) + swizzle<D>(vk + 4 * k, word >> 2) * 16 + (word & 3) * 4, &w[k]);
               const uint32_t x0 = __byte_perm(w[0], w[1], pick), y0 = __byte_perm(w[2], w[3], pick);
               auto tile = [&](int u, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                  for (int tp = TP - 1; tp >= 0; --tp)
-                    mma<false>(acc[nt][g * 2 + u], a0, a1, a2, a3, pb[nt][g][tp][0], pb[nt][g][tp][1]);
+                  for (int t = TERMS - 1; t >= 0; --t)
+                    mma(acc[nt][g * 2 + u], a0, a1, a2, a3, pb[nt][g][t][0], pb[nt][g][t][1]);
               };
-              tile(0, pair_bf16<0>(x0), pair_bf16<2>(x0), pair_bf16<0>(y0), pair_bf16<2>(y0));
-              tile(1, pair_bf16<1>(x0), pair_bf16<3>(x0), pair_bf16<1>(y0), pair_bf16<3>(y0));
+              // (codes 0 and 2, then 1 and 3 of a half: both even or both odd)
+              tile(0, x0 & kEven, (x0 >> 8) & kEven, y0 & kEven, (y0 >> 8) & kEven);
+              tile(1, x0 & kOdd, (x0 >> 8) & kOdd, y0 & kOdd, (y0 >> 8) & kOdd);
             }
           }
         }
+      };
+
+      look_up();
+#pragma unroll
+      for (int i = 0; i < S::STAGES - 1; ++i) {
+        start_copy();
+        look_up();
+      }
+      for (int key0 = t0 * kTile; key0 < t1 * kTile; key0 += kTile) {
+        copy_wait<S::STAGES - 2>();
+        __syncwarp();
+        start_copy();
+        look_up();
+        if (key0 >= ent.end) break;  // (a tile without keys: the only one of its segment)
+        {
+          float sk[NG], zk[NG];
+          ring.load(st_out, 0, key0 + lane < ent.end, sk, zk);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            // (an infinite key would give scores of either infinity: no number, as its products are)
+            sk[g] = fmaf(sk[g], 0x1p24f, fmaf(0.f, sk[g], 0.f * zk[g]));
+          }
+          ring.share(sk, zk);
+        }
+        __syncwarp();
+        if (key0 + kTile > lim_min)
+          stage(st_out, key0, std::true_type());
+        else
+          stage(st_out, key0, std::false_type());
+        st_out = st_out + 1 == S::STAGES ? 0 : st_out + 1;
       }
 
-      // ---- join the warps: each writes its rows, the block adds them up ----
+      // ---- the segment's result, or this warp's part of it ----
       copy_wait<0>();
-      __syncthreads();
-      float* join = reinterpret_cast<float*>(smem);                    // [warp][ROWS][OROW]
-      float* join_ml = join + kWarps * ROWS * S::OROW;                 // [warp][ROWS][2]
+      __syncwarp();
+      const int64_t segment = static_cast<int64_t>(e) * kv_heads + h;
+      const bool whole = t0 == 0 && t1 == ent.tiles;
+      if (lane == 0) {
+        if (t0 == 0) p.span[segment].x = self;
+        if (t1 == ent.tiles) p.span[segment].y = self;
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
           const int row = nt * 8 + 2 * t4 + cc;
+          float sum = l[nt][cc];
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
-            l[nt][cc] += __shfl_xor_sync(0xffffffffu, l[nt][cc], o);
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
 #pragma unroll
             for (int g = 0; g < NG; ++g) bsum[nt][cc][g] += __shfl_xor_sync(0xffffffffu, bsum[nt][cc][g], o);
           }
-          float* dst = join + (warp * ROWS + row) * S::OROW;
+          const int r = ent.block * ROWS + row;
+          const int tok = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(r)));
+          const float inv = sum == 0.f || tok >= ent.count ? 0.f : 1.f / sum;
+          T* out = static_cast<T*>(p.o) +
+                   ((static_cast<int64_t>(ent.b) * p.heads + h * p.per + (r - tok * p.per)) * p.tokens + tok) * D;
+          const int64_t slot = (2 * static_cast<int64_t>(self) + (t0 > 0 ? 0 : 1)) * ROWS + row;
+          // `n` (4 or 8) neighbouring head dimensions from d on
+          auto put = [&](int d, const float* v, auto n_c) {
+            constexpr int N = decltype(n_c)::value;
+            if (!whole) {
+#pragma unroll
+              for (int i = 0; i < N; i += 4)
+                *reinterpret_cast<float4*>(p.part + slot * D + d + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            } else if (tok < p.tokens) {
+              float f[N];
+#pragma unroll
+              for (int i = 0; i < N; ++i) f[i] = inv == 0.f ? 0.f : v[i] * inv;
+              if constexpr (S::F32) {
+#pragma unroll
+                for (int i = 0; i < N; i += 4)
+                  *reinterpret_cast<float4*>(out + d + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+              } else if constexpr (N == 8) {
+                *reinterpret_cast<uint4*>(out + d) = make_uint4(pack_out<T>(f[0], f[1]), pack_out<T>(f[2], f[3]),
+                                                                pack_out<T>(f[4], f[5]), pack_out<T>(f[6], f[7]));
+              } else {
+                *reinterpret_cast<uint2*>(out + d) = make_uint2(pack_out<T>(f[0], f[1]), pack_out<T>(f[2], f[3]));
+              }
+            }
+          };
+          // what a sum counts: n is n 2^-24 in it, odd codes sixteenfold, value scales times v_up
+          const float even = 0x1p24f / v_up, odd = 0x1p20f / v_up;
+          auto moved = [&](int g) {  // what a group's outputs still lack
+            return S::CENTRED ? fmaf(-8.f / v_up, ones[nt][g / 2][(g & 1) * 2 + cc], bsum[nt][cc][g]) : bsum[nt][cc][g];
+          };
           if constexpr (G >= 64) {
 #pragma unroll
             for (int j = 0; j < D / 64; ++j) {
-              const float z = bsum[nt][cc][j * 64 / G];
-              float4* at = reinterpret_cast<float4*>(dst + (j * 8 + r8) * 8);
-              at[0] = make_float4(acc[nt][j * 4][cc] + z, acc[nt][j * 4 + 1][cc] + z, acc[nt][j * 4 + 2][cc] + z, acc[nt][j * 4 + 3][cc] + z);
-              at[1] = make_float4(acc[nt][j * 4][2 + cc] + z, acc[nt][j * 4 + 1][2 + cc] + z, acc[nt][j * 4 + 2][2 + cc] + z, acc[nt][j * 4 + 3][2 + cc] + z);
+              const float z = moved(j * 64 / G);
+              float v[8];
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                v[u] = fmaf(acc[nt][j * 4 + u][cc], u & 1 ? odd : even, z);
+                v[u + 4] = fmaf(acc[nt][j * 4 + u][2 + cc], u & 1 ? odd : even, z);
+              }
+              put((j * 8 + r8) * 8, v, std::integral_constant<int, 8>());
             }
           } else {
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-              const float z = bsum[nt][cc][g];
-              *reinterpret_cast<float4*>(dst + (g * 4 + (r8 & 3)) * 8 + (r8 & 4)) =
-                  make_float4(acc[nt][g * 2][cc] + z, acc[nt][g * 2 + 1][cc] + z, acc[nt][g * 2][2 + cc] + z, acc[nt][g * 2 + 1][2 + cc] + z);
+              const float z = moved(g);
+              const float v[4] = {fmaf(acc[nt][g * 2][cc], even, z), fmaf(acc[nt][g * 2 + 1][cc], odd, z),
+                                  fmaf(acc[nt][g * 2][2 + cc], even, z), fmaf(acc[nt][g * 2 + 1][2 + cc], odd, z)};
+              put((g * 4 + (r8 & 3)) * 8 + (r8 & 4), v, std::integral_constant<int, 4>());
             }
           }
-          if (r8 == 0) {
-            join_ml[(warp * ROWS + row) * 2] = m[nt][cc];
-            join_ml[(warp * ROWS + row) * 2 + 1] = l[nt][cc];
+          if (!whole && r8 == 0) {
+            p.part_ml[slot * 2] = pass[nt][cc] == kFloor ? kFloor : m[nt][cc];  // (kFloor: no key seen)
+            p.part_ml[slot * 2 + 1] = sum;
           }
         }
-      __syncthreads();
-      const bool whole = t0 == 0 && t1 == ent.tiles;
-      const int slot = t0 > 0 ? 0 : 1;
-      if (!whole) (slot == 0 ? left0 : left1) = static_cast<int64_t>(e) * kv_heads + h;
-      for (int i = threadIdx.x; i < ROWS * (D / 4); i += kWarps * 32) {
-        const int row = i / (D / 4), d4 = i % (D / 4);
-        float mm = kFloor;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, join_ml[(w * ROWS + row) * 2]);
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        float ll = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float f = exp2_fast(join_ml[(w * ROWS + row) * 2] - mm);
-          const float4 v = *reinterpret_cast<const float4*>(join + (w * ROWS + row) * S::OROW + d4 * 4);
-          ll = fmaf(f, join_ml[(w * ROWS + row) * 2 + 1], ll);
-          o.x = fmaf(f, v.x, o.x);
-          o.y = fmaf(f, v.y, o.y);
-          o.z = fmaf(f, v.z, o.z);
-          o.w = fmaf(f, v.w, o.w);
-        }
-        if (whole) {
-          const int r = ent.block * ROWS + row;
-          const int tok = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(r)));
-          if (tok < p.tokens) {
-            const float inv = ll == 0.f || tok >= ent.count ? 0.f : 1.f / ll;
-            T* dst = static_cast<T*>(p.o) +
-                     ((static_cast<int64_t>(ent.b) * p.heads + h * p.per + (r - tok * p.per)) * p.tokens + tok) * D + d4 * 4;
-            if (inv == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);
-            if constexpr (S::F32)
-              *reinterpret_cast<float4*>(dst) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-            else
-              *reinterpret_cast<uint2*>(dst) = make_uint2(pack_out<T>(o.x * inv, o.y * inv), pack_out<T>(o.z * inv, o.w * inv));
-          }
-        } else {
-          const int64_t at = (2 * static_cast<int64_t>(blockIdx.x) + slot) * ROWS + row;
-          *reinterpret_cast<float4*>(p.part + at * D + d4 * 4) = o;
-          if (d4 == 0) {
-            p.part_ml[at * 2] = mm;
-            p.part_ml[at * 2 + 1] = ll;
-          }
-        }
-      }
-      __syncthreads();  // before the next segment's copies reuse the shared memory
     }
-    base += static_cast<int64_t>(kv_heads) * ent.tiles;
+    base += static_cast<int64_t>(kv_heads) * units;
     ++e;
-  }
-  if (threadIdx.x == 0) {
-    p.meta[2 * blockIdx.x] = left0;
-    p.meta[2 * blockIdx.x + 1] = left1;
   }
 }
 
-// Joins the partials of the segment that block blockIdx.x began and left:
-// its partial 1, then the partials 0 of the blocks after it, in that order.
-// One block of the grid per row.
-template <typename S, typename T>
-__global__ void __launch_bounds__(S::D) combine_kernel(const AttnParams p, int n) {
-  constexpr int D = S::D, ROWS = S::ROWS;
-  const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
+// Joins the partials of a segment: partial 1 of its first warp, then the
+// partials 0 of the warps after it, in that order.  A warp to a row and a block
+// to a segment; or (WIDE, for segments of many partials) a block to a row, its
+// warps taking every eighth partial each, joined in shared memory.
+template <typename S, typename T, bool WIDE>
+__global__ void __launch_bounds__(256) combine_kernel(const AttnParams p) {
+  constexpr int D = S::D, ROWS = S::ROWS, E = D / 32;
+  const int segment = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // attn_kernel is done and its partials are visible
-  const int64_t seg = p.meta[2 * c + 1];
-  if (seg < 0) return;
+  const int2 span = p.span[segment];
+  if (span.x == span.y) return;
   const int kv_heads = p.c.map.kv_heads;
-  const int e = static_cast<int>(seg / kv_heads), h = static_cast<int>(seg - static_cast<int64_t>(e) * kv_heads);
+  const int e = segment / kv_heads, h = segment - e * kv_heads;
   const int b = static_cast<int>(div_by(p.by_blocks, static_cast<uint32_t>(e)));
+  const int row = WIDE ? blockIdx.y : blockIdx.y * 8 + warp;
   const int r = (e - b * p.blocks) * ROWS + row;
   const int tok = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(r)));
   if (tok >= p.tokens) return;
   const bool live = !p.counts || tok < p.counts[b];
-  __shared__ int s_last;
-  // how many blocks after c go on with the segment
-  int last = c;
-  for (int c0 = c + 1;; c0 += D) {
-    if (tid == 0) s_last = c0 + D;
-    __syncthreads();
-    if (c0 + tid >= n || p.meta[2 * (c0 + tid)] != seg) atomicMin(&s_last, c0 + tid);
-    __syncthreads();
-    last = s_last - 1;
-    __syncthreads();
-    if (last < c0 + D - 1) break;
-  }
-  auto at = [&](int k) { return (2 * static_cast<int64_t>(k) + (k == c ? 1 : 0)) * ROWS + row; };
-  __shared__ float s_max[D / 32];
+  auto at = [&](int k) { return (2 * static_cast<int64_t>(k) + (k == span.x ? 1 : 0)) * ROWS + row; };
   float mm = kFloor;
-  for (int k = c + tid; k <= last; k += D) mm = fmaxf(mm, p.part_ml[at(k) * 2]);
+  for (int k = span.x + lane; k <= span.y; k += 32) mm = fmaxf(mm, p.part_ml[at(k) * 2]);
   mm = warp_max(mm);
-  if ((tid & 31) == 0) s_max[tid >> 5] = mm;
-  __syncthreads();
+  float o[E], l = 0.f;
 #pragma unroll
-  for (int w = 0; w < D / 32; ++w) mm = fmaxf(mm, s_max[w]);
-  float o = 0.f, l = 0.f;
+  for (int i = 0; i < E; ++i) o[i] = 0.f;
 #pragma unroll 4
-  for (int k = c; k <= last; ++k) {
-    const float f = exp2_fast(p.part_ml[at(k) * 2] - mm);
-    l = fmaf(f, p.part_ml[at(k) * 2 + 1], l);
-    o = fmaf(f, p.part[at(k) * D + tid], o);
+  for (int k = span.x + (WIDE ? warp : 0); k <= span.y; k += WIDE ? 8 : 1) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at(k) * 2);
+    const float f = exp2_fast(ml.x - mm);
+    l = fmaf(f, ml.y, l);
+    const float2* v = reinterpret_cast<const float2*>(p.part + at(k) * D) + lane;
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+      const float2 x = v[i * 16];
+      o[i] = fmaf(f, x.x, o[i]);
+      o[i + 1] = fmaf(f, x.y, o[i + 1]);
+    }
   }
-  static_cast<T*>(p.o)[((static_cast<int64_t>(b) * p.heads + h * p.per + (r - tok * p.per)) * p.tokens + tok) * D + tid] =
-      from_f32<T>(l == 0.f || !live ? 0.f : o / l);
+  if constexpr (WIDE) {
+    __shared__ float s_o[8][D], s_l[8];
+#pragma unroll
+    for (int i = 0; i < E; i += 2) *reinterpret_cast<float2*>(&s_o[warp][i * 32 + lane * 2]) = make_float2(o[i], o[i + 1]);
+    if (lane == 0) s_l[warp] = l;
+    __syncthreads();
+    if (warp) return;
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      l += s_l[w];
+#pragma unroll
+      for (int i = 0; i < E; i += 2) {
+        o[i] += s_o[w][i * 32 + lane * 2];
+        o[i + 1] += s_o[w][i * 32 + lane * 2 + 1];
+      }
+    }
+  }
+  const float inv = l == 0.f || !live ? 0.f : 1.f / l;
+  T* out = static_cast<T*>(p.o) + ((static_cast<int64_t>(b) * p.heads + h * p.per + (r - tok * p.per)) * p.tokens + tok) * D + lane * 2;
+#pragma unroll
+  for (int i = 0; i < E; i += 2) {
+    const float x = inv == 0.f ? 0.f : o[i] * inv, y = inv == 0.f ? 0.f : o[i + 1] * inv;
+    if constexpr (S::F32)
+      *reinterpret_cast<float2*>(out + i * 32) = make_float2(x, y);
+    else
+      *reinterpret_cast<uint32_t*>(out + i * 32) = pack_out<T>(x, y);
+  }
 }
 
-// What a launch of attn_kernel needs from the host.
-struct AttnPlan {
-  int rows, grid;
-  size_t bytes;
-};
-
-template <typename S> AttnPlan plan_of() {
-  AttnPlan a;
-  a.rows = S::ROWS;
-  a.grid = sm_count_current() * S::CTAS;
-  a.bytes = static_cast<size_t>(a.grid) * 2 * (static_cast<size_t>(S::ROWS) * (S::D + 2) * 4 + 8);
-  return a;
+// Blocks of a launch and its scratch bytes: partials of every warp, a span per segment.
+template <typename S> int grid_of() { return sm_count_current() * S::CTAS; }
+template <typename S> size_t part_floats() { return static_cast<size_t>(grid_of<S>()) * kWarps * 2 * S::ROWS; }
+template <typename S> int64_t blocks_of(int64_t rows) { return (rows + S::ROWS - 1) / S::ROWS; }
+template <typename S> size_t bytes_of(int64_t batch, int kv_heads, int64_t rows) {
+  return part_floats<S>() * (S::D + 2) * 4 + static_cast<size_t>(batch * kv_heads * blocks_of<S>(rows)) * sizeof(int2);
 }
 
 // Dynamic shared memory of a kernel above 48 KB, allowed once per device (bit d: done on device d).
@@ -837,29 +986,37 @@ template <typename K> int allow_smem(SmemAllowed& done, K* kernel, int bytes) {
 }
 
 template <typename S, typename T> int launch_attn(AttnParams p, void* workspace, cudaStream_t st) {
-  const AttnPlan a = plan_of<S>();
-  const int64_t rows = static_cast<int64_t>(p.tokens) * p.per;
-  p.blocks = static_cast<int>((rows + S::ROWS - 1) / S::ROWS);
-  p.by_blocks = fast_div(static_cast<uint32_t>(p.blocks));
-  PHEW_REQUIRE(static_cast<int64_t>(p.batch) * p.blocks < (1ll << 31), "phew_kv_attention: too many query rows");
-  p.meta = static_cast<int64_t*>(workspace);
-  p.part = reinterpret_cast<float*>(p.meta + 2 * a.grid);
-  p.part_ml = p.part + static_cast<size_t>(a.grid) * 2 * S::ROWS * S::D;
+  const int64_t blocks = blocks_of<S>(static_cast<int64_t>(p.tokens) * p.per);
+  const int64_t segments = p.batch * blocks * p.c.map.kv_heads;
+  PHEW_REQUIRE(segments < (1ll << 31), "phew_kv_attention: too many query rows");
+  p.blocks = static_cast<int>(blocks);
+  p.by_blocks = fast_div(static_cast<uint32_t>(blocks));
+  const int page = p.c.map.page_size;
+  p.step_col = kTile / page;
+  p.step_row = kTile % page;
+  p.page_rows = static_cast<uint32_t>(p.c.map.kv_heads) * static_cast<uint32_t>(page);
+  p.eights = page % 8 == 0;
+  p.part = static_cast<float*>(workspace);
+  p.part_ml = p.part + part_floats<S>() * S::D;
+  p.span = reinterpret_cast<int2*>(p.part_ml + part_floats<S>() * 2);
   static SmemAllowed allowed;
   if (int s = allow_smem(allowed, attn_kernel<S, T>, S::SMEM)) return s;
-  attn_kernel<S, T><<<a.grid, kWarps * 32, S::SMEM, st>>>(p);
+  attn_kernel<S, T><<<grid_of<S>(), kWarps * 32, S::SMEM, st>>>(p);
   if (int s = launch_status("kv attn_kernel")) return s;
   // a programmatic dependent: set up while attn_kernel runs
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.grid, S::ROWS);
-  cfg.blockDim = dim3(S::D);
+  // partials of a segment: about the warps that it could be spread over
+  const bool wide = segments * 16 < static_cast<int64_t>(grid_of<S>()) * kWarps;
+  cfg.gridDim = dim3(static_cast<unsigned>(segments), wide ? S::ROWS : S::NT);
+  cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  PHEW_CHECK_CUDA(cudaLaunchKernelEx(&cfg, combine_kernel<S, T>, p, static_cast<int>(a.grid)));
+  PHEW_CHECK_CUDA(wide ? cudaLaunchKernelEx(&cfg, combine_kernel<S, T, true>, p)
+                       : cudaLaunchKernelEx(&cfg, combine_kernel<S, T, false>, p));
   return launch_status("kv combine_kernel");
 }
 
@@ -890,17 +1047,17 @@ template <typename T, typename F> auto with_shape(int head_dim, int group, int64
 }
 
 // Scratch bytes and launch per type; instantiated in a translation unit each, which compile side by side.
-template <typename T> size_t attn_bytes(int head_dim, int group, int64_t rows) {
-  return with_shape<T>(head_dim, group, rows, [](auto s) { return plan_of<decltype(s)>().bytes; });
+template <typename T> size_t attn_bytes(int64_t batch, int kv_heads, int head_dim, int group, int64_t rows) {
+  return with_shape<T>(head_dim, group, rows, [&](auto s) { return bytes_of<decltype(s)>(batch, kv_heads, rows); });
 }
 template <typename T> int run_attn(const AttnParams& p, void* workspace, cudaStream_t st) {
   return with_shape<T>(p.c.head_dim, p.c.group, static_cast<int64_t>(p.tokens) * p.per,
                        [&](auto s) { return launch_attn<decltype(s), T>(p, workspace, st); });
 }
 #ifndef PHEW_KV_ATTN_TYPE
-extern template size_t attn_bytes<float>(int, int, int64_t);
-extern template size_t attn_bytes<f16>(int, int, int64_t);
-extern template size_t attn_bytes<bf16>(int, int, int64_t);
+extern template size_t attn_bytes<float>(int64_t, int, int, int, int64_t);
+extern template size_t attn_bytes<f16>(int64_t, int, int, int, int64_t);
+extern template size_t attn_bytes<bf16>(int64_t, int, int, int, int64_t);
 extern template int run_attn<float>(const AttnParams&, void*, cudaStream_t);
 extern template int run_attn<f16>(const AttnParams&, void*, cudaStream_t);
 extern template int run_attn<bf16>(const AttnParams&, void*, cudaStream_t);

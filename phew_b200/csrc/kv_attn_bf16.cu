@@ -5,7 +5,7 @@
 namespace phew {
 namespace kv {
 
-template size_t attn_bytes<PHEW_KV_ATTN_TYPE>(int, int, int64_t);
+template size_t attn_bytes<PHEW_KV_ATTN_TYPE>(int64_t, int, int, int, int64_t);
 template int run_attn<PHEW_KV_ATTN_TYPE>(const AttnParams&, void*, cudaStream_t);
 
 }  // namespace kv
