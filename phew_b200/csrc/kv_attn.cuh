@@ -340,82 +340,159 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
   constexpr int WT = D / 32;    // of a row
   extern __shared__ __align__(128) uint8_t smem[];
   // (shared memory of its own would cost a block its place on the SM: these come before the ring's use of it)
-  int64_t* s_red = reinterpret_cast<int64_t*>(smem);
-  int64_t* s_prefix = s_red + kWarps;
-  int* s_entry = reinterpret_cast<int*>(s_prefix + kWarps);
+  uint64_t* s_red = reinterpret_cast<uint64_t*>(smem);
+  uint64_t* s_prefix = s_red + kWarps;
+  uint64_t* s_target = s_prefix + kWarps;
+  int* s_entry = reinterpret_cast<int*>(s_target + kWarps);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r8 = lane >> 2, t4 = lane & 3;
   const int kv_heads = p.c.map.kv_heads;
 
-  // ---- this warp's share of the line ----
+  // ---- this warp's share of the line: of W units the first W mod n warps take one more ----
   const int entries = p.batch * p.blocks;
-  int64_t mine = 0;
+  uint32_t own = 0;  // units of this thread's entry (of the first of several) for one head
+  uint64_t mine = 0;
   for (int e = threadIdx.x; e < entries; e += kWarps * 32) {
     const Entry t = entry_at(p, e, ROWS);
-    mine += t.tiles + kBegin;
+    const uint32_t units = t.tiles + kBegin;
+    if (e == static_cast<int>(threadIdx.x)) own = units;
+    mine += units;
     if (blockIdx.x == 0 && t.block == 0 && __ldg(p.lengths + t.b) != t.length) atomicExch(p.error_flag, PHEW_ERR_INVALID);
   }
+  asm volatile("griddepcontrol.launch_dependents;");  // the combine kernel may be set up from here on; it waits for this one
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   if (lane == 0) s_red[warp] = mine;
   __syncthreads();
-  const int64_t total = (s_red[0] + s_red[1] + s_red[2] + s_red[3]) * kv_heads;
-  const int64_t all_warps = static_cast<int64_t>(gridDim.x) * kWarps;
-  const int64_t n = total < all_warps ? total : all_warps;
-  // neighbours on the line run on different SMs, and a short line on as many as it can
-  const int self = warp * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x);
-  asm volatile("griddepcontrol.launch_dependents;");  // the combine kernel may be set up from here on; it waits for this one
+  const uint64_t total = (s_red[0] + s_red[1] + s_red[2] + s_red[3]) * kv_heads;
+  const uint32_t all_warps = gridDim.x * kWarps;
+  const uint32_t n = total < all_warps ? static_cast<uint32_t>(total) : all_warps;
   if (blockIdx.x >= n) return;  // no warp of the block has work
-  // the entries that the warps' first units lie in: the first whose units, with those before it, pass them
-  {
-    int64_t run = 0;
-    const int64_t most = total * (min(static_cast<int64_t>((kWarps - 1) * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x)), n - 1)) / n / kv_heads;
-    for (int e0 = 0; e0 < entries; e0 += kWarps * 32) {
-      const int e = e0 + static_cast<int>(threadIdx.x);
-      const int64_t own = e < entries ? entry_at(p, e, ROWS).tiles + kBegin : 0;
-      int64_t inc = own;
+  // neighbours on the line run on different SMs, and a short line on as many as it can
+  const uint32_t self = warp * gridDim.x + blockIdx.x;
+  const bool narrow = total >> 32 == 0;
+  const uint64_t each = narrow ? static_cast<uint32_t>(total) / n : total / n;
+  const uint32_t more = static_cast<uint32_t>(total - each * n);
+  uint64_t x = self * each + min(self, more);
+  const uint64_t x_end = x + each + (self < more);
+  // the entry that the first unit lies in: the first whose units, with those before it, pass x / kv_heads
+  if (lane == 0) s_target[warp] = self < n ? (narrow ? static_cast<uint32_t>(x) / static_cast<uint32_t>(kv_heads) : x / kv_heads) : ~0ull;
+  uint64_t run = 0;
+  for (int e0 = 0; e0 < entries; e0 += kWarps * 32) {
+    const int e = e0 + static_cast<int>(threadIdx.x);
+    if (e0 > 0) own = e < entries ? entry_at(p, e, ROWS).tiles + kBegin : 0;
+    uint64_t inc = own;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += up;
-      }
-      __syncthreads();
-      if (lane == 31) s_red[warp] = inc;
-      __syncthreads();
-      for (int w = 0; w < warp; ++w) inc += s_red[w];
-      inc += run;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const int64_t target = total * (static_cast<int64_t>(w) * gridDim.x + blockIdx.x) / n / kv_heads;
-        if (inc > target && inc - own <= target) {
-          s_entry[w] = e;
-          s_prefix[w] = inc - own;
-        }
-      }
-      run += s_red[0] + s_red[1] + s_red[2] + s_red[3];
-      if (run > most) break;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
     }
     __syncthreads();
+    if (lane == 31) s_red[warp] = inc;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) inc += s_red[w];
+    inc += run;
+    uint64_t most = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const uint64_t target = s_target[w];
+      if (inc > target && inc - own <= target) {
+        s_entry[w] = e;
+        s_prefix[w] = inc - own;
+      }
+      if (target != ~0ull) most = target;  // (targets grow with the warp)
+    }
+    run += s_red[0] + s_red[1] + s_red[2] + s_red[3];
+    if (run > most) break;
   }
+  __syncthreads();
   int e = s_entry[warp];
-  int64_t base = s_prefix[warp] * kv_heads;
+  uint64_t base = s_prefix[warp] * kv_heads;
   __syncthreads();  // (the ring takes the shared memory over; the last barrier)
   if (self >= n) return;
-  int64_t x = total * self / n;
-  const int64_t x_end = total * (self + 1) / n;
 
   Ring<S, T> ring{p.c, smem_addr(smem) + warp * S::RING, lane, 0u};
 
   while (x < x_end) {
     const Entry ent = entry_at(p, e, ROWS);
-    const int units = ent.tiles + kBegin;
-    for (; x < x_end && x < base + static_cast<int64_t>(kv_heads) * units;) {
-      const int h = static_cast<int>((x - base) / units);
-      const int64_t seg0 = base + static_cast<int64_t>(h) * units;
+    const uint32_t units = ent.tiles + kBegin;  // (units of a sequence's heads together fit 32 bits)
+    for (; x < x_end && x < base + static_cast<uint64_t>(kv_heads) * units;) {
+      const int h = static_cast<int>(static_cast<uint32_t>(x - base) / units);
+      const uint64_t seg0 = base + static_cast<uint64_t>(h) * units;
       const int t0 = max(static_cast<int>(x - seg0) - kBegin, 0);
       x = min(x_end, seg0 + units);
       const int t1 = static_cast<int>(x - seg0) - kBegin;
       if (t1 <= t0) continue;  // units of the begin alone
+
+      // ---- the ring: page numbers one stage ahead of the copies, copies STAGES - 1 ahead of the products.
+      // A lane without a key copies row 0 of the cache: whatever it holds is masked. ----
+      struct Look {
+        int page;  // -1: no key
+        uint32_t row;
+      };
+      int key = t0 * kTile + lane;  // of the next look-up
+      int col = static_cast<int>(div_by(p.c.map.by_page, static_cast<uint32_t>(key)));
+      int in_page = key - col * p.c.map.page_size;
+      const int32_t* pages = p.c.map.table ? p.c.map.table + ent.b * p.c.map.table_stride : nullptr;
+      const uint32_t head_row = static_cast<uint32_t>(h) * static_cast<uint32_t>(p.c.map.page_size);
+      const int key_end = min(ent.end, t1 * kTile);
+      auto look_up = [&]() {
+        Look k{0, 0};
+        const bool have = key < key_end;
+        if (have) k.page = pages ? __ldg(pages + col) : ent.b;
+        k.row = have ? head_row + static_cast<uint32_t>(in_page) : kNoRow;
+        key += kTile;
+        in_page += p.step_row;
+        col += p.step_col;
+        if (in_page >= p.c.map.page_size) {
+          in_page -= p.c.map.page_size;
+          ++col;
+        }
+        return k;
+      };
+      int left = t1 - t0, st_in = 0, st_out = 0;  // copies still to start, and the stages that come next
+      auto start_copy = [&](const Look& k) {
+        if (left > 0) {
+          uint32_t row = 0;
+          if (k.row != kNoRow) {
+            if (page_ok(p.c.map, k.page))
+              row = static_cast<uint32_t>(k.page) * p.page_rows + k.row;
+            else
+              atomicExch(p.error_flag, PHEW_ERR_INVALID);
+          }
+          if (p.eights)
+            ring.template issue<true>(st_in, row);
+          else
+            ring.template issue<false>(st_in, row);
+          st_in = st_in + 1 == S::STAGES ? 0 : st_in + 1;
+          --left;
+        } else {
+          copy_commit();
+        }
+      };
+      Look first[S::STAGES - 1];
+#pragma unroll
+      for (int i = 0; i < S::STAGES - 1; ++i) first[i] = look_up();
+      Look next = look_up();
+
+      // ---- queries: their loads travel beside the look-ups' ----
+      constexpr int QV = static_cast<int>(sizeof(T)) / 2;  // 16-byte loads of eight values
+      uint4 raw[NT][WT][QV];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int r = ent.block * ROWS + nt * 8 + r8;
+        const int tok = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(r)));
+        const T* q = static_cast<const T*>(p.q) + ent.b * p.st[2] + (h * p.per + (r - tok * p.per)) * p.st[1] + tok * p.st[0];
+#pragma unroll
+        for (int w = 0; w < WT; ++w)
+#pragma unroll
+          for (int k = 0; k < QV; ++k)
+            raw[nt][w][k] = tok < ent.count
+                                ? __ldg(reinterpret_cast<const uint4*>(q + (w / WPT) * G + (t4 * WPT + w % WPT) * 8) + k)
+                                : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < S::STAGES - 1; ++i) start_copy(first[i]);
 
       // ---- queries as the n operand, their group sums, and how far each row sees ----
       uint32_t qf[NT][TERMS][WT][4];
@@ -423,24 +500,14 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
       int lim[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int r = ent.block * ROWS + nt * 8 + r8;
-        const int tok = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(r)));
-        const bool have = tok < ent.count;
-        const T* q = static_cast<const T*>(p.q) + ent.b * p.st[2] + (h * p.per + (r - tok * p.per)) * p.st[1] + tok * p.st[0];
         float v[WT][8], top = 0.f;
 #pragma unroll
-        for (int w = 0; w < WT; ++w) {
-          uint4 raw[sizeof(T) / 2];
-#pragma unroll
-          for (int k = 0; k < static_cast<int>(sizeof(T)) / 2; ++k)
-            raw[k] = have ? __ldg(reinterpret_cast<const uint4*>(q + (w / WPT) * G + (t4 * WPT + w % WPT) * 8) + k)
-                          : make_uint4(0, 0, 0, 0);
+        for (int w = 0; w < WT; ++w)
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            v[w][k] = to_f32(reinterpret_cast<const T*>(raw)[k]);
+            v[w][k] = to_f32(reinterpret_cast<const T*>(raw[nt][w])[k]);
             top = fmaxf(top, fabsf(v[w][k]));
           }
-        }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // the row's largest magnitude to [2^14, 2^15)
@@ -514,50 +581,6 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
         }
       }
 
-      // ---- the ring: page numbers one stage ahead of the copies, copies STAGES - 1 ahead of the products.
-      // A lane without a key copies row 0 of the cache: whatever it holds is masked. ----
-      const int steps = t1 - t0;
-      int key = t0 * kTile + lane;  // of the next look-up
-      int col = static_cast<int>(div_by(p.c.map.by_page, static_cast<uint32_t>(key)));
-      int in_page = key - col * p.c.map.page_size;
-      const int32_t* pages = p.c.map.table ? p.c.map.table + ent.b * p.c.map.table_stride : nullptr;
-      const uint32_t head_row = static_cast<uint32_t>(h) * static_cast<uint32_t>(p.c.map.page_size);
-      const int key_end = min(ent.end, t1 * kTile);
-      int want_page = 0;
-      uint32_t want_r = 0;
-      bool want = false;
-      auto look_up = [&]() {
-        want = key < key_end;
-        if (want) want_page = pages ? __ldg(pages + col) : ent.b;
-        want_r = head_row + static_cast<uint32_t>(in_page);
-        key += kTile;
-        in_page += p.step_row;
-        col += p.step_col;
-        if (in_page >= p.c.map.page_size) {
-          in_page -= p.c.map.page_size;
-          ++col;
-        }
-      };
-      int left = steps, st_in = 0, st_out = 0;  // copies still to start, and the stages that come next
-      auto start_copy = [&]() {
-        if (left > 0) {
-          uint32_t row = 0;
-          if (want) {
-            if (page_ok(p.c.map, want_page))
-              row = static_cast<uint32_t>(want_page) * p.page_rows + want_r;
-            else
-              atomicExch(p.error_flag, PHEW_ERR_INVALID);
-          }
-          if (p.eights)
-            ring.template issue<true>(st_in, row);
-          else
-            ring.template issue<false>(st_in, row);
-          st_in = st_in + 1 == S::STAGES ? 0 : st_in + 1;
-          --left;
-        } else {
-          copy_commit();
-        }
-      };
       const int my_key = key_of_slot(r8);
 
       // One stage of 32 keys; EDGE: some row does not see all of them.
@@ -777,17 +800,11 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
         }
       };
 
-      look_up();
-#pragma unroll
-      for (int i = 0; i < S::STAGES - 1; ++i) {
-        start_copy();
-        look_up();
-      }
       for (int key0 = t0 * kTile; key0 < t1 * kTile; key0 += kTile) {
         copy_wait<S::STAGES - 2>();
         __syncwarp();
-        start_copy();
-        look_up();
+        start_copy(next);
+        next = look_up();
         if (key0 >= ent.end) break;  // (a tile without keys: the only one of its segment)
         {
           float sk[NG], zk[NG];
@@ -813,8 +830,8 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
       const int64_t segment = static_cast<int64_t>(e) * kv_heads + h;
       const bool whole = t0 == 0 && t1 == ent.tiles;
       if (lane == 0) {
-        if (t0 == 0) p.span[segment].x = self;
-        if (t1 == ent.tiles) p.span[segment].y = self;
+        if (t0 == 0) p.span[segment].x = static_cast<int>(self);
+        if (t1 == ent.tiles) p.span[segment].y = static_cast<int>(self);
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -889,7 +906,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
           }
         }
     }
-    base += static_cast<int64_t>(kv_heads) * units;
+    base += static_cast<uint64_t>(kv_heads) * units;
     ++e;
   }
 }
@@ -914,42 +931,47 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnParams p) {
   if (tok >= p.tokens) return;
   const bool live = !p.counts || tok < p.counts[b];
   auto at = [&](int k) { return (2 * static_cast<int64_t>(k) + (k == span.x ? 1 : 0)) * ROWS + row; };
-  float mm = kFloor;
-  for (int k = span.x + lane; k <= span.y; k += 32) mm = fmaxf(mm, p.part_ml[at(k) * 2]);
-  mm = warp_max(mm);
-  float o[E], l = 0.f;
+  // (a running maximum, so that no load waits for another)
+  float m = kFloor, l = 0.f, o[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) o[i] = 0.f;
 #pragma unroll 4
   for (int k = span.x + (WIDE ? warp : 0); k <= span.y; k += WIDE ? 8 : 1) {
     const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at(k) * 2);
-    const float f = exp2_fast(ml.x - mm);
-    l = fmaf(f, ml.y, l);
     const float2* v = reinterpret_cast<const float2*>(p.part + at(k) * D) + lane;
+    const float m_new = fmaxf(m, ml.x), was = exp2_fast(m - m_new), f = exp2_fast(ml.x - m_new);
+    m = m_new;
+    l = fmaf(l, was, f * ml.y);
 #pragma unroll
     for (int i = 0; i < E; i += 2) {
       const float2 x = v[i * 16];
-      o[i] = fmaf(f, x.x, o[i]);
-      o[i + 1] = fmaf(f, x.y, o[i + 1]);
+      o[i] = fmaf(f, x.x, o[i] * was);
+      o[i + 1] = fmaf(f, x.y, o[i + 1] * was);
     }
   }
   if constexpr (WIDE) {
-    __shared__ float s_o[8][D], s_l[8];
+    __shared__ float s_o[8][D], s_l[8], s_m[8];
 #pragma unroll
     for (int i = 0; i < E; i += 2) *reinterpret_cast<float2*>(&s_o[warp][i * 32 + lane * 2]) = make_float2(o[i], o[i + 1]);
-    if (lane == 0) s_l[warp] = l;
+    if (lane == 0) {
+      s_l[warp] = l;
+      s_m[warp] = m;
+    }
     __syncthreads();
     if (warp) return;
+#pragma unroll
+    for (int w = 1; w < 8; ++w) m = fmaxf(m, s_m[w]);
     l = 0.f;
 #pragma unroll
     for (int i = 0; i < E; ++i) o[i] = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
-      l += s_l[w];
+      const float f = exp2_fast(s_m[w] - m);
+      l = fmaf(f, s_l[w], l);
 #pragma unroll
       for (int i = 0; i < E; i += 2) {
-        o[i] += s_o[w][i * 32 + lane * 2];
-        o[i + 1] += s_o[w][i * 32 + lane * 2 + 1];
+        o[i] = fmaf(f, s_o[w][i * 32 + lane * 2], o[i]);
+        o[i + 1] = fmaf(f, s_o[w][i * 32 + lane * 2 + 1], o[i + 1]);
       }
     }
   }
@@ -989,6 +1011,8 @@ template <typename S, typename T> int launch_attn(AttnParams p, void* workspace,
   const int64_t blocks = blocks_of<S>(static_cast<int64_t>(p.tokens) * p.per);
   const int64_t segments = p.batch * blocks * p.c.map.kv_heads;
   PHEW_REQUIRE(segments < (1ll << 31), "phew_kv_attention: too many query rows");
+  PHEW_REQUIRE((capacity(p.c.map) / kTile + kBegin + 1) * p.c.map.kv_heads < (1ll << 32),
+               "phew_kv_attention: too many tokens for a sequence");
   p.blocks = static_cast<int>(blocks);
   p.by_blocks = fast_div(static_cast<uint32_t>(blocks));
   const int page = p.c.map.page_size;
