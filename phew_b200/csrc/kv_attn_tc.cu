@@ -3,29 +3,35 @@
 //
 // The rows of a cache head are r = token * per + head over its `per` query
 // heads; a CTA takes 256 of them (two 128-row tiles a and b) and walks the
-// keys in tiles of 128.  Bound by the tensor cores and, at the same rate, by
-// the exponentials; the cache is read once per 256 rows.  What the dense kernel
-// fetches as 16-bit tiles by TMA is made here from codes: four producer warps
-// copy packed rows (cp.async, three half-steps ahead), expand them as
-// T(scale * code + bias) - two instructions a value: a shift and a logic
-// operation per pair of codes, an exact subtraction, a packed multiply-add -
-// and store them in the 128-byte swizzle that the tensor core reads.  That is
-// a fifth of the SM's issue slots beside the softmax, so the packed cache
-// costs no time over a dense one.
+// keys in tiles of 128.  Bound by the chain score product - softmax - output
+// product of each tile, at about the rate of the exponentials.  Two forms:
 //
-//   warps 0-3    warp 0: TMEM owner and MMA issuer: per key tile j and query
-//                tile t, O_t += P_t V_j, then S_t = Q_t K_{j+1}^T
-//   warps 4-7    producers: warp w expands keys 32 w .. 32 w + 31 of each tile,
-//                K_j and V_j in turn, into two-deep rings
-//   warps 8-15   softmax of tile a and b, one query row per thread; they also
-//                load Q and write O
+// Dense (kExpandBlocks row blocks or more, whose every CTA would expand the
+// same keys again): the cache is expanded once to 16 bits in scratch, as
+// phew_kv_fetch does, and tiles arrive by TMA.  One pass of HBM over the keys
+// against 0.5 us for each CTA and tile (measured: 256 CTAs x 56 tiles).
 //
-// Registers move from the first two groups to the softmax (40 + 72 + 2 x 200
-// = 4 x 128).  TMEM: S_a, S_b, O_a, O_b of 128 columns each.
+// Packed (few row blocks): producer warps load packed rows (two units of 32
+// keys ahead, in registers), expand them as T(scale * code + bias) - two
+// instructions a value: a shift and a logic operation per pair of codes, an
+// exact subtraction, a packed multiply-add - and store them in the 128-byte
+// swizzle that the tensor core reads.  Those instructions take issue slots
+// from the softmax, which is why the dense form exists; more producer warps
+// (7 for 3) did not help.
 //
-// Within eight neighbouring head dimensions tiles hold them in the order
-// 0 4 1 5 2 6 3 7, which is how pairs fall out of a word of codes; queries are
-// stored to match and outputs read back through the same order.
+//   warp 0        TMEM owner and MMA issuer: per key tile j and query tile t,
+//                 O_t += P_t V_j, then S_t = Q_t K_{j+1}^T
+//   next warps    dense: one, TMA.  Packed: three producers; the line of units
+//                 K_0, V_0, K_1, ... in quarters of 32 keys, every third one to
+//                 a warp.  Both fill two-deep rings of K and V
+//   last 8 warps  softmax of tile a and b, one query row per thread; they also
+//                 load Q and write O
+//
+// TMEM: S_a, S_b, O_a, O_b of 128 columns each.
+//
+// Within eight neighbouring head dimensions packed tiles hold them in the
+// order 0 4 1 5 2 6 3 7, which is how pairs fall out of a word of codes; queries
+// are stored to match and outputs read back through the same order.
 //
 // Long caches with few rows are split: a CTA takes a share of the key tiles
 // and leaves partial sums, joined in a fixed order by the combine kernel.
@@ -48,7 +54,7 @@ using attn::row_max;
 constexpr int kTileRows = 128;
 constexpr int kTcTile = 128;       // keys of a tile
 constexpr int kTcRows = 256;       // query rows of a CTA
-constexpr int kTcThreads = 512;
+constexpr int kProducers = 3;      // warps 1 .. 3 of the packed form
 constexpr int kTmemCols = 512;
 constexpr float kTcFloor = -1.0e38f;
 constexpr float kTcGrow = 8.0f;    // log2 units: the running maximum moves when a tile passes it by more
@@ -58,12 +64,10 @@ template <int D_, int G_> struct TcShape {
   static constexpr int HALVES = D / 64;
   static constexpr int HALF_BYTES = kTcTile * 128;           // 64 columns of 16 bits, 128-byte rows
   static constexpr int TILE_BYTES = HALF_BYTES * HALVES;
-  static constexpr int SB = NG * 2, SROW = SB < 4 ? 4 : SB;  // a key's scales
-  static constexpr int WARP_CODES = 32 * D / 2;              // one warp's share of a side's codes
-  static constexpr int WARP_STAGE = WARP_CODES + 2 * 32 * SROW;
-  static constexpr int STAGES = 3;
-  static constexpr int SMEM = 6 * TILE_BYTES + 4 * STAGES * WARP_STAGE + 1024 + 256;
+  static constexpr int SMEM = 6 * TILE_BYTES + 1024 + 256;
 };
+
+constexpr int tc_threads(bool dense) { return 32 * ((dense ? 2 : 1 + kProducers) + 8); }
 
 struct TcParams {
   Cache c;
@@ -75,6 +79,7 @@ struct TcParams {
   int batch, heads, tokens, per;
   int blocks;  // 256-row blocks of a cache head
   int splits;
+  int rows;    // dense: token rows of a cache head in the expanded keys and values
   FastDiv by_per;
   float scale_log2;  // > 0
   bool causal;
@@ -84,13 +89,6 @@ struct TcParams {
   unsigned long long wait_ns;
   int withhold;  // test hook: the V tile of this key tile is never announced (-1: none)
 };
-
-template <int N> __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int valid) {
-  if constexpr (N == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(valid) : "memory");
-}
 
 // code pairs (U, U + 4) of a word as 16-bit floats, exactly
 template <bool BF16, int U> __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
@@ -123,17 +121,18 @@ __device__ __forceinline__ void store_shared16(uint32_t at, uint32_t a, uint32_t
 // shared-memory writes of this thread become visible to the tensor core
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-template <typename S, bool BF16>
-__global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcParams p) {
+template <typename S, bool BF16, bool DENSE>
+__global__ void __launch_bounds__(tc_threads(DENSE), 1)
+    attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const TcParams p) {
   constexpr int D = S::D, NG = S::NG;
+  constexpr int FIRST = DENSE ? 2 : 1 + kProducers;  // softmax warp
   using T = typename std::conditional<BF16, bf16, f16>::type;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                          // [2] tiles
   uint8_t* sK = smem + 2 * S::TILE_BYTES;      // [2]
   uint8_t* sV = smem + 4 * S::TILE_BYTES;      // [2]
-  uint8_t* stage = smem + 6 * S::TILE_BYTES;   // [4 warps][STAGES]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(stage + 4 * S::STAGES * S::WARP_STAGE);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * S::TILE_BYTES);
   uint64_t* q_full = bars;        // [2]
   uint64_t* k_full = bars + 2;    // [2]
   uint64_t* k_empty = bars + 4;   // [2]
@@ -175,14 +174,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcParams p
   const int j0 = static_cast<int>(static_cast<int64_t>(all) * split / p.splits);
   const int n_max = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / p.splits) - j0;
   const int n_t[2] = {min(max(need[0] - j0, 0), n_max), min(max(need[1] - j0, 0), n_max)};
-  const int key_end = max(0, length);  // rows behind it are never read
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 4);
-      mbar_init(&k_full[i], 4);
+      mbar_init(&k_full[i], DENSE ? 1 : 4);
       mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], 4);
+      mbar_init(&v_full[i], DENSE ? 1 : 4);
       mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
@@ -198,10 +196,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcParams p
   fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
+  int k_last[2] = {-1, -1}, v_last[2] = {-1, -1};  // dense: the key tile whose load each ring slot received last
 
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 0 && lane == 0) {
+  if (warp == 0) {
+    if (lane == 0) {
       // ---------------- MMA issuer ----------------
       constexpr uint32_t id_qk = instr_desc_f16(BF16 ? 1 : 0, 0, kTileRows, kTcTile);
       constexpr uint32_t id_pv = instr_desc_f16(BF16 ? 1 : 0, 1, kTileRows, D);
@@ -255,95 +253,86 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcParams p
         if (more) commit(&k_empty[s1]);
       }
     }
-  } else if (warp < 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  } else if (DENSE && warp == 1) {
+    // ---------------- TMA ----------------
+    if (lane == 0 && n_max > 0) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");  // the expanded keys and values are there
+      const int first = bh * p.rows + j0 * kTcTile;
+      auto load = [&](const CUtensorMap* tm, uint64_t* bar, uint8_t* dst, int row) {
+        mbar_expect_tx(bar, S::TILE_BYTES);
+#pragma unroll
+        for (int i = 0; i < S::HALVES; ++i) tma_load_2d(dst + i * S::HALF_BYTES, tm, bar, i * 64, row);
+      };
+      for (int j = 0; j < n_max && ok; ++j) {
+        const int s = j & 1;
+        const uint32_t ph = ((j >> 1) & 1) ^ 1;
+        if (!mbar_wait(&k_empty[s], ph, wait_flag, p.wait_ns)) { ok = false; break; }
+        load(&tm_k, &k_full[s], sK + s * S::TILE_BYTES, first + j * kTcTile);
+        (s ? k_last[1] : k_last[0]) = j;
+        if (!mbar_wait(&v_empty[s], ph, wait_flag, p.wait_ns)) { ok = false; break; }
+        if (j == p.withhold) continue;  // test hook: this V tile never lands
+        load(&tm_v, &v_full[s], sV + s * S::TILE_BYTES, first + j * kTcTile);
+        (s ? v_last[1] : v_last[0]) = j;
+      }
+    }
+  } else if (!DENSE && warp <= kProducers) {
     // ---------------- producers ----------------
-    const int w = warp - 4;
-    const uint32_t ring = smem_u32(stage + w * S::STAGES * S::WARP_STAGE);
-    const int row = w * 32 + lane;  // of the tile
-    const int steps = 2 * n_max;    // K_0, V_0, K_1, ...
-    // page lookup one tile ahead of its copies
-    int look_page = -1, look_r = 0;
-    bool look_any = false;
-    auto look_up = [&](int j) {
-      const int key = (j0 + j) * kTcTile + row;
-      look_any = j < n_max && key < key_end;
-      if (look_any) {
+    // unit u: quarter u % 4 of K (u / 4 even) or V (odd) of tile u / 8; this warp takes u = warp - 1, + 3, ...
+    const int units = 8 * n_max;
+    // a lane's key of a unit: its row (looked up a round ahead), then its codes and scales, which wait in
+    // registers until the unit's turn comes.  (Copies to shared memory in their place would have to land
+    // before every fence_async_shared.)
+    struct Look {
+      int page, row;  // row -1: no key
+    };
+    struct Packed {
+      uint4 code[D / 32];
+      uint32_t sb[2][(NG + 1) / 2];  // scales, biases
+    };
+    auto look_up = [&](int u) {
+      Look k{0, -1};
+      const int key = (j0 + (u >> 3)) * kTcTile + (u & 3) * 32 + lane;
+      if (u < units && key < length) {
         const int col = static_cast<int>(div_by(p.c.map.by_page, static_cast<uint32_t>(key)));
-        look_r = key - col * p.c.map.page_size;
-        look_page = page_at(p.c.map, b, col);
+        k.row = key - col * p.c.map.page_size;
+        k.page = page_at(p.c.map, b, col);
       }
+      return k;
     };
-    uint32_t src_row = kNoRow;
-    uint32_t odd = 0;  // per stage (byte): the key's scales are the upper half of the loaded word
-    auto start_copy = [&](int q) {
-      if (q < steps) {
-        const int side = q & 1, s = q % S::STAGES;
-        if (side == 0) {
-          src_row = kNoRow;
-          if (look_any) {
-            if (page_ok(p.c.map, look_page))
-              src_row = row_at(p.c.map, look_page, h, look_r);
-            else
-              atomicExch(p.error_flag, PHEW_ERR_INVALID);
-          }
-          look_up((q >> 1) + 1);
-        }
-        const uint32_t at = ring + s * S::WARP_STAGE;
-        constexpr int CH = D / 32;
+    auto fetch = [&](int u, const Look& k) {
+      Packed x{};
+      if (k.row >= 0) {
+        if (page_ok(p.c.map, k.page)) {
+          const int side = (u >> 2) & 1;
+          const int64_t row = row_at(p.c.map, k.page, h, k.row);
+          const uint4* codes = reinterpret_cast<const uint4*>(p.c.codes[side] + row * (D / 8));
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          const int id = i * 32 + lane, r = id / CH, ch = id % CH;
-          const uint32_t src = __shfl_sync(0xffffffffu, src_row, r);
-          const bool have = src != kNoRow;
-          const int sw = CH == 4 ? ch ^ ((r >> 1) & 3) : ch ^ ((r >> 2) & 1);  // eight rows' same chunk: eight bank groups
-          copy16<16>(at + r * (D / 2) + sw * 16, p.c.codes[side] + (have ? static_cast<int64_t>(src) * (D / 8) + ch * 4 : 0),
-                     have ? 16 : 0);
-        }
-        const bool have = src_row != kNoRow;
+          for (int i = 0; i < D / 32; ++i) x.code[i] = __ldg(codes + i);
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          const char* arr = static_cast<const char*>(a ? p.c.biases[side] : p.c.scales[side]);
-          const uint32_t dst = at + S::WARP_CODES + (a * 32 + lane) * S::SROW;
-          if constexpr (S::SB == 2) {
-            const int64_t off = (static_cast<int64_t>(have ? src_row : 0) * 2) & ~3ll;
-            const uint32_t rows = static_cast<uint32_t>(p.c.map.pages) * static_cast<uint32_t>(p.c.map.kv_heads) *
-                                  static_cast<uint32_t>(p.c.map.page_size);
-            copy16<4>(dst, arr + off, !have ? 0 : (src_row | 1u) < rows ? 4 : 2);
-          } else {
-            copy16<S::SB>(dst, arr + (have ? static_cast<int64_t>(src_row) * S::SB : 0), have ? S::SB : 0);
+          for (int a = 0; a < 2; ++a) {
+            const T* at = static_cast<const T*>(a ? p.c.biases[side] : p.c.scales[side]) + row * NG;
+            if constexpr (NG == 1) {
+              x.sb[a][0] = __ldg(reinterpret_cast<const uint16_t*>(at));
+            } else {
+#pragma unroll
+              for (int i = 0; i < NG / 2; ++i) x.sb[a][i] = __ldg(reinterpret_cast<const uint32_t*>(at) + i);
+            }
           }
+        } else {
+          atomicExch(p.error_flag, PHEW_ERR_INVALID);
         }
-        odd = (odd & ~(1u << s)) | ((have ? src_row & 1u : 0u) << s);
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      return x;
     };
-    look_up(0);
-    start_copy(0);
-    start_copy(1);
-    for (int q = 0; q < steps && ok; ++q) {
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
-      __syncwarp();
-      start_copy(q + 2);  // into the stage read in step q - 1
-      const int j = q >> 1, side = q & 1, s = q % S::STAGES;
-      const int slot = j & 1;
-      const uint32_t at = ring + s * S::WARP_STAGE;
-      // this key's scales and biases, each twice in a register
-      uint32_t sc[NG], bi[NG];
+    auto expand = [&](int u, Packed& x) {
+      const int j = u >> 3, side = (u >> 2) & 1, row = (u & 3) * 32 + lane, slot = j & 1;
+      uint32_t sc[NG], bi[NG];  // each twice in a register
       bool fine = true;
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        const uint32_t src = at + S::WARP_CODES + (a * 32 + lane) * S::SROW;
-        uint32_t v[S::SROW / 4];
-#pragma unroll
-        for (int i = 0; i < S::SROW / 4; ++i) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[i]) : "r"(src + 4 * i));
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const bool upper = S::SB == 2 ? (odd >> s) & 1 : g & 1;
-          const uint32_t x = __byte_perm(v[g / 2], 0, upper ? 0x3232 : 0x1010);
-          fine = fine && finite16(x, BF16);
-          (a ? bi[g] : sc[g]) = x;
-        }
+      for (int g = 0; g < NG; ++g) {
+        sc[g] = __byte_perm(x.sb[0][g / 2], 0, g & 1 ? 0x3232 : 0x1010);
+        bi[g] = __byte_perm(x.sb[1][g / 2], 0, g & 1 ? 0x3232 : 0x1010);
+        fine = fine && finite16(sc[g], BF16) && finite16(bi[g], BF16);
       }
       if (side == 1 && !fine) {
         // a weight of zero times infinity is no number, and a later query's keys may not touch an earlier
@@ -354,15 +343,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcParams p
       }
       uint64_t* full = side == 0 ? &k_full[slot] : &v_full[slot];
       uint64_t* empty = side == 0 ? &k_empty[slot] : &v_empty[slot];
-      if (!mbar_wait(empty, ((j >> 1) & 1) ^ 1, wait_flag, p.wait_ns)) { ok = false; break; }
+      if (lane == 0 && !mbar_wait(empty, ((j >> 1) & 1) ^ 1, wait_flag, p.wait_ns)) ok = false;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) return;
       const uint32_t dst = smem_u32((side == 0 ? sK : sV) + slot * S::TILE_BYTES) + row * 128;
 #pragma unroll
       for (int ch = 0; ch < D / 32; ++ch) {
-        const int sw = D == 128 ? ch ^ ((lane >> 1) & 3) : ch ^ ((lane >> 2) & 1);
-        uint32_t word[4];
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(word[0]), "=r"(word[1]), "=r"(word[2]), "=r"(word[3])
-                     : "r"(at + lane * (D / 2) + sw * 16));
+        const uint32_t word[4] = {x.code[ch].x, x.code[ch].y, x.code[ch].z, x.code[ch].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int g = (ch * 32 + i * 8) / S::G, c16 = ch * 4 + i;
@@ -376,36 +363,56 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcParams p
       fence_async_shared();
       __syncwarp();
       if (lane == 0 && !(side == 1 && j == p.withhold)) mbar_arrive(full);
+    };
+    constexpr int P = kProducers;
+    const int u0 = warp - 1;
+    Look la = look_up(u0), lb = look_up(u0 + P);
+    Packed xa = fetch(u0, la), xb = fetch(u0 + P, lb);
+    la = look_up(u0 + 2 * P);
+    lb = look_up(u0 + 3 * P);
+    for (int u = u0; u < units && ok; u += 2 * P) {
+      expand(u, xa);
+      xa = fetch(u + 2 * P, la);
+      la = look_up(u + 4 * P);
+      if (!ok || u + P >= units) break;
+      expand(u + P, xb);
+      xb = fetch(u + 3 * P, lb);
+      lb = look_up(u + 5 * P);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---------------- softmax and output ----------------
-    const int t = (warp - 8) >> 2;
+    const int t = (warp - FIRST) >> 2;
     const int quarter = warp & 3;             // TMEM lanes this warp may access
     const int row = quarter * 32 + lane;      // of the query tile
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_addr = tmem + lane_addr + t * 128;
     const uint32_t o_addr = tmem + lane_addr + 256 + t * 128;
-    const int r = row0 + t * kTileRows + row;
-    const int tok = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(r)));
-    const int head = h * p.per + (r - tok * p.per);
     const int nkv = t ? n_t[1] : n_t[0];
     const float c = p.scale_log2;
-    const int lim = seen_end(length, count, tok, p.causal);
-    if (nkv > 0) {
-      const bool have = tok < count;
-      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.st[2] + head * p.st[1] + tok * p.st[0]);
-      const uint32_t dst = smem_u32(sQ + t * S::TILE_BYTES) + row * 128;
+    int lim;
+    {
+      const int r = row0 + t * kTileRows + row;
+      const int tok = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(r)));
+      lim = seen_end(length, count, tok, p.causal) - j0 * kTcTile;
+      if (nkv > 0) {
+        const bool have = tok < count;
+        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.st[2] +
+                                                        (h * p.per + (r - tok * p.per)) * p.st[1] + tok * p.st[0]);
+        const uint32_t dst = smem_u32(sQ + t * S::TILE_BYTES) + row * 128;
 #pragma unroll
-      for (int c16 = 0; c16 < D / 8; ++c16) {
-        const uint4 x = have ? __ldg(q + c16) : make_uint4(0, 0, 0, 0);
-        store_shared16(dst + (c16 >> 3) * S::HALF_BYTES + (((c16 & 7) ^ (row & 7)) << 4), __byte_perm(x.x, x.z, 0x5410),
-                       __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+        for (int c16 = 0; c16 < D / 8; ++c16) {
+          const uint4 x = have ? __ldg(q + c16) : make_uint4(0, 0, 0, 0);
+          const uint32_t at = dst + (c16 >> 3) * S::HALF_BYTES + (((c16 & 7) ^ (row & 7)) << 4);
+          if constexpr (DENSE)
+            store_shared16(at, x.x, x.y, x.z, x.w);
+          else
+            store_shared16(at, __byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410),
+                           __byte_perm(x.y, x.w, 0x7632));
+        }
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[t]);
       }
-      fence_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[t]);
     }
     float m_ref = kTcFloor, l = 0.f;
     for (int j = 0; j < nkv && ok; ++j) {
@@ -415,11 +422,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcParams p
 #pragma unroll
       for (int k = 0; k < 4; ++k) tmem_ld32(s_addr + k * 32, raw + k * 32);
       tmem_ld_wait();
-      const int left = lim - (j0 + j) * kTcTile;  // keys of this tile that the row sees
-      if (left < kTcTile) {
+      if (lim < kTcTile) {  // (lim: keys that the row sees, from this tile's first on)
 #pragma unroll
         for (int i = 0; i < 128; ++i)
-          if (i >= left) raw[i] = __float_as_uint(-INFINITY);
+          if (i >= lim) raw[i] = __float_as_uint(-INFINITY);
       }
       float tile_sum;
       bool rescale = false;
@@ -455,6 +461,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcParams p
         }
       }
       l = fmaf(l, alpha, tile_sum);
+      lim -= kTcTile;
       tmem_st_wait();
       fence_before_sync();
       __syncwarp();
@@ -463,8 +470,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcParams p
     if (ok && nkv > 0 && !mbar_wait(&o_done[t], (nkv - 1) & 1, wait_flag, p.wait_ns)) ok = false;
     fence_after_sync();
     if (ok) {
-      if (lim > *reinterpret_cast<volatile int*>(s_poison)) l = __int_as_float(0x7fc00000);
-      const bool live = nkv > 0 && lim > 0;
+      // (where the row lies is worked out again: the loop has no registers to keep it in)
+      int again = row;
+      asm volatile("" : "+r"(again));
+      const int r = row0 + t * kTileRows + again;
+      const int tok = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(r)));
+      const int head = h * p.per + (r - tok * p.per);
+      const int end = seen_end(length, count, tok, p.causal);
+      if (!DENSE && end > *reinterpret_cast<volatile int*>(s_poison)) l = __int_as_float(0x7fc00000);
+      const bool live = nkv > 0 && end > 0;
       const bool split_up = p.splits > 1;
       const float inv = !live || l == 0.f ? 0.f : 1.f / l;
       const int64_t at = (static_cast<int64_t>(bh) * p.blocks + rb) * p.splits + split;
@@ -490,17 +504,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcParams p
         if (!mine) continue;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t* e = o + 8 * i;  // head dimensions 0 4 1 5 2 6 3 7 of eight
+          float f[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x)  // packed tiles: head dimensions 0 4 1 5 2 6 3 7 of eight
+            f[x] = __uint_as_float(o[8 * i + (DENSE ? x : 2 * (x & 3) + (x >> 2))]);
           if (split_up) {
             float4* dst = reinterpret_cast<float4*>(part + k * 32 + i * 8);
-            dst[0] = make_float4(__uint_as_float(e[0]), __uint_as_float(e[2]), __uint_as_float(e[4]), __uint_as_float(e[6]));
-            dst[1] = make_float4(__uint_as_float(e[1]), __uint_as_float(e[3]), __uint_as_float(e[5]), __uint_as_float(e[7]));
+            dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+            dst[1] = make_float4(f[4], f[5], f[6], f[7]);
           } else {
-            float f[8];
 #pragma unroll
-            for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(e[x]) * inv;
-            *reinterpret_cast<uint4*>(out + k * 32 + i * 8) = make_uint4(pack2<BF16>(f[0], f[2]), pack2<BF16>(f[4], f[6]),
-                                                                         pack2<BF16>(f[1], f[3]), pack2<BF16>(f[5], f[7]));
+            for (int x = 0; x < 8; ++x) f[x] *= inv;
+            *reinterpret_cast<uint4*>(out + k * 32 + i * 8) = make_uint4(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]),
+                                                                         pack2<BF16>(f[4], f[5]), pack2<BF16>(f[6], f[7]));
           }
         }
       }
@@ -509,10 +525,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcParams p
   if (!ok) atomicExch(wait_flag, PHEW_ERR_TIMEOUT);
   fence_before_sync();
   if (__syncthreads_or(!ok)) {
-    // a wait ran out somewhere: let the issued products finish before the TMEM and shared memory go
+    // a wait ran out somewhere: let the issued products and loads finish before the TMEM and shared memory go
     if (warp == 0 && lane == 0) {
       commit(drain);
       mbar_wait(drain, 0, nullptr, p.wait_ns);
+    } else if (DENSE && warp == 1 && lane == 0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (k_last[i] >= 0) mbar_wait(&k_full[i], (k_last[i] >> 1) & 1, nullptr, p.wait_ns);
+        if (v_last[i] >= 0) mbar_wait(&v_full[i], (v_last[i] >> 1) & 1, nullptr, p.wait_ns);
+      }
     }
     fence_before_sync();
     __syncthreads();
@@ -557,59 +579,95 @@ __global__ void __launch_bounds__(256) combine_tc_kernel(const TcParams p) {
   for (int i = 0; i < E; ++i) out[i * 32 + lane] = from_f32<T>(o[i] * inv);
 }
 
-// CTAs of a call and how many ways each row block's keys are split: enough to
-// give every SM a CTA, at most a tile of the longest possible sequence each.
+// CTAs of a call, how many ways each row block's keys are split (enough to give
+// every SM a CTA, two tiles of the longest possible sequence or more each), and
+// whether the cache is expanded first.
+constexpr int64_t kExpandBlocks = 3;               // row blocks from which one expansion beats one per CTA
+constexpr int64_t kExpandBytes = int64_t(1) << 30;  // scratch that a call may take for it
+
 struct TcPlan {
   int64_t blocks, splits, ctas;
+  int64_t rows;  // token rows of a cache head in the expanded cache; 0: packed
+  size_t part_bytes, side_bytes;
 };
-TcPlan tc_plan(int64_t batch, int kv_heads, int64_t rows, int64_t cap) {
+TcPlan tc_plan(int64_t batch, int kv_heads, int head_dim, int64_t q_rows, int64_t cap) {
   TcPlan t;
-  t.blocks = (rows + kTcRows - 1) / kTcRows;
+  t.blocks = (q_rows + kTcRows - 1) / kTcRows;
   const int64_t base = batch * kv_heads * t.blocks, sms = sm_count_current();
   const int64_t tiles = (cap + kTcTile - 1) / kTcTile;
   t.splits = base >= sms ? 1 : sms / base;
   if (t.splits > tiles / 2) t.splits = tiles / 2;
   if (t.splits < 1) t.splits = 1;
   t.ctas = base * t.splits;
+  t.part_bytes = t.splits == 1 ? 0 : static_cast<size_t>(t.ctas) * kTcRows * (static_cast<size_t>(head_dim) + 2) * 4;
+  t.rows = tiles * kTcTile;
+  t.side_bytes = static_cast<size_t>(batch) * kv_heads * t.rows * head_dim * 2;
+  if (t.blocks < kExpandBlocks || static_cast<int64_t>(2 * t.side_bytes) > kExpandBytes ||
+      batch * kv_heads * t.rows >= kMaxRows) {
+    t.rows = 0;
+    t.side_bytes = 0;
+  }
   return t;
 }
 
-template <typename S, bool BF16> int launch_tc(TcParams p, unsigned grid, cudaStream_t st) {
+// [batch * kv_heads * rows][D] of 16-bit values; box of 64 columns x 128 rows, 128-byte swizzle.
+int dense_map(CUtensorMap* tm, const void* base, bool bf16_type, int64_t rows, int D) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(D), static_cast<uint64_t>(rows)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(D) * 2};
+  const uint32_t box[2] = {64, static_cast<uint32_t>(kTcTile)};
+  return make_map_16bit(tm, base, bf16_type, 2, dims, strides, box);
+}
+
+template <typename S, bool BF16, bool DENSE>
+int launch_tc(const CUtensorMap& tk, const CUtensorMap& tv, const TcParams& p, unsigned grid, cudaStream_t st) {
   static SmemAllowed allowed;
-  if (int s = allow_smem(allowed, attn_tc_kernel<S, BF16>, S::SMEM)) return s;
-  attn_tc_kernel<S, BF16><<<grid, kTcThreads, S::SMEM, st>>>(p);
-  if (int s = launch_status("kv attn_tc_kernel")) return s;
-  if (p.splits == 1) return PHEW_OK;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.batch) * p.c.map.kv_heads * p.blocks * (kTcRows / 8)));
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
+  if (int s = allow_smem(allowed, attn_tc_kernel<S, BF16, DENSE>, S::SMEM)) return s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(tc_threads(DENSE));
+  cfg.dynamicSmemBytes = S::SMEM;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = DENSE ? 1 : 0;  // set up while the cache is expanded
+  PHEW_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_tc_kernel<S, BF16, DENSE>, tk, tv, p));
+  if (int s = launch_status("kv attn_tc_kernel")) return s;
+  if (p.splits == 1) return PHEW_OK;
+  cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.batch) * p.c.map.kv_heads * p.blocks * (kTcRows / 8)));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   PHEW_CHECK_CUDA(cudaLaunchKernelEx(&cfg, combine_tc_kernel<S::D, BF16>, p));
   return launch_status("kv combine_tc_kernel");
 }
 
-template <bool BF16> int dispatch_tc(const TcParams& p, unsigned grid, cudaStream_t st) {
+template <bool BF16>
+int dispatch_tc(const CUtensorMap& tk, const CUtensorMap& tv, const TcParams& p, unsigned grid, cudaStream_t st) {
+  if (p.rows)  // (the group no longer matters)
+    return p.c.head_dim == 64 ? launch_tc<TcShape<64, 64>, BF16, true>(tk, tv, p, grid, st)
+                              : launch_tc<TcShape<128, 128>, BF16, true>(tk, tv, p, grid, st);
   if (p.c.head_dim == 64)
-    return p.c.group == 32 ? launch_tc<TcShape<64, 32>, BF16>(p, grid, st) : launch_tc<TcShape<64, 64>, BF16>(p, grid, st);
-  if (p.c.group == 32) return launch_tc<TcShape<128, 32>, BF16>(p, grid, st);
-  if (p.c.group == 64) return launch_tc<TcShape<128, 64>, BF16>(p, grid, st);
-  return launch_tc<TcShape<128, 128>, BF16>(p, grid, st);
+    return p.c.group == 32 ? launch_tc<TcShape<64, 32>, BF16, false>(tk, tv, p, grid, st)
+                           : launch_tc<TcShape<64, 64>, BF16, false>(tk, tv, p, grid, st);
+  if (p.c.group == 32) return launch_tc<TcShape<128, 32>, BF16, false>(tk, tv, p, grid, st);
+  if (p.c.group == 64) return launch_tc<TcShape<128, 64>, BF16, false>(tk, tv, p, grid, st);
+  return launch_tc<TcShape<128, 128>, BF16, false>(tk, tv, p, grid, st);
 }
 
 }  // namespace
 
 size_t tc_bytes(int64_t batch, int kv_heads, int head_dim, int64_t rows, int64_t cap) {
-  const TcPlan t = tc_plan(batch, kv_heads, rows, cap);
-  return t.splits == 1 ? 0 : static_cast<size_t>(t.ctas) * kTcRows * (static_cast<size_t>(head_dim) + 2) * 4;
+  const TcPlan t = tc_plan(batch, kv_heads, head_dim, rows, cap);
+  return 2 * t.side_bytes + t.part_bytes;
 }
 
 int run_attn_tc(const AttnParams& a, bool bf16_type, void* workspace, cudaStream_t st) {
-  const TcPlan t = tc_plan(a.batch, a.c.map.kv_heads, static_cast<int64_t>(a.tokens) * a.per, capacity(a.c.map));
+  const int D = a.c.head_dim;
+  const TcPlan t = tc_plan(a.batch, a.c.map.kv_heads, D, static_cast<int64_t>(a.tokens) * a.per, capacity(a.c.map));
   PHEW_REQUIRE(t.ctas < (1ll << 31) / 32, "phew_kv_attention: too many query rows");
   TcParams p;
   p.c = a.c;
@@ -624,17 +682,26 @@ int run_attn_tc(const AttnParams& a, bool bf16_type, void* workspace, cudaStream
   p.per = a.per;
   p.blocks = static_cast<int>(t.blocks);
   p.splits = static_cast<int>(t.splits);
+  p.rows = static_cast<int>(t.rows);
   p.by_per = a.by_per;
   p.scale_log2 = a.scale_log2;
   p.causal = a.causal;
-  p.part = static_cast<float*>(workspace);
-  p.part_ml = p.part + static_cast<size_t>(t.ctas) * kTcRows * a.c.head_dim;
+  char* scratch = static_cast<char*>(workspace);
+  CUtensorMap tk = {}, tv = {};
+  if (t.rows) {
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.c.map.kv_heads * t.rows;
+    if (int s = dense_map(&tk, scratch, bf16_type, rows, D)) return s;
+    if (int s = dense_map(&tv, scratch + t.side_bytes, bf16_type, rows, D)) return s;
+    if (int s = expand(a.c, bf16_type, scratch, scratch + t.side_bytes, a.batch, t.rows, a.lengths, a.error_flag, st)) return s;
+  }
+  p.part = reinterpret_cast<float*>(scratch + 2 * t.side_bytes);
+  p.part_ml = p.part + static_cast<size_t>(t.ctas) * kTcRows * D;
   p.error_flag = a.error_flag;
   const tc::TestStall stall = tc::take_test_stall();
   p.wait_ns = stall.wait_ns;
   p.withhold = stall.withhold;
   const unsigned grid = static_cast<unsigned>(t.ctas);
-  return bf16_type ? dispatch_tc<true>(p, grid, st) : dispatch_tc<false>(p, grid, st);
+  return bf16_type ? dispatch_tc<true>(tk, tv, p, grid, st) : dispatch_tc<false>(tk, tv, p, grid, st);
 }
 
 }  // namespace kv

@@ -22,7 +22,6 @@ namespace kv {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int64_t kMaxRows = (1ll << 31) - (1 << 16);  // row numbers of a block past the last one stay 32-bit
 
 // Two floats in one 64-bit register, for the packed fp32 instructions (each half rounds like the scalar one).
 __device__ __forceinline__ uint64_t two(float lo, float hi) {
@@ -342,8 +341,10 @@ struct FetchParams {
 // a row to a thread, as in update_kernel.  A code becomes a float by a byte
 // permutation into 2^23 + code (conversions run at an eighth of the rate),
 // two values to an instruction from there.
-template <typename T, int BITS, int D>
+// EXPAND: as expand() says.
+template <typename T, int BITS, int D, bool EXPAND>
 __global__ void __launch_bounds__(kThreads) fetch_kernel(const FetchParams p) {
+  if (EXPAND) asm volatile("griddepcontrol.launch_dependents;");
   constexpr int LANES = D / 16;
   constexpr int PER_PASS = kThreads / LANES;
   constexpr int W = BITS / 4;  // words of eight codes
@@ -352,14 +353,18 @@ __global__ void __launch_bounds__(kThreads) fetch_kernel(const FetchParams p) {
   const int row0 = blockIdx.x * (PER_PASS * kRows) + static_cast<int>(threadIdx.x) / LANES;
   const int ng = D / p.c.group, shift = p.c.group == 32 ? 5 : p.c.group == 64 ? 6 : 7;
   uint32_t at[kRows];
+  bool skip[kRows];
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
     const int row = row0 + u * PER_PASS;
     at[u] = kNoRow;
+    skip[u] = row >= p.rows;
     if (row < p.rows) {
       int b, h, pos;
       split_row(p.split, row, b, h, pos);
-      if (pos < __ldg(p.lengths + b)) {
+      const int length = __ldg(p.lengths + b);
+      if (EXPAND) skip[u] = (pos & ~127) >= length;
+      if (pos < length) {
         at[u] = row_of(p.c.map, b, h, pos);
         if (at[u] == kNoRow) atomicExch(p.error_flag, PHEW_ERR_INVALID);
       }
@@ -383,12 +388,20 @@ __global__ void __launch_bounds__(kThreads) fetch_kernel(const FetchParams p) {
       const int64_t s_at = static_cast<int64_t>(at[u]) * ng + ((half * (D / 2) + c * 8) >> shift);
       sc[u][half] = static_cast<const T*>(p.c.scales[side])[s_at];
       bi[u][half] = static_cast<const T*>(p.c.biases[side])[s_at];
+      if (EXPAND) {
+        const float s = to_f32(side ? sc[u][half] : static_cast<const T*>(p.c.scales[1])[s_at]);
+        const float z = to_f32(side ? bi[u][half] : static_cast<const T*>(p.c.biases[1])[s_at]);
+        if (!(fabsf(s) < INFINITY && fabsf(z) < INFINITY)) {
+          sc[u][half] = from_f32<T>(0.f);
+          bi[u][half] = from_f32<T>(side ? 0.f : __int_as_float(0x7fc00000));
+        }
+      }
     }
   }
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
     const int row = row0 + u * PER_PASS;
-    if (row >= p.rows) continue;
+    if (skip[u]) continue;
     T* dst = static_cast<T*>(p.dense[side]) + static_cast<int64_t>(row) * D + c * 8;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -450,10 +463,19 @@ template <typename T> int update_typed(const UpdateParams& p, cudaStream_t st) {
 template <typename T, int BITS> void launch_fetch(const FetchParams& p, cudaStream_t st) {
   const dim3 grid = grid_for(p.rows, p.c.head_dim);
   switch (p.c.head_dim) {
-    case 64: fetch_kernel<T, BITS, 64><<<grid, kThreads, 0, st>>>(p); break;
-    case 128: fetch_kernel<T, BITS, 128><<<grid, kThreads, 0, st>>>(p); break;
-    default: fetch_kernel<T, BITS, 256><<<grid, kThreads, 0, st>>>(p); break;
+    case 64: fetch_kernel<T, BITS, 64, false><<<grid, kThreads, 0, st>>>(p); break;
+    case 128: fetch_kernel<T, BITS, 128, false><<<grid, kThreads, 0, st>>>(p); break;
+    default: fetch_kernel<T, BITS, 256, false><<<grid, kThreads, 0, st>>>(p); break;
   }
+}
+
+template <typename T> int expand_typed(const FetchParams& p, cudaStream_t st) {
+  const dim3 grid = grid_for(p.rows, p.c.head_dim);
+  if (p.c.head_dim == 64)
+    fetch_kernel<T, 4, 64, true><<<grid, kThreads, 0, st>>>(p);
+  else
+    fetch_kernel<T, 4, 128, true><<<grid, kThreads, 0, st>>>(p);
+  return launch_status("kv expand");
 }
 
 template <typename T> int fetch_typed(const FetchParams& p, cudaStream_t st) {
@@ -465,6 +487,19 @@ template <typename T> int fetch_typed(const FetchParams& p, cudaStream_t st) {
 }
 
 }  // namespace
+
+int expand(const Cache& c, bool bf16_type, void* k, void* v, int64_t batch, int64_t rows, const int32_t* lengths,
+           int* error_flag, cudaStream_t st) {
+  FetchParams p;
+  p.c = c;
+  p.dense[0] = k;
+  p.dense[1] = v;
+  p.lengths = lengths;
+  p.split = {fast_div(static_cast<uint32_t>(rows)), fast_div(static_cast<uint32_t>(c.map.kv_heads))};
+  p.rows = static_cast<int>(batch * c.map.kv_heads * rows);
+  p.error_flag = error_flag;
+  return bf16_type ? expand_typed<bf16>(p, st) : expand_typed<f16>(p, st);
+}
 
 int make_cache(const phew_kv_cache* c, const int* table, int64_t table_stride, int64_t columns, int64_t batch,
                const char* who, Cache* out) {

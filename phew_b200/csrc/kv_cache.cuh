@@ -20,5 +20,16 @@ struct Cache {
 int make_cache(const phew_kv_cache* c, const int* table, int64_t table_stride, int64_t columns, int64_t batch,
                const char* who, Cache* out);
 
+constexpr int64_t kMaxRows = (1ll << 31) - (1 << 16);  // row numbers of a block past the last one stay 32-bit
+
+// Values of a cache of 16-bit type as [batch][kv_heads][rows][head_dim]
+// arrays, for attention's tiles of 128 keys: written up to a sequence's last
+// tile, zero behind its last key.  A key whose value's scale or bias is not
+// finite gets zero for a value and NaN for a key: a masked weight of zero
+// would make a NaN of it, and rows that see it get one through their score.
+// Launched so that a programmatic dependent may be set up meanwhile.
+int expand(const Cache& c, bool bf16_type, void* k, void* v, int64_t batch, int64_t rows, const int32_t* lengths,
+           int* error_flag, cudaStream_t st);
+
 }  // namespace kv
 }  // namespace phew
