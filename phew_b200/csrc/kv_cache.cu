@@ -46,13 +46,6 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
-// max(a, |b|, |c|), NaN when one of them is
-__device__ __forceinline__ float max_abs(float a, float b, float c) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
-  return d;
-}
-
 // Eight consecutive elements of a token row, as they lie in memory.
 template <typename T> struct Eight {
   uint32_t w[2 * sizeof(T)];
@@ -160,11 +153,31 @@ template <> struct Range<float> {
 struct RowSplit {
   FastDiv by_n, by_heads;
 };
-__device__ __forceinline__ void split_row(const RowSplit& s, int row, int& b, int& h, int& i) {
+struct Row {
+  int b, h, i;
+};
+__device__ __forceinline__ Row split_row(const RowSplit& s, int row) {
+  Row r;
   const int bh = static_cast<int>(div_by(s.by_n, static_cast<uint32_t>(row)));
-  i = row - bh * static_cast<int>(s.by_n.d);
-  b = static_cast<int>(div_by(s.by_heads, static_cast<uint32_t>(bh)));
-  h = bh - b * static_cast<int>(s.by_heads.d);
+  r.i = row - bh * static_cast<int>(s.by_n.d);
+  r.b = static_cast<int>(div_by(s.by_heads, static_cast<uint32_t>(bh)));
+  r.h = bh - r.b * static_cast<int>(s.by_heads.d);
+  return r;
+}
+// Row `first` + l of a block of at most `most` rows whose first is known: no division where a block spans two
+// heads at most.
+__device__ __forceinline__ Row row_after(const RowSplit& s, const Row& first, int first_row, int l, uint32_t most) {
+  if (s.by_n.d < most) return split_row(s, first_row + l);
+  Row r = first;
+  r.i += l;
+  if (r.i >= static_cast<int>(s.by_n.d)) {
+    r.i -= static_cast<int>(s.by_n.d);
+    if (++r.h == static_cast<int>(s.by_heads.d)) {
+      r.h = 0;
+      ++r.b;
+    }
+  }
+  return r;
 }
 
 // Token rows a thread works on at once: their loads are in flight together.
@@ -189,48 +202,57 @@ struct UpdateParams {
 // The group's scale and bias, and the reciprocal that codes are taken with.
 struct Affine {
   float sc, bi, inv;
-  bool plain;  // every quotient lies in [0, top + 1/2): no clamping
+  bool plain;  // quotients lie in [0, top + 1/2), and the reciprocal's steps below give them
 };
 template <typename T, int BITS> __device__ __forceinline__ Affine affine_of(const Range<T>& r) {
-  constexpr float top = (1 << BITS) - 1;
+  constexpr float top = (1 << BITS) - 1, part = 1.f / top;
   Affine a;
-  const float lo = r.lo(), hi = r.hi();
-  a.sc = round_to<T>(fmaxf(__fdiv_rn(hi - lo, top), 1e-8f));
+  const float lo = r.lo(), hi = r.hi(), d = hi - lo;
+  // d / top by the rounded reciprocal of top and the remainder: the IEEE quotient (Markstein, "Computation of
+  // elementary functions on the IBM RISC System/6000 processor", 1990; checked for every mantissa of d) unless
+  // something over- or underflows; below 1e-8 it does not count
+  float q = d * part;
+  q = fmaf(fmaf(-top, q, d), part, q);
+  if (!(d < 1e38f)) q = __fdiv_rn(d, top);
+  a.sc = round_to<T>(fmaxf(q, 1e-8f));
   a.bi = lo;  // a value of type T
   a.inv = __frcp_rn(a.sc);
-  a.plain = (hi - lo) * a.inv < top + 0.4999f;
+  a.plain = d * a.inv < top + 0.4999f;
+  if (sizeof(T) == 4) a.plain = a.plain && (__float_as_uint(a.sc) & 0x7fffffu) != 0x7fffffu;
   return a;
 }
 
-// Codes of eight values: words for the cache, and as floats.  The product
-// with the reciprocal lies within three roundings of the IEEE quotient, so it
-// names the same code unless it falls next to a border between two; only such
-// values (one in a few hundred of bf16 data, whose quotients often hit a
-// border exactly) are divided.  Two values to an instruction throughout.
+// Codes of eight values: words for the cache, and as floats.  (x - bias) /
+// scale is the product with the rounded reciprocal corrected by its remainder
+// (Markstein's steps: one gives the IEEE quotient of a 16-bit type's short
+// scale, two that of any scale but the one of all-ones mantissa), two values to
+// an instruction.  Ties between codes are frequent in 16-bit data (one value
+// in 450 of bf16 normals), so a quotient that is only nearly right would need
+// a second look in every third warp.
 template <typename T, int BITS>
 __device__ __forceinline__ void codes8(const Eight<T>& x, const Affine& a, uint32_t* words, uint64_t* q) {
   constexpr float top = (1 << BITS) - 1;
-  constexpr float sure = 0.5f - (BITS == 4 ? 1.f / (1 << 17) : 1.f / (1 << 13));  // three roundings of 2 top
-  const uint64_t nb = two(-a.bi, -a.bi), inv = two(a.inv, a.inv), up = two(kRound, kRound), down = two(-kRound, -kRound);
-  uint64_t v[4], t[4];
-  float off = 0.f;
+  const uint64_t nb = two(-a.bi, -a.bi), inv = two(a.inv, a.inv), ns = two(-a.sc, -a.sc);
+  const uint64_t up = two(kRound, kRound), down = two(-kRound, -kRound);
+  uint64_t t[4], any = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    v[i] = mul2(add2(pair_of(x, i), nb), inv);
-    t[i] = add2(v[i], up);
+    const uint64_t d = add2(pair_of(x, i), nb);
+    any = add2(any, d);
+    uint64_t v = mul2(d, inv);
+#pragma unroll
+    for (int k = 0; k < static_cast<int>(sizeof(T)) / 2; ++k) v = fma2(fma2(ns, v, d), inv, v);
+    t[i] = add2(v, up);
     q[i] = add2(t[i], down);
-    v[i] = fma2(q[i], two(-1.f, -1.f), v[i]);
-    off = max_abs(off, lo_of(v[i]), hi_of(v[i]));
   }
-  if (!(off < sure) || !a.plain) {
+  if (!a.plain || !(lo_of(any) + hi_of(any) < INFINITY)) {  // odd scales, or a value that is no number (code 0)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint64_t xs = pair_of(x, i);
-      float f[2] = {lo_of(q[i]), hi_of(q[i])};
+      float f[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        if (!a.plain || !(fabsf(k ? hi_of(v[i]) : lo_of(v[i])) < sure))
-          f[k] = fminf(fmaxf(rintf(__fdiv_rn((k ? hi_of(xs) : lo_of(xs)) - a.bi, a.sc)), 0.f), top);
+        f[k] = fminf(fmaxf(rintf(__fdiv_rn((k ? hi_of(xs) : lo_of(xs)) - a.bi, a.sc)), 0.f), top);
       q[i] = two(f[0], f[1]);
       t[i] = add2(q[i], up);
     }
@@ -260,7 +282,8 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const UpdateParams p) 
   constexpr int NG = D / G;
   const int side = blockIdx.y;
   const int c = threadIdx.x % LANES;
-  const int row0 = blockIdx.x * (PER_PASS * kRows) + static_cast<int>(threadIdx.x) / LANES;
+  const int first_row = blockIdx.x * (PER_PASS * kRows), row0 = first_row + static_cast<int>(threadIdx.x) / LANES;
+  const Row first = split_row(p.split, first_row);
   const T* xs = static_cast<const T*>(p.x[side]);
   Eight<T> in[kRows][2];
   int b[kRows], h[kRows], tok[kRows];
@@ -270,7 +293,10 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const UpdateParams p) 
     tok[u] = -1;
     in[u][0] = in[u][1] = Eight<T>{};
     if (row < p.rows) {
-      split_row(p.split, row, b[u], h[u], tok[u]);
+      const Row r = row_after(p.split, first, first_row, row - first_row, PER_PASS * kRows);
+      b[u] = r.b;
+      h[u] = r.h;
+      tok[u] = r.i;
       const T* x = xs + b[u] * p.st[side][2] + h[u] * p.st[side][1] + tok[u] * p.st[side][0] + c * 8;
       in[u][0] = load8(x);
       in[u][1] = load8(x + D / 2);
@@ -350,7 +376,8 @@ __global__ void __launch_bounds__(kThreads) fetch_kernel(const FetchParams p) {
   constexpr int W = BITS / 4;  // words of eight codes
   const int side = blockIdx.y;
   const int c = threadIdx.x % LANES;
-  const int row0 = blockIdx.x * (PER_PASS * kRows) + static_cast<int>(threadIdx.x) / LANES;
+  const int first_row = blockIdx.x * (PER_PASS * kRows), row0 = first_row + static_cast<int>(threadIdx.x) / LANES;
+  const Row first = split_row(p.split, first_row);
   const int ng = D / p.c.group, shift = p.c.group == 32 ? 5 : p.c.group == 64 ? 6 : 7;
   uint32_t at[kRows];
   bool skip[kRows];
@@ -360,12 +387,11 @@ __global__ void __launch_bounds__(kThreads) fetch_kernel(const FetchParams p) {
     at[u] = kNoRow;
     skip[u] = row >= p.rows;
     if (row < p.rows) {
-      int b, h, pos;
-      split_row(p.split, row, b, h, pos);
-      const int length = __ldg(p.lengths + b);
-      if (EXPAND) skip[u] = (pos & ~127) >= length;
-      if (pos < length) {
-        at[u] = row_of(p.c.map, b, h, pos);
+      const Row r = row_after(p.split, first, first_row, row - first_row, PER_PASS * kRows);
+      const int length = __ldg(p.lengths + r.b);
+      if (EXPAND) skip[u] = (r.i & ~127) >= length;
+      if (r.i < length) {
+        at[u] = row_of(p.c.map, r.b, r.h, r.i);
         if (at[u] == kNoRow) atomicExch(p.error_flag, PHEW_ERR_INVALID);
       }
     }
