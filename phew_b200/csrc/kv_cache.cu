@@ -21,7 +21,7 @@ namespace phew {
 namespace kv {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 // Two floats in one 64-bit register, for the packed fp32 instructions (each half rounds like the scalar one).
 __device__ __forceinline__ uint64_t two(float lo, float hi) {
@@ -195,7 +195,7 @@ struct UpdateParams {
   const int32_t* offsets;
   const int32_t* counts;  // null: all `tokens`
   RowSplit split;
-  int rows, tokens;
+  int rows;
   int* error_flag;
 };
 
@@ -216,7 +216,15 @@ template <typename T, int BITS> __device__ __forceinline__ Affine affine_of(cons
   if (!(d < 1e38f)) q = __fdiv_rn(d, top);
   a.sc = round_to<T>(fmaxf(q, 1e-8f));
   a.bi = lo;  // a value of type T
-  a.inv = __frcp_rn(a.sc);
+  if (sizeof(T) == 2) {
+    // one Newton step from one unit in the last place: the rounded reciprocal of a mantissa of 8 or 11 bits
+    // (whose reciprocals keep 2^-36 away from the middle between two floats)
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(a.sc));
+    a.inv = fmaf(fmaf(-a.sc, y, 1.f), y, y);
+  } else {
+    a.inv = __frcp_rn(a.sc);
+  }
   a.plain = d * a.inv < top + 0.4999f;
   if (sizeof(T) == 4) a.plain = a.plain && (__float_as_uint(a.sc) & 0x7fffffu) != 0x7fffffu;
   return a;
@@ -286,20 +294,26 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const UpdateParams p) 
   const Row first = split_row(p.split, first_row);
   const T* xs = static_cast<const T*>(p.x[side]);
   Eight<T> in[kRows][2];
-  int b[kRows], h[kRows], tok[kRows];
+  bool have[kRows];     // a row of x
+  bool live[kRows];     // ... that goes into the cache
+  uint32_t at[kRows];   // ... there
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
     const int row = row0 + u * PER_PASS;
-    tok[u] = -1;
+    have[u] = row < p.rows;
+    live[u] = false;
+    at[u] = kNoRow;
     in[u][0] = in[u][1] = Eight<T>{};
-    if (row < p.rows) {
+    if (have[u]) {
       const Row r = row_after(p.split, first, first_row, row - first_row, PER_PASS * kRows);
-      b[u] = r.b;
-      h[u] = r.h;
-      tok[u] = r.i;
-      const T* x = xs + b[u] * p.st[side][2] + h[u] * p.st[side][1] + tok[u] * p.st[side][0] + c * 8;
+      const T* x = xs + r.b * p.st[side][2] + r.h * p.st[side][1] + r.i * p.st[side][0] + c * 8;
       in[u][0] = load8(x);
       in[u][1] = load8(x + D / 2);
+      live[u] = !p.counts || r.i < __ldg(p.counts + r.b);
+      if (live[u]) {
+        at[u] = row_of(p.c.map, r.b, r.h, static_cast<int64_t>(__ldg(p.offsets + r.b)) + r.i);
+        if (at[u] == kNoRow) atomicExch(p.error_flag, PHEW_ERR_INVALID);
+      }
     }
   }
 #pragma unroll
@@ -313,33 +327,30 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const UpdateParams p) 
       r[1].across(LG);
     else
       r[1] = r[0];
-    if (tok[u] < 0) continue;
-    const int count = p.counts ? clamp_count(__ldg(p.counts + b[u]), p.tokens) : p.tokens;
+    if (!have[u]) continue;
     T* dense = nullptr;
     if (p.dense[side]) dense = static_cast<T*>(p.dense[side]) + static_cast<int64_t>(row0 + u * PER_PASS) * D + c * 8;
-    if (tok[u] >= count) {
+    if (!live[u]) {
       if (dense) {
         store8(dense, Eight<T>{});
         store8(dense + D / 2, Eight<T>{});
       }
       continue;
     }
-    const uint32_t at = row_of(p.c.map, b[u], h[u], static_cast<int64_t>(__ldg(p.offsets + b[u])) + tok[u]);
-    if (at == kNoRow) atomicExch(p.error_flag, PHEW_ERR_INVALID);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const Affine a = affine_of<T, BITS>(r[half]);
       uint32_t words[BITS / 4];
       uint64_t q[4];
       codes8<T, BITS>(in[u][half], a, words, q);
-      if (at != kNoRow) {
-        uint32_t* dst = p.c.codes[side] + static_cast<int64_t>(at) * (D * BITS / 32) + (half * (D / 16) + c) * (BITS / 4);
+      if (at[u] != kNoRow) {
+        uint32_t* dst = p.c.codes[side] + static_cast<int64_t>(at[u]) * (D * BITS / 32) + (half * (D / 16) + c) * (BITS / 4);
         if (BITS == 4)
           dst[0] = words[0];
         else
           *reinterpret_cast<uint2*>(dst) = make_uint2(words[0], words[BITS / 4 - 1]);
         if (c % LG == 0 && (G < D || half == 0)) {
-          const int64_t s_at = static_cast<int64_t>(at) * NG + (half * (D / 2) + c * 8) / G;
+          const int64_t s_at = static_cast<int64_t>(at[u]) * NG + (half * (D / 2) + c * 8) / G;
           static_cast<T*>(p.c.scales[side])[s_at] = from_f32<T>(a.sc);
           static_cast<T*>(p.c.biases[side])[s_at] = from_f32<T>(a.bi);
         }
@@ -603,7 +614,6 @@ extern "C" int phew_kv_update(const phew_kv_cache* cache, const void* k, const v
   p.counts = counts;
   p.split = {kv::fast_div(static_cast<uint32_t>(tokens)), kv::fast_div(static_cast<uint32_t>(cache->kv_heads))};
   p.rows = static_cast<int>(batch * cache->kv_heads * tokens);
-  p.tokens = static_cast<int>(tokens);
   p.error_flag = error_flag;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (cache->dtype) {
