@@ -349,22 +349,23 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
   const int kv_heads = p.c.map.kv_heads;
 
   // ---- this warp's share of the line: of W units the first W mod n warps take one more ----
+  asm volatile("griddepcontrol.launch_dependents;");  // the combine kernel may be set up from here on; it waits for this one
   const int entries = p.batch * p.blocks;
-  uint32_t own = 0;  // units of this thread's entry (of the first of several) for one head
-  uint64_t mine = 0;
+  uint32_t own = 0;  // units of this thread's first entry for one head
+  uint64_t sum = 0;
   for (int e = threadIdx.x; e < entries; e += kWarps * 32) {
     const Entry t = entry_at(p, e, ROWS);
     const uint32_t units = t.tiles + kBegin;
     if (e == static_cast<int>(threadIdx.x)) own = units;
-    mine += units;
+    sum += units;
     if (blockIdx.x == 0 && t.block == 0 && __ldg(p.lengths + t.b) != t.length) atomicExch(p.error_flag, PHEW_ERR_INVALID);
   }
-  asm volatile("griddepcontrol.launch_dependents;");  // the combine kernel may be set up from here on; it waits for this one
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) s_red[warp] = mine;
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) s_red[warp] = sum;
   __syncthreads();
-  const uint64_t total = (s_red[0] + s_red[1] + s_red[2] + s_red[3]) * kv_heads;
+  sum = s_red[0] + s_red[1] + s_red[2] + s_red[3];
+  const uint64_t total = sum * kv_heads;
   const uint32_t all_warps = gridDim.x * kWarps;
   const uint32_t n = total < all_warps ? static_cast<uint32_t>(total) : all_warps;
   if (blockIdx.x >= n) return;  // no warp of the block has work
@@ -376,11 +377,12 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
   uint64_t x = self * each + min(self, more);
   const uint64_t x_end = x + each + (self < more);
   // the entry that the first unit lies in: the first whose units, with those before it, pass x / kv_heads
-  if (lane == 0) s_target[warp] = self < n ? (narrow ? static_cast<uint32_t>(x) / static_cast<uint32_t>(kv_heads) : x / kv_heads) : ~0ull;
+  if (lane == 0)
+    s_target[warp] = self < n ? (narrow ? static_cast<uint32_t>(x) / static_cast<uint32_t>(kv_heads) : x / kv_heads) : ~0ull;
   uint64_t run = 0;
   for (int e0 = 0; e0 < entries; e0 += kWarps * 32) {
-    const int e = e0 + static_cast<int>(threadIdx.x);
-    if (e0 > 0) own = e < entries ? entry_at(p, e, ROWS).tiles + kBegin : 0;
+    const int i = e0 + static_cast<int>(threadIdx.x);
+    if (e0 > 0) own = i < entries ? entry_at(p, i, ROWS).tiles + kBegin : 0;
     uint64_t inc = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -395,21 +397,22 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
     uint64_t most = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const uint64_t target = s_target[w];
-      if (inc > target && inc - own <= target) {
-        s_entry[w] = e;
+      const uint64_t want = s_target[w];
+      if (inc > want && inc - own <= want) {
+        s_entry[w] = i;
         s_prefix[w] = inc - own;
       }
-      if (target != ~0ull) most = target;  // (targets grow with the warp)
+      if (want != ~0ull) most = want;  // (targets grow with the warp)
     }
     run += s_red[0] + s_red[1] + s_red[2] + s_red[3];
     if (run > most) break;
   }
   __syncthreads();
   int e = s_entry[warp];
-  uint64_t base = s_prefix[warp] * kv_heads;
+  uint64_t base = s_prefix[warp];
   __syncthreads();  // (the ring takes the shared memory over; the last barrier)
   if (self >= n) return;
+  base *= kv_heads;
 
   Ring<S, T> ring{p.c, smem_addr(smem) + warp * S::RING, lane, 0u};
 
@@ -912,12 +915,13 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
 }
 
 // Joins the partials of a segment: partial 1 of its first warp, then the
-// partials 0 of the warps after it, in that order.  A warp to a row and a block
-// to a segment; or (WIDE, for segments of many partials) a block to a row, its
-// warps taking every eighth partial each, joined in shared memory.
-template <typename S, typename T, bool WIDE>
-__global__ void __launch_bounds__(256) combine_kernel(const AttnParams p) {
+// partials 0 of the warps after it, in that order.  WARPS 1: a warp to a row, a
+// block to eight rows of a segment.  Else a block to a row, its warps taking
+// every WARPS-th partial each, joined in shared memory.
+template <typename S, typename T, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS) combine_kernel(const AttnParams p) {
   constexpr int D = S::D, ROWS = S::ROWS, E = D / 32;
+  constexpr bool WIDE = WARPS > 1;
   const int segment = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // attn_kernel is done and its partials are visible
   const int2 span = p.span[segment];
@@ -936,7 +940,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnParams p) {
 #pragma unroll
   for (int i = 0; i < E; ++i) o[i] = 0.f;
 #pragma unroll 4
-  for (int k = span.x + (WIDE ? warp : 0); k <= span.y; k += WIDE ? 8 : 1) {
+  for (int k = span.x + (WIDE ? warp : 0); k <= span.y; k += WARPS) {
     const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at(k) * 2);
     const float2* v = reinterpret_cast<const float2*>(p.part + at(k) * D) + lane;
     const float m_new = fmaxf(m, ml.x), was = exp2_fast(m - m_new), f = exp2_fast(ml.x - m_new);
@@ -950,7 +954,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnParams p) {
     }
   }
   if constexpr (WIDE) {
-    __shared__ float s_o[8][D], s_l[8], s_m[8];
+    __shared__ float s_o[WARPS][D], s_l[WARPS], s_m[WARPS];
 #pragma unroll
     for (int i = 0; i < E; i += 2) *reinterpret_cast<float2*>(&s_o[warp][i * 32 + lane * 2]) = make_float2(o[i], o[i + 1]);
     if (lane == 0) {
@@ -960,12 +964,12 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnParams p) {
     __syncthreads();
     if (warp) return;
 #pragma unroll
-    for (int w = 1; w < 8; ++w) m = fmaxf(m, s_m[w]);
+    for (int w = 1; w < WARPS; ++w) m = fmaxf(m, s_m[w]);
     l = 0.f;
 #pragma unroll
     for (int i = 0; i < E; ++i) o[i] = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       const float f = exp2_fast(s_m[w] - m);
       l = fmaf(f, s_l[w], l);
 #pragma unroll
@@ -1029,18 +1033,21 @@ template <typename S, typename T> int launch_attn(AttnParams p, void* workspace,
   if (int s = launch_status("kv attn_kernel")) return s;
   // a programmatic dependent: set up while attn_kernel runs
   cudaLaunchConfig_t cfg = {};
-  // partials of a segment: about the warps that it could be spread over
-  const bool wide = segments * 16 < static_cast<int64_t>(grid_of<S>()) * kWarps;
-  cfg.gridDim = dim3(static_cast<unsigned>(segments), wide ? S::ROWS : S::NT);
-  cfg.blockDim = dim3(256);
+  // partials to a segment: about the warps that it could be spread over.  Up to four, one warp reads them in one
+  // go; eight warps (18 to a segment: 15 us for a call, 24 with one warp); sixteen (222: 45 us, 49 with eight)
+  const int64_t spread = static_cast<int64_t>(grid_of<S>()) * kWarps / segments;
+  const int warps = spread <= 4 ? 1 : spread <= 64 ? 8 : 16;
+  cfg.gridDim = dim3(static_cast<unsigned>(segments), warps > 1 ? S::ROWS : S::NT);
+  cfg.blockDim = dim3(warps > 1 ? 32 * warps : 256);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  PHEW_CHECK_CUDA(wide ? cudaLaunchKernelEx(&cfg, combine_kernel<S, T, true>, p)
-                       : cudaLaunchKernelEx(&cfg, combine_kernel<S, T, false>, p));
+  PHEW_CHECK_CUDA(warps == 1   ? cudaLaunchKernelEx(&cfg, combine_kernel<S, T, 1>, p)
+                  : warps == 8 ? cudaLaunchKernelEx(&cfg, combine_kernel<S, T, 8>, p)
+                               : cudaLaunchKernelEx(&cfg, combine_kernel<S, T, 16>, p));
   return launch_status("kv combine_kernel");
 }
 
