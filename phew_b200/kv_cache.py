@@ -194,6 +194,11 @@ def _rows(x, what: str, cache: QuantizedKVCache):
     return t, _strides(n, h, b)
 
 
+def _empty_like(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous array like `t` (empty_like is the quickest way to one, but keeps a view's strides)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _stream(cache: QuantizedKVCache) -> int:
     return torch.cuda.current_stream(cache.device).cuda_stream
 
@@ -259,7 +264,7 @@ def quantized_cache_update(cache: QuantizedKVCache, k, v, offsets, *, block_tabl
     keep, table, stride, columns = _table(block_table, batch, "quantized_cache_update", cache)
     out = None
     if fetch:
-        out = (k.new_empty(shape), k.new_empty(shape))
+        out = (_empty_like(k), _empty_like(k))
     _call("phew_kv_update", cache, k.data_ptr(), v.data_ptr(), ks, vs, batch, tokens, off.data_ptr(),
           None if cnt is None else cnt.data_ptr(), table, stride, columns,
           out[0].data_ptr() if fetch else None, out[1].data_ptr() if fetch else None)
@@ -284,7 +289,8 @@ def quantized_cache_fetch(cache: QuantizedKVCache, lengths, *, block_table=None,
         raise ValueError(f"quantized_cache_fetch: max_length must be positive, got {max_length}")
     shape = (batch, cache.kv_heads, out_len, cache.head_dim)
     one = cache.keys[1]._t
-    k, v = one.new_empty(shape), one.new_empty(shape)
+    k = one.new_empty(shape)
+    v = torch.empty_like(k)
     _call("phew_kv_fetch", cache, k.data_ptr(), v.data_ptr(), batch, out_len, n.data_ptr(), table, stride, columns)
     del keep
     return core.array._wrap(k), core.array._wrap(v)
@@ -318,7 +324,7 @@ def quantized_cache_attention(q, cache: QuantizedKVCache, lengths, *, block_tabl
     size = _workspace(cache.device.index, cache.page_size, cache.kv_heads, cache.head_dim, cache.group_size,
                       cache.dtype.code, batch, heads, tokens, columns)
     work = n.new_empty(size // 4)
-    o = q.new_empty(shape)
+    o = _empty_like(q)
     _call("phew_kv_attention", cache, q.data_ptr(), qs, o.data_ptr(), batch, heads, tokens, n.data_ptr(),
           None if cnt is None else cnt.data_ptr(), table, stride, columns, scale, 0 if mask is None else 1,
           work.data_ptr(), size)
