@@ -80,6 +80,7 @@ struct TcParams {
   int blocks;  // 256-row blocks of a cache head
   int splits;
   int rows;    // dense: token rows of a cache head in the expanded keys and values
+  bool q_tma;  // dense: tiles of queries arrive by TMA too
   FastDiv by_per;
   float scale_log2;  // > 0
   bool causal;
@@ -123,7 +124,8 @@ __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy
 
 template <typename S, bool BF16, bool DENSE>
 __global__ void __launch_bounds__(tc_threads(DENSE), 1)
-    attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const TcParams p) {
+    attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                   const __grid_constant__ CUtensorMap tm_v, const TcParams p) {
   constexpr int D = S::D, NG = S::NG;
   constexpr int FIRST = DENSE ? 2 : 1 + kProducers;  // softmax warp
   using T = typename std::conditional<BF16, bf16, f16>::type;
@@ -149,13 +151,14 @@ __global__ void __launch_bounds__(tc_threads(DENSE), 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // ---- which rows and which keys ----
-  // Row blocks from the last (the longest under a causal mask) down; the heads and sequences of one row
-  // block side by side.
+  // Cache heads in groups of 16, so that the CTAs running at one time share few heads' keys in the L2; within a
+  // group row blocks from the last (the longest under a causal mask) down, a block's heads and splits together.
   const int kv_heads = p.c.map.kv_heads;
-  const int per_block = p.batch * kv_heads * p.splits;
-  const int rb = p.blocks - 1 - static_cast<int>(blockIdx.x) / per_block;
-  const int rest = static_cast<int>(blockIdx.x) % per_block;
-  const int split = rest % p.splits, bh = rest / p.splits;
+  const int all_heads = p.batch * kv_heads, in_group = 16 * p.blocks * p.splits;
+  const int group = static_cast<int>(blockIdx.x) / in_group, rem = static_cast<int>(blockIdx.x) % in_group;
+  const int wide = min(16, all_heads - 16 * group) * p.splits;
+  const int rb = p.blocks - 1 - rem / wide;
+  const int split = rem % wide % p.splits, bh = 16 * group + rem % wide / p.splits;
   const int b = bh / kv_heads, h = bh % kv_heads;
   const int count = p.counts ? clamp_count(__ldg(p.counts + b), p.tokens) : p.tokens;
   const int length = clamp_count(__ldg(p.lengths + b), capacity(p.c.map));
@@ -177,7 +180,7 @@ __global__ void __launch_bounds__(tc_threads(DENSE), 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 4);
+      mbar_init(&q_full[i], DENSE && p.q_tma ? 1 : 4);
       mbar_init(&k_full[i], DENSE ? 1 : 4);
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], DENSE ? 1 : 4);
@@ -189,6 +192,18 @@ __global__ void __launch_bounds__(tc_threads(DENSE), 1)
     mbar_init(drain, 1);
     *s_poison = 0x7fffffff;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (DENSE && p.q_tma) {
+      // rows token * per + head: boxes of `per` heads x 128 / per tokens
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (n_t[t] > 0) {
+          mbar_expect_tx(&q_full[t], S::TILE_BYTES);
+          const int tok = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(row0 + t * kTileRows)));
+#pragma unroll
+          for (int i = 0; i < S::HALVES; ++i)
+            tma_load_4d(sQ + t * S::TILE_BYTES + i * S::HALF_BYTES, &tm_q, &q_full[t], i * 64, h * p.per, tok, b);
+        }
+    }
   }
   if (warp == 0) tmem_alloc(tmem_slot, kTmemCols);
   fence_before_sync();
@@ -394,7 +409,7 @@ __global__ void __launch_bounds__(tc_threads(DENSE), 1)
       const int r = row0 + t * kTileRows + row;
       const int tok = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(r)));
       lim = seen_end(length, count, tok, p.causal) - j0 * kTcTile;
-      if (nkv > 0) {
+      if (nkv > 0 && !(DENSE && p.q_tma)) {
         const bool have = tok < count;
         const uint4* q = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.st[2] +
                                                         (h * p.per + (r - tok * p.per)) * p.st[1] + tok * p.st[0]);
@@ -527,6 +542,9 @@ __global__ void __launch_bounds__(tc_threads(DENSE), 1)
   if (__syncthreads_or(!ok)) {
     // a wait ran out somewhere: let the issued products and loads finish before the TMEM and shared memory go
     if (warp == 0 && lane == 0) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (DENSE && p.q_tma && n_t[t] > 0) mbar_wait(&q_full[t], 0, nullptr, p.wait_ns);
       commit(drain);
       mbar_wait(drain, 0, nullptr, p.wait_ns);
     } else if (DENSE && warp == 1 && lane == 0) {
@@ -618,8 +636,12 @@ int dense_map(CUtensorMap* tm, const void* base, bool bf16_type, int64_t rows, i
   return make_map_16bit(tm, base, bf16_type, 2, dims, strides, box);
 }
 
+struct Maps {
+  CUtensorMap q, k, v;  // dense
+};
+
 template <typename S, bool BF16, bool DENSE>
-int launch_tc(const CUtensorMap& tk, const CUtensorMap& tv, const TcParams& p, unsigned grid, cudaStream_t st) {
+int launch_tc(const Maps& m, const TcParams& p, unsigned grid, cudaStream_t st) {
   static SmemAllowed allowed;
   if (int s = allow_smem(allowed, attn_tc_kernel<S, BF16, DENSE>, S::SMEM)) return s;
   cudaLaunchAttribute attr[1];
@@ -632,7 +654,7 @@ int launch_tc(const CUtensorMap& tk, const CUtensorMap& tv, const TcParams& p, u
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = DENSE ? 1 : 0;  // set up while the cache is expanded
-  PHEW_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_tc_kernel<S, BF16, DENSE>, tk, tv, p));
+  PHEW_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_tc_kernel<S, BF16, DENSE>, m.q, m.k, m.v, p));
   if (int s = launch_status("kv attn_tc_kernel")) return s;
   if (p.splits == 1) return PHEW_OK;
   cfg = {};
@@ -646,16 +668,16 @@ int launch_tc(const CUtensorMap& tk, const CUtensorMap& tv, const TcParams& p, u
 }
 
 template <bool BF16>
-int dispatch_tc(const CUtensorMap& tk, const CUtensorMap& tv, const TcParams& p, unsigned grid, cudaStream_t st) {
+int dispatch_tc(const Maps& m, const TcParams& p, unsigned grid, cudaStream_t st) {
   if (p.rows)  // (the group no longer matters)
-    return p.c.head_dim == 64 ? launch_tc<TcShape<64, 64>, BF16, true>(tk, tv, p, grid, st)
-                              : launch_tc<TcShape<128, 128>, BF16, true>(tk, tv, p, grid, st);
+    return p.c.head_dim == 64 ? launch_tc<TcShape<64, 64>, BF16, true>(m, p, grid, st)
+                              : launch_tc<TcShape<128, 128>, BF16, true>(m, p, grid, st);
   if (p.c.head_dim == 64)
-    return p.c.group == 32 ? launch_tc<TcShape<64, 32>, BF16, false>(tk, tv, p, grid, st)
-                           : launch_tc<TcShape<64, 64>, BF16, false>(tk, tv, p, grid, st);
-  if (p.c.group == 32) return launch_tc<TcShape<128, 32>, BF16, false>(tk, tv, p, grid, st);
-  if (p.c.group == 64) return launch_tc<TcShape<128, 64>, BF16, false>(tk, tv, p, grid, st);
-  return launch_tc<TcShape<128, 128>, BF16, false>(tk, tv, p, grid, st);
+    return p.c.group == 32 ? launch_tc<TcShape<64, 32>, BF16, false>(m, p, grid, st)
+                           : launch_tc<TcShape<64, 64>, BF16, false>(m, p, grid, st);
+  if (p.c.group == 32) return launch_tc<TcShape<128, 32>, BF16, false>(m, p, grid, st);
+  if (p.c.group == 64) return launch_tc<TcShape<128, 64>, BF16, false>(m, p, grid, st);
+  return launch_tc<TcShape<128, 128>, BF16, false>(m, p, grid, st);
 }
 
 }  // namespace
@@ -687,11 +709,22 @@ int run_attn_tc(const AttnParams& a, bool bf16_type, void* workspace, cudaStream
   p.scale_log2 = a.scale_log2;
   p.causal = a.causal;
   char* scratch = static_cast<char*>(workspace);
-  CUtensorMap tk = {}, tv = {};
+  Maps m = {};
+  p.q_tma = false;
   if (t.rows) {
     const int64_t rows = static_cast<int64_t>(a.batch) * a.c.map.kv_heads * t.rows;
-    if (int s = dense_map(&tk, scratch, bf16_type, rows, D)) return s;
-    if (int s = dense_map(&tv, scratch + t.side_bytes, bf16_type, rows, D)) return s;
+    if (int s = dense_map(&m.k, scratch, bf16_type, rows, D)) return s;
+    if (int s = dense_map(&m.v, scratch + t.side_bytes, bf16_type, rows, D)) return s;
+    // tiles of queries are boxes where a tile holds whole tokens and every axis has a stride
+    p.q_tma = kTileRows % a.per == 0 && a.st[0] > 0 && a.st[1] > 0 && a.st[2] > 0;
+    if (p.q_tma) {
+      const uint64_t dims[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(a.heads), static_cast<uint64_t>(a.tokens),
+                                static_cast<uint64_t>(a.batch)};
+      const uint64_t strides[3] = {static_cast<uint64_t>(a.st[1]) * 2, static_cast<uint64_t>(a.st[0]) * 2,
+                                   static_cast<uint64_t>(a.st[2]) * 2};
+      const uint32_t box[4] = {64, static_cast<uint32_t>(a.per), static_cast<uint32_t>(kTileRows / a.per), 1};
+      if (int s = make_map_16bit(&m.q, a.q, bf16_type, 4, dims, strides, box)) return s;
+    }
     if (int s = expand(a.c, bf16_type, scratch, scratch + t.side_bytes, a.batch, t.rows, a.lengths, a.error_flag, st)) return s;
   }
   p.part = reinterpret_cast<float*>(scratch + 2 * t.side_bytes);
@@ -701,7 +734,7 @@ int run_attn_tc(const AttnParams& a, bool bf16_type, void* workspace, cudaStream
   p.wait_ns = stall.wait_ns;
   p.withhold = stall.withhold;
   const unsigned grid = static_cast<unsigned>(t.ctas);
-  return bf16_type ? dispatch_tc<true>(tk, tv, p, grid, st) : dispatch_tc<false>(tk, tv, p, grid, st);
+  return bf16_type ? dispatch_tc<true>(m, p, grid, st) : dispatch_tc<false>(m, p, grid, st);
 }
 
 }  // namespace kv
