@@ -8,22 +8,6 @@
 // mx.fast.quantized_scaled_dot_product_attention (phew emit/codegen.py:428-449).
 #include "kv_attn_tc.cuh"
 
-namespace phew {
-namespace kv {
-namespace {
-
-// Query rows to a cache head from which the tcgen05 kernel takes over: below, the mma.sync kernel's one or
-// two passes over the cache cost less than a 256-row tile that is mostly empty.
-constexpr int64_t kTcMinRows = 64;
-
-bool takes_tc(int dtype, int head_dim, int64_t rows) {
-  return dtype != PHEW_F32 && head_dim <= 128 && rows >= kTcMinRows;
-}
-
-}  // namespace
-}  // namespace kv
-}  // namespace phew
-
 using namespace phew;
 
 extern "C" size_t phew_kv_attention_workspace(const phew_kv_cache* cache, int64_t batch, int64_t heads,
@@ -36,8 +20,9 @@ extern "C" size_t phew_kv_attention_workspace(const phew_kv_cache* cache, int64_
     case PHEW_F16: few = kv::attn_bytes<f16>(batch, cache->kv_heads, cache->head_dim, cache->group_size, rows); break;
     default: few = kv::attn_bytes<bf16>(batch, cache->kv_heads, cache->head_dim, cache->group_size, rows);
   }
-  if (kv::takes_tc(cache->dtype, cache->head_dim, rows))
-    many = kv::tc_bytes(batch, cache->kv_heads, cache->head_dim, rows, columns * cache->page_size);
+  const int64_t cap = columns * cache->page_size;
+  if (kv::takes_tc(batch, cache->kv_heads, cache->head_dim, cache->dtype, rows, cap))
+    many = kv::tc_bytes(batch, cache->kv_heads, cache->head_dim, rows, cap);
   return few > many ? few : many;
 }
 
@@ -78,7 +63,8 @@ extern "C" int phew_kv_attention(const phew_kv_cache* cache, const void* q, cons
   p.error_flag = error_flag;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // (the tcgen05 kernel takes its maxima over unscaled scores)
-  if (kv::takes_tc(cache->dtype, cache->head_dim, static_cast<int64_t>(p.tokens) * p.per) && p.scale_log2 > 0.f)
+  if (p.scale_log2 > 0.f && kv::takes_tc(batch, cache->kv_heads, cache->head_dim, cache->dtype,
+                                         static_cast<int64_t>(p.tokens) * p.per, kv::capacity(p.c.map)))
     return kv::run_attn_tc(p, cache->dtype == PHEW_BF16, workspace, st);
   switch (cache->dtype) {
     case PHEW_F32: return kv::run_attn<float>(p, workspace, st);

@@ -27,7 +27,8 @@
 //   last 8 warps  softmax of tile a and b, one query row per thread; they also
 //                 load Q and write O
 //
-// TMEM: S_a, S_b, O_a, O_b of 128 columns each.
+// TMEM: S_a, S_b, O_a, O_b of 128 columns each.  Heads of 256 have one query
+// tile to a CTA (O takes 256 columns), rings one deep and always the dense form.
 //
 // Within eight neighbouring head dimensions packed tiles hold them in the
 // order 0 4 1 5 2 6 3 7, which is how pairs fall out of a word of codes; queries
@@ -53,7 +54,6 @@ using attn::row_max;
 
 constexpr int kTileRows = 128;
 constexpr int kTcTile = 128;       // keys of a tile
-constexpr int kTcRows = 256;       // query rows of a CTA
 constexpr int kProducers = 3;      // warps 1 .. 3 of the packed form
 constexpr int kTmemCols = 512;
 constexpr float kTcFloor = -1.0e38f;
@@ -64,10 +64,16 @@ template <int D_, int G_> struct TcShape {
   static constexpr int HALVES = D / 64;
   static constexpr int HALF_BYTES = kTcTile * 128;           // 64 columns of 16 bits, 128-byte rows
   static constexpr int TILE_BYTES = HALF_BYTES * HALVES;
-  static constexpr int SMEM = 6 * TILE_BYTES + 1024 + 256;
+  static constexpr int QT = D <= 128 ? 2 : 1;                // query tiles of a CTA
+  static constexpr int ROWS = QT * kTileRows;
+  static constexpr int RING = D <= 128 ? 2 : 1;              // tiles of K, and of V, in flight
+  static constexpr int SMEM = (QT + 2 * RING) * TILE_BYTES + 1024 + 256;
+  // slot and phase of key tile j in the rings
+  static __device__ __forceinline__ int slot(int j) { return RING == 2 ? j & 1 : 0; }
+  static __device__ __forceinline__ uint32_t phase(int j) { return (RING == 2 ? j >> 1 : j) & 1; }
 };
 
-constexpr int tc_threads(bool dense) { return 32 * ((dense ? 2 : 1 + kProducers) + 8); }
+constexpr int tc_threads(bool dense, int tiles) { return 32 * ((dense ? 2 : 1 + kProducers) + 4 * tiles); }
 
 struct TcParams {
   Cache c;
@@ -123,7 +129,7 @@ __device__ __forceinline__ void store_shared16(uint32_t at, uint32_t a, uint32_t
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 template <typename S, bool BF16, bool DENSE>
-__global__ void __launch_bounds__(tc_threads(DENSE), 1)
+__global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
     attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const TcParams p) {
   constexpr int D = S::D, NG = S::NG;
@@ -131,10 +137,10 @@ __global__ void __launch_bounds__(tc_threads(DENSE), 1)
   using T = typename std::conditional<BF16, bf16, f16>::type;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;                          // [2] tiles
-  uint8_t* sK = smem + 2 * S::TILE_BYTES;      // [2]
-  uint8_t* sV = smem + 4 * S::TILE_BYTES;      // [2]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * S::TILE_BYTES);
+  uint8_t* sQ = smem;                                       // [QT] tiles
+  uint8_t* sK = smem + S::QT * S::TILE_BYTES;               // [RING]
+  uint8_t* sV = smem + (S::QT + S::RING) * S::TILE_BYTES;   // [RING]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (S::QT + 2 * S::RING) * S::TILE_BYTES);
   uint64_t* q_full = bars;        // [2]
   uint64_t* k_full = bars + 2;    // [2]
   uint64_t* k_empty = bars + 4;   // [2]
@@ -163,7 +169,7 @@ __global__ void __launch_bounds__(tc_threads(DENSE), 1)
   const int count = p.counts ? clamp_count(__ldg(p.counts + b), p.tokens) : p.tokens;
   const int length = clamp_count(__ldg(p.lengths + b), capacity(p.c.map));
   if (threadIdx.x == 0 && length != __ldg(p.lengths + b)) atomicExch(p.error_flag, PHEW_ERR_INVALID);
-  const int row0 = rb * kTcRows;
+  const int row0 = rb * S::ROWS;
   // key tiles that each query tile needs, and this CTA's share of them
   int need[2];
 #pragma unroll
@@ -171,7 +177,7 @@ __global__ void __launch_bounds__(tc_threads(DENSE), 1)
     const int first = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(row0 + t * kTileRows)));
     const int last = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(row0 + t * kTileRows + kTileRows - 1)));
     const int end = first >= count ? 0 : seen_end(length, count, last < count ? last : count - 1, p.causal);
-    need[t] = (end + kTcTile - 1) / kTcTile;
+    need[t] = t < S::QT ? (end + kTcTile - 1) / kTcTile : 0;
   }
   const int all = max(need[0], need[1]);
   const int j0 = static_cast<int>(static_cast<int64_t>(all) * split / p.splits);
@@ -240,10 +246,10 @@ __global__ void __launch_bounds__(tc_threads(DENSE), 1)
         if (ok) commit(&k_empty[0]);
       }
       for (int j = 0; j < n_max && ok; ++j) {
-        const int s = j & 1, s1 = (j + 1) & 1;
+        const int s = S::slot(j), s1 = S::slot(j + 1);
         const bool more = j + 1 < n_max;
-        if (!mbar_wait(&v_full[s], (j >> 1) & 1, wait_flag, p.wait_ns)) { ok = false; break; }
-        if (more && !mbar_wait(&k_full[s1], ((j + 1) >> 1) & 1, wait_flag, p.wait_ns)) { ok = false; break; }
+        if (!mbar_wait(&v_full[s], S::phase(j), wait_flag, p.wait_ns)) { ok = false; break; }
+        if (more && !mbar_wait(&k_full[s1], S::phase(j + 1), wait_flag, p.wait_ns)) { ok = false; break; }
         const uint32_t v_addr = smem_u32(sV + s * S::TILE_BYTES);
         const uint32_t k_addr = smem_u32(sK + s1 * S::TILE_BYTES);
 #pragma unroll
@@ -279,8 +285,8 @@ __global__ void __launch_bounds__(tc_threads(DENSE), 1)
         for (int i = 0; i < S::HALVES; ++i) tma_load_2d(dst + i * S::HALF_BYTES, tm, bar, i * 64, row);
       };
       for (int j = 0; j < n_max && ok; ++j) {
-        const int s = j & 1;
-        const uint32_t ph = ((j >> 1) & 1) ^ 1;
+        const int s = S::slot(j);
+        const uint32_t ph = S::phase(j) ^ 1;
         if (!mbar_wait(&k_empty[s], ph, wait_flag, p.wait_ns)) { ok = false; break; }
         load(&tm_k, &k_full[s], sK + s * S::TILE_BYTES, first + j * kTcTile);
         (s ? k_last[1] : k_last[0]) = j;
@@ -340,7 +346,7 @@ __global__ void __launch_bounds__(tc_threads(DENSE), 1)
       return x;
     };
     auto expand = [&](int u, Packed& x) {
-      const int j = u >> 3, side = (u >> 2) & 1, row = (u & 3) * 32 + lane, slot = j & 1;
+      const int j = u >> 3, side = (u >> 2) & 1, row = (u & 3) * 32 + lane, slot = S::slot(j);
       uint32_t sc[NG], bi[NG];  // each twice in a register
       bool fine = true;
 #pragma unroll
@@ -358,7 +364,7 @@ __global__ void __launch_bounds__(tc_threads(DENSE), 1)
       }
       uint64_t* full = side == 0 ? &k_full[slot] : &v_full[slot];
       uint64_t* empty = side == 0 ? &k_empty[slot] : &v_empty[slot];
-      if (lane == 0 && !mbar_wait(empty, ((j >> 1) & 1) ^ 1, wait_flag, p.wait_ns)) ok = false;
+      if (lane == 0 && !mbar_wait(empty, S::phase(j) ^ 1, wait_flag, p.wait_ns)) ok = false;
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) return;
       const uint32_t dst = smem_u32((side == 0 ? sK : sV) + slot * S::TILE_BYTES) + row * 128;
@@ -497,11 +503,11 @@ __global__ void __launch_bounds__(tc_threads(DENSE), 1)
       const bool split_up = p.splits > 1;
       const float inv = !live || l == 0.f ? 0.f : 1.f / l;
       const int64_t at = (static_cast<int64_t>(bh) * p.blocks + rb) * p.splits + split;
-      float* part = split_up ? p.part + (at * kTcRows + t * kTileRows + row) * D : nullptr;
+      float* part = split_up ? p.part + (at * S::ROWS + t * kTileRows + row) * D : nullptr;
       T* out = static_cast<T*>(p.o) + ((static_cast<int64_t>(b) * p.heads + head) * p.tokens + tok) * D;
       const bool mine = tok < p.tokens;
       if (split_up && mine) {
-        float* ml = p.part_ml + (at * kTcRows + t * kTileRows + row) * 2;
+        float* ml = p.part_ml + (at * S::ROWS + t * kTileRows + row) * 2;
         ml[0] = live ? m_ref : kTcFloor;
         ml[1] = live ? l : 0.f;
       }
@@ -550,8 +556,8 @@ __global__ void __launch_bounds__(tc_threads(DENSE), 1)
     } else if (DENSE && warp == 1 && lane == 0) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (k_last[i] >= 0) mbar_wait(&k_full[i], (k_last[i] >> 1) & 1, nullptr, p.wait_ns);
-        if (v_last[i] >= 0) mbar_wait(&v_full[i], (v_last[i] >> 1) & 1, nullptr, p.wait_ns);
+        if (k_last[i] >= 0) mbar_wait(&k_full[i], S::phase(k_last[i]), nullptr, p.wait_ns);
+        if (v_last[i] >= 0) mbar_wait(&v_full[i], S::phase(v_last[i]), nullptr, p.wait_ns);
       }
     }
     fence_before_sync();
@@ -564,28 +570,29 @@ __global__ void __launch_bounds__(tc_threads(DENSE), 1)
 }
 
 // Joins the splits of a row: one warp per row, splits in their order.
-template <int D, bool BF16>
+template <typename S, bool BF16>
 __global__ void __launch_bounds__(256) combine_tc_kernel(const TcParams p) {
+  constexpr int D = S::D, ROWS = S::ROWS;
   using T = typename std::conditional<BF16, bf16, f16>::type;
   constexpr int E = D / 32;
   const int lane = threadIdx.x & 31;
   const int64_t slot = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);  // (bh, block, row)
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int row = static_cast<int>(slot % kTcRows);
-  const int64_t seg = slot / kTcRows;
+  const int row = static_cast<int>(slot % ROWS);
+  const int64_t seg = slot / ROWS;
   const int rb = static_cast<int>(seg % p.blocks);
   const int bh = static_cast<int>(seg / p.blocks);
-  const int r = rb * kTcRows + row;
+  const int r = rb * ROWS + row;
   const int tok = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(r)));
   if (tok >= p.tokens) return;
   const int b = bh / p.c.map.kv_heads, head = (bh % p.c.map.kv_heads) * p.per + (r - tok * p.per);
   float m = kTcFloor;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[((seg * p.splits + s) * kTcRows + row) * 2]);
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[((seg * p.splits + s) * ROWS + row) * 2]);
   float o[E], l = 0.f;
 #pragma unroll
   for (int i = 0; i < E; ++i) o[i] = 0.f;
   for (int s = 0; s < p.splits; ++s) {
-    const int64_t at = (seg * p.splits + s) * kTcRows + row;
+    const int64_t at = (seg * p.splits + s) * ROWS + row;
     const float f = ex2(p.part_ml[at * 2] - m);
     l = fmaf(f, p.part_ml[at * 2 + 1], l);
 #pragma unroll
@@ -600,8 +607,14 @@ __global__ void __launch_bounds__(256) combine_tc_kernel(const TcParams p) {
 // CTAs of a call, how many ways each row block's keys are split (enough to give
 // every SM a CTA, two tiles of the longest possible sequence or more each), and
 // whether the cache is expanded first.
+// Query rows to a cache head from which the kernel is taken: below, the mma.sync kernel's passes of 8 or 16
+// rows over the cache cost less than a tile of 128 that is mostly empty.  Heads of 256 (always expanded: their
+// packed tiles would find no room for a second ring slot either) from 128 on.
+constexpr int64_t kTcMinRows = 64, kTcMinRowsWide = 128;
 constexpr int64_t kExpandBlocks = 3;               // row blocks from which one expansion beats one per CTA
 constexpr int64_t kExpandBytes = int64_t(1) << 30;  // scratch that a call may take for it
+
+int rows_of(int head_dim) { return head_dim <= 128 ? TcShape<128, 128>::ROWS : TcShape<256, 128>::ROWS; }
 
 struct TcPlan {
   int64_t blocks, splits, ctas;
@@ -610,17 +623,18 @@ struct TcPlan {
 };
 TcPlan tc_plan(int64_t batch, int kv_heads, int head_dim, int64_t q_rows, int64_t cap) {
   TcPlan t;
-  t.blocks = (q_rows + kTcRows - 1) / kTcRows;
+  const int rows = rows_of(head_dim);
+  t.blocks = (q_rows + rows - 1) / rows;
   const int64_t base = batch * kv_heads * t.blocks, sms = sm_count_current();
   const int64_t tiles = (cap + kTcTile - 1) / kTcTile;
   t.splits = base >= sms ? 1 : sms / base;
   if (t.splits > tiles / 2) t.splits = tiles / 2;
   if (t.splits < 1) t.splits = 1;
   t.ctas = base * t.splits;
-  t.part_bytes = t.splits == 1 ? 0 : static_cast<size_t>(t.ctas) * kTcRows * (static_cast<size_t>(head_dim) + 2) * 4;
+  t.part_bytes = t.splits == 1 ? 0 : static_cast<size_t>(t.ctas) * rows * (static_cast<size_t>(head_dim) + 2) * 4;
   t.rows = tiles * kTcTile;
   t.side_bytes = static_cast<size_t>(batch) * kv_heads * t.rows * head_dim * 2;
-  if (t.blocks < kExpandBlocks || static_cast<int64_t>(2 * t.side_bytes) > kExpandBytes ||
+  if ((t.blocks < kExpandBlocks && head_dim <= 128) || static_cast<int64_t>(2 * t.side_bytes) > kExpandBytes ||
       batch * kv_heads * t.rows >= kMaxRows) {
     t.rows = 0;
     t.side_bytes = 0;
@@ -649,7 +663,7 @@ int launch_tc(const Maps& m, const TcParams& p, unsigned grid, cudaStream_t st) 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(tc_threads(DENSE));
+  cfg.blockDim = dim3(tc_threads(DENSE, S::QT));
   cfg.dynamicSmemBytes = S::SMEM;
   cfg.stream = st;
   cfg.attrs = attr;
@@ -658,20 +672,22 @@ int launch_tc(const Maps& m, const TcParams& p, unsigned grid, cudaStream_t st) 
   if (int s = launch_status("kv attn_tc_kernel")) return s;
   if (p.splits == 1) return PHEW_OK;
   cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.batch) * p.c.map.kv_heads * p.blocks * (kTcRows / 8)));
+  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.batch) * p.c.map.kv_heads * p.blocks * (S::ROWS / 8)));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  PHEW_CHECK_CUDA(cudaLaunchKernelEx(&cfg, combine_tc_kernel<S::D, BF16>, p));
+  PHEW_CHECK_CUDA(cudaLaunchKernelEx(&cfg, combine_tc_kernel<S, BF16>, p));
   return launch_status("kv combine_tc_kernel");
 }
 
 template <bool BF16>
 int dispatch_tc(const Maps& m, const TcParams& p, unsigned grid, cudaStream_t st) {
-  if (p.rows)  // (the group no longer matters)
-    return p.c.head_dim == 64 ? launch_tc<TcShape<64, 64>, BF16, true>(m, p, grid, st)
-                              : launch_tc<TcShape<128, 128>, BF16, true>(m, p, grid, st);
+  if (p.rows) {  // (the group no longer matters)
+    if (p.c.head_dim == 64) return launch_tc<TcShape<64, 64>, BF16, true>(m, p, grid, st);
+    if (p.c.head_dim == 128) return launch_tc<TcShape<128, 128>, BF16, true>(m, p, grid, st);
+    return launch_tc<TcShape<256, 128>, BF16, true>(m, p, grid, st);
+  }
   if (p.c.head_dim == 64)
     return p.c.group == 32 ? launch_tc<TcShape<64, 32>, BF16, false>(m, p, grid, st)
                            : launch_tc<TcShape<64, 64>, BF16, false>(m, p, grid, st);
@@ -681,6 +697,12 @@ int dispatch_tc(const Maps& m, const TcParams& p, unsigned grid, cudaStream_t st
 }
 
 }  // namespace
+
+bool takes_tc(int64_t batch, int kv_heads, int head_dim, int dtype, int64_t rows, int64_t cap) {
+  if (dtype == PHEW_F32) return false;
+  if (head_dim <= 128) return rows >= kTcMinRows;
+  return rows >= kTcMinRowsWide && tc_plan(batch, kv_heads, head_dim, rows, cap).rows > 0;
+}
 
 size_t tc_bytes(int64_t batch, int kv_heads, int head_dim, int64_t rows, int64_t cap) {
   const TcPlan t = tc_plan(batch, kv_heads, head_dim, rows, cap);
@@ -728,7 +750,7 @@ int run_attn_tc(const AttnParams& a, bool bf16_type, void* workspace, cudaStream
     if (int s = expand(a.c, bf16_type, scratch, scratch + t.side_bytes, a.batch, t.rows, a.lengths, a.error_flag, st)) return s;
   }
   p.part = reinterpret_cast<float*>(scratch + 2 * t.side_bytes);
-  p.part_ml = p.part + static_cast<size_t>(t.ctas) * kTcRows * D;
+  p.part_ml = p.part + static_cast<size_t>(t.ctas) * rows_of(D) * D;
   p.error_flag = a.error_flag;
   const tc::TestStall stall = tc::take_test_stall();
   p.wait_ns = stall.wait_ns;

@@ -508,10 +508,11 @@ template <typename T, int BITS> void launch_fetch(const FetchParams& p, cudaStre
 
 template <typename T> int expand_typed(const FetchParams& p, cudaStream_t st) {
   const dim3 grid = grid_for(p.rows, p.c.head_dim);
-  if (p.c.head_dim == 64)
-    fetch_kernel<T, 4, 64, true><<<grid, kThreads, 0, st>>>(p);
-  else
-    fetch_kernel<T, 4, 128, true><<<grid, kThreads, 0, st>>>(p);
+  switch (p.c.head_dim) {
+    case 64: fetch_kernel<T, 4, 64, true><<<grid, kThreads, 0, st>>>(p); break;
+    case 128: fetch_kernel<T, 4, 128, true><<<grid, kThreads, 0, st>>>(p); break;
+    default: fetch_kernel<T, 4, 256, true><<<grid, kThreads, 0, st>>>(p); break;
+  }
   return launch_status("kv expand");
 }
 

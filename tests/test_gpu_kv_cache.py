@@ -273,6 +273,45 @@ def test_attention_chunks(mx, dtype, tokens, lengths, heads, kv_heads, causal):
     attend(mx, plan, rand((len(lengths), heads, tokens, 128), dtype, 6), causal=causal)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("head_dim,group", [(64, 32), (64, 64), (128, 32), (128, 128), (256, 32), (256, 128)])
+@pytest.mark.parametrize("tokens,heads", [(40, 4), (150, 4), (150, 12), (400, 8)])
+def test_attention_chunks_of_every_head(mx, dtype, head_dim, group, tokens, heads):
+    """Few row blocks (packed tiles) and many (the cache expanded first), padded batches, odd pages."""
+    lengths, counts = [900, tokens, 0, 131], [tokens, tokens, 3, 100 if tokens > 100 else 7]
+    plan = Plan(mx, lengths, kv_heads=2, head_dim=head_dim, group=group, dtype=dtype, page=24, seed=heads)
+    attend(mx, plan, rand((4, heads, tokens, head_dim), dtype, 7), counts, causal=True)
+
+
+def test_attention_chunk_with_a_wide_table(mx):
+    """A table for far more tokens than the sequence has: too much to expand, and many empty splits."""
+    plan = Plan(mx, [700], kv_heads=2, page=16)
+    wide = torch.full((1, 1 << 17), -5, dtype=torch.int32, device="cuda")
+    wide[:, : plan.table.shape[1]] = plan.table
+    plan.table = wide
+    attend(mx, plan, rand((1, 8, 300, 128), "bfloat16", 17), causal=True)
+    attend(mx, plan, rand((1, 8, 1, 128), "bfloat16", 18))
+
+
+@pytest.mark.parametrize("head_dim,tokens", [(128, 70), (128, 600), (256, 200)])
+@pytest.mark.parametrize("stage", [0, 1])
+def test_stalled_pipeline_is_reported(mx, head_dim, tokens, stage):
+    """A value tile that is never announced: the waits run out, the call reports it and the next one works."""
+    from phew_b200 import _native
+    from phew_b200.ops import check_device_errors
+
+    plan = Plan(mx, [700], kv_heads=2, head_dim=head_dim, dtype="bfloat16")
+    q = rand((1, 4, tokens, head_dim), "bfloat16", 19)
+    attend(mx, plan, q, causal=True)
+    mx.synchronize()
+    _native.call("phew_test_inject_stall", stage, 20_000_000)
+    mx.fast.quantized_cache_attention(mx.array(q), plan.cache, [700], block_table=mx.array(plan.table), mask="causal")
+    with pytest.raises(_native.PhewError, match="timed out"):
+        check_device_errors()
+    for _ in range(3):
+        attend(mx, plan, q, causal=True)
+
+
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("tokens", [1, 40])
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
