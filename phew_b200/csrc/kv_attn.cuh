@@ -22,14 +22,17 @@
 //    makes a pair of operands, `w & 0x000f000f` or `w & 0x00f000f0`, and one
 //    shift by eight brings the word's other half under the same masks: 5
 //    instructions for eight codes.  The 16 goes into the query (keys) or out of
-//    the sum (values), exactly.  (e4m3, which holds a nibble in a byte as it
+//    the sum (values), exactly.  (f16 values, and f32's keys and values, take
+//    n - 8 as normal numbers, one more instruction a pair: Shape says why.
+//    e4m3, which holds a nibble in a byte as it
 //    is, was tried: mma.sync on that type is expanded into conversions here,
 //    11 instructions each.)
 //  * queries and weights are f16 after a power of two: a row's largest query
 //    element goes to [2^14, 2^15); weights, at most 2^kGrow, times a value scale
 //    kept at most 2^7 by a power of two that follows the largest scale met.
 //    What falls below f16's range is then under 2^-38 of the largest.  f32
-//    queries and weights are two f16 terms (22 bits);
+//    queries and weights are two f16 terms (22 bits), and its sums leave the
+//    tensor core, which cuts what it adds off, every 16 keys;
 //  * a word's eight codes stay with the thread that loads it: the order of
 //    the head dimension inside a product is free, so queries are arranged to
 //    match and nothing is shuffled; weights move from the score fragment
@@ -59,6 +62,7 @@ constexpr int kTile = 32;       // keys of a tile: one warp's stage
 constexpr int kBegin = 2;       // tiles that the latencies of a segment's begin are worth
 constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;  // codes of a word as pairs of f16
 constexpr float kGrow = 8.0f;                   // log2 units a score may pass the running maximum by
+constexpr int kCentreTiles = 16;                // tiles of bare codes in one sum
 constexpr float kFloor = -1.0e38f;              // running maximum before the first key
 
 struct AttnParams {
@@ -111,9 +115,11 @@ template <typename T, int D_, int G_, int NT_> struct Shape {
   static constexpr bool F32 = sizeof(T) == 4;
   // f16 terms of a query and of a weight: one is exact for 16-bit queries and rounds a weight by 2^-12 of it
   static constexpr int TERMS = F32 ? 2 : 1;
-  // f16 results see that rounding: it is halved by weighing n - 8 instead of n, the 8 times the sum of the
-  // rounded weights (an accumulator of its own) subtracted at the end
-  static constexpr bool CENTRED = std::is_same<T, f16>::value;
+  // n - 8 instead of n in the second product: exact, and the rounded weights are then multiplied by half as
+  // much.  f16 results see that (3.0e-4 of their norm instead of 3.8e-4, attend_long 45 -> 48 us), bf16's do
+  // not.  f32 takes keys that way too: the tensor core lines a subnormal up as 2^-14 when it adds, so products
+  // of the bare digits lose their last bits (5e-6 of an output's norm instead of 4e-7).
+  static constexpr bool V_CENTRED = !std::is_same<T, bf16>::value;
   static constexpr int SB = NG * static_cast<int>(sizeof(T));   // bytes of a key's scales
   static constexpr int SROW = SB < 4 ? 4 : SB;
   static constexpr int CODE_BYTES = kTile * D / 2;         // one side's codes of a stage
@@ -177,6 +183,21 @@ __device__ __forceinline__ void mma_first(float* c, uint32_t a0, uint32_t a1, ui
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
                : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// A word's codes under a mask as pairs of f16, digits of a subnormal: n 2^-24 (odd codes 16 n 2^-24).  CENTRED:
+// n - 8 (16 (n - 8)), by way of 1024 + n.
+template <bool CENTRED> __device__ __forceinline__ uint32_t even_codes(uint32_t w) {
+  if constexpr (!CENTRED) return w & kEven;
+  uint32_t d;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"((w & kEven) | 0x64006400u), "r"(0x64086408u));
+  return d;
+}
+template <bool CENTRED> __device__ __forceinline__ uint32_t odd_codes(uint32_t w) {
+  if constexpr (!CENTRED) return w & kOdd;
+  uint32_t d;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"((w & kOdd) | 0x64006400u), "r"(0x64806480u));
+  return d;
 }
 
 // Two values rounded to f16 (lo in the low half); `rest`: what is left of them.
@@ -336,6 +357,7 @@ template <typename S, typename T> struct Ring {
 template <typename S, typename T>
 __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnParams p) {
   constexpr int D = S::D, G = S::G, NT = S::NT, NG = S::NG, ROWS = S::ROWS, TERMS = S::TERMS;
+  constexpr bool KC = S::F32, VC = S::V_CENTRED;  // key and value codes less 8 in the products
   constexpr int WPT = G / 32;   // words of a group that one thread multiplies with the queries
   constexpr int WT = D / 32;    // of a row
   extern __shared__ __align__(128) uint8_t smem[];
@@ -561,8 +583,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
       // a row's weights are 2^(score - m); m moves when a score passes it by `pass`, which is kGrow once the
       // row has seen a key and below any score before
       float m[NT][2], pass[NT][2], l[NT][2], bsum[NT][2][NG];
-      constexpr int SUM_TILES = (NG + 1) / 2;
-      float ones[NT][SUM_TILES][4];  // CENTRED: sums of the rounded weights, two groups to a tile
+      float wsum[NT][2][NG];  // of bf16: the weights behind `acc`
       float v_up = 0x1p60f;          // value scales are taken times this
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -571,16 +592,12 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
 #pragma unroll
           for (int k = 0; k < 4; ++k) acc[nt][i][k] = 0.f;
 #pragma unroll
-        for (int g = 0; g < SUM_TILES; ++g)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) ones[nt][g][k] = 0.f;
-#pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
           m[nt][cc] = 0.f;
           pass[nt][cc] = kFloor;
           l[nt][cc] = 0.f;
 #pragma unroll
-          for (int g = 0; g < NG; ++g) bsum[nt][cc][g] = 0.f;
+          for (int g = 0; g < NG; ++g) bsum[nt][cc][g] = wsum[nt][cc][g] = 0.f;
         }
       }
 
@@ -613,10 +630,12 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
                 for (int t = TERMS - 1; t >= 0; --t) {
                   const uint32_t* q = qf[nt][t][g * WPT + w];
                   if (w == 0 && t == TERMS - 1)
-                    mma_first(d[nt], wa[w] & kEven, wb[w] & kEven, wa[w] & kOdd, wb[w] & kOdd, q[0], q[1]);
+                    mma_first(d[nt], even_codes<KC>(wa[w]), even_codes<KC>(wb[w]), odd_codes<KC>(wa[w]), odd_codes<KC>(wb[w]),
+                              q[0], q[1]);
                   else
-                    mma(d[nt], wa[w] & kEven, wb[w] & kEven, wa[w] & kOdd, wb[w] & kOdd, q[0], q[1]);
-                  mma(d[nt], ya & kEven, yb & kEven, ya & kOdd, yb & kOdd, q[2], q[3]);
+                    mma(d[nt], even_codes<KC>(wa[w]), even_codes<KC>(wb[w]), odd_codes<KC>(wa[w]), odd_codes<KC>(wb[w]), q[0],
+                        q[1]);
+                  mma(d[nt], even_codes<KC>(ya), even_codes<KC>(yb), odd_codes<KC>(ya), odd_codes<KC>(yb), q[2], q[3]);
                 }
             }
 #pragma unroll
@@ -659,11 +678,9 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
               m[nt][cc] += by;
               l[nt][cc] *= alpha;
 #pragma unroll
-              for (int g = 0; g < NG; ++g) bsum[nt][cc][g] *= alpha;
-#pragma unroll
-              for (int g = 0; g < SUM_TILES; ++g) {
-                ones[nt][g][cc] *= alpha;
-                ones[nt][g][2 + cc] *= alpha;
+              for (int g = 0; g < NG; ++g) {
+                bsum[nt][cc][g] *= alpha;
+                wsum[nt][cc][g] *= alpha;
               }
 #pragma unroll
               for (int j = 0; j < D / 16; ++j) {
@@ -698,14 +715,15 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
 #pragma unroll
                 for (int k = 0; k < 4; ++k) acc[nt][i][k] *= f;
 #pragma unroll
-              for (int g = 0; g < SUM_TILES; ++g)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) ones[nt][g][k] *= f;
+              for (int g = 0; g < NG; ++g) {
+                wsum[nt][0][g] *= f;
+                wsum[nt][1][g] *= f;
+              }
             }
           }
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
-            if (S::CENTRED) zv[g] = fmaf(8.f, sv[g], zv[g]);
+            if (VC) zv[g] = fmaf(8.f, sv[g], zv[g]);
             sv[g] *= v_up;
           }
           __syncwarp();
@@ -736,6 +754,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
                   // a key that this row does not see may hold anything
                   const bool none = EDGE && w[cc] == 0.f;
                   f[cc] = none ? 0.f : w[cc] * sv[g];
+                  if (!VC) wsum[nt][cc][g] += f[cc];
                   bsum[nt][cc][g] = none ? bsum[nt][cc][g] : fmaf(w[cc], zv[g], bsum[nt][cc][g]);
                 }
 #pragma unroll
@@ -743,17 +762,20 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
               }
             }
           }
-          if constexpr (S::CENTRED) {
-            constexpr uint32_t one = 0x3c003c00u;
+          // outputs of fragment i, in group g: these 16 keys' weights times their codes
+          auto tile = [&](int i, int g, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
+              if constexpr (TERMS == 2) {
+                float d[4];
+                mma_first(d, a0, a1, a2, a3, pb[nt][g][1][0], pb[nt][g][1][1]);
+                mma(d, a0, a1, a2, a3, pb[nt][g][0][0], pb[nt][g][0][1]);
 #pragma unroll
-              for (int g = 0; g < NG; ++g)
-#pragma unroll
-                for (int t = TERMS - 1; t >= 0; --t)
-                  mma(ones[nt][g / 2], g & 1 ? 0u : one, g & 1 ? one : 0u, g & 1 ? 0u : one, g & 1 ? one : 0u,
-                      pb[nt][g][t][0], pb[nt][g][t][1]);
-          }
+                for (int k = 0; k < 4; ++k) acc[nt][i][k] += d[k];
+              } else {
+                mma(acc[nt][i], a0, a1, a2, a3, pb[nt][g][0][0], pb[nt][g][0][1]);
+              }
+          };
           const int vk = kb * 16 + t4;  // keys vk, + 4, + 8, + 12
           if constexpr (G >= 64) {
 #pragma unroll
@@ -765,17 +787,10 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
                 load_words<1>(v_at + (vk + 4 * k) * (D / 2) + swizzle<D>(vk + 4 * k, word >> 2) * 16 + (word & 3) * 4, &w[k]);
               const uint32_t x0 = __byte_perm(w[0], w[1], 0x5410), x1 = __byte_perm(w[0], w[1], 0x7632);
               const uint32_t y0 = __byte_perm(w[2], w[3], 0x5410), y1 = __byte_perm(w[2], w[3], 0x7632);
-              auto tile = [&](int u, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                  for (int t = TERMS - 1; t >= 0; --t)
-                    mma(acc[nt][j * 4 + u], a0, a1, a2, a3, pb[nt][g][t][0], pb[nt][g][t][1]);
-              };
-              tile(0, x0 & kEven, x1 & kEven, y0 & kEven, y1 & kEven);
-              tile(1, x0 & kOdd, x1 & kOdd, y0 & kOdd, y1 & kOdd);
-              tile(2, (x0 >> 8) & kEven, (x1 >> 8) & kEven, (y0 >> 8) & kEven, (y1 >> 8) & kEven);
-              tile(3, (x0 >> 8) & kOdd, (x1 >> 8) & kOdd, (y0 >> 8) & kOdd, (y1 >> 8) & kOdd);
+              tile(j * 4 + 0, g, even_codes<VC>(x0), even_codes<VC>(x1), even_codes<VC>(y0), even_codes<VC>(y1));
+              tile(j * 4 + 1, g, odd_codes<VC>(x0), odd_codes<VC>(x1), odd_codes<VC>(y0), odd_codes<VC>(y1));
+              tile(j * 4 + 2, g, even_codes<VC>(x0 >> 8), even_codes<VC>(x1 >> 8), even_codes<VC>(y0 >> 8), even_codes<VC>(y1 >> 8));
+              tile(j * 4 + 3, g, odd_codes<VC>(x0 >> 8), odd_codes<VC>(x1 >> 8), odd_codes<VC>(y0 >> 8), odd_codes<VC>(y1 >> 8));
             }
           } else {
             // groups of four words: a fragment's eight rows are the two halves of each
@@ -788,19 +803,36 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
               for (int k = 0; k < 4; ++k)
                 load_words<1>(v_at + (vk + 4 * k) * (D / 2) + swizzle<D>(vk + 4 * k, word >> 2) * 16 + (word & 3) * 4, &w[k]);
               const uint32_t x0 = __byte_perm(w[0], w[1], pick), y0 = __byte_perm(w[2], w[3], pick);
-              auto tile = [&](int u, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                  for (int t = TERMS - 1; t >= 0; --t)
-                    mma(acc[nt][g * 2 + u], a0, a1, a2, a3, pb[nt][g][t][0], pb[nt][g][t][1]);
-              };
               // (codes 0 and 2, then 1 and 3 of a half: both even or both odd)
-              tile(0, x0 & kEven, (x0 >> 8) & kEven, y0 & kEven, (y0 >> 8) & kEven);
-              tile(1, x0 & kOdd, (x0 >> 8) & kOdd, y0 & kOdd, (y0 >> 8) & kOdd);
+              tile(g * 2 + 0, g, even_codes<VC>(x0), even_codes<VC>(x0 >> 8), even_codes<VC>(y0), even_codes<VC>(y0 >> 8));
+              tile(g * 2 + 1, g, odd_codes<VC>(x0), odd_codes<VC>(x0 >> 8), odd_codes<VC>(y0), odd_codes<VC>(y0 >> 8));
             }
           }
         }
+      };
+
+      // Bare digits' sums grow with the keys, and the tensor core cuts off what it adds to them: 2^-24 of the
+      // sum a step, always towards zero, hundreds of times that of what a flat softmax leaves of it.  So 8 times
+      // the weights go over to the biases' side before a sum is kCentreTiles long.
+      auto centre = [&]() {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) {
+              float& w = wsum[nt][cc][g];
+              bsum[nt][cc][g] = fmaf(8.f / v_up, w, bsum[nt][cc][g]);
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+#pragma unroll
+              for (int i = g * G / 16; i < (g + 1) * G / 16; ++i) {
+                const float f = i & 1 ? -0x1p-17f : -0x1p-21f;
+                acc[nt][i][cc] = fmaf(f, w, acc[nt][i][cc]);
+                acc[nt][i][2 + cc] = fmaf(f, w, acc[nt][i][2 + cc]);
+              }
+              w = 0.f;
+            }
       };
 
       for (int key0 = t0 * kTile; key0 < t1 * kTile; key0 += kTile) {
@@ -814,8 +846,9 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
           ring.load(st_out, 0, key0 + lane < ent.end, sk, zk);
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
+            if (KC) zk[g] = fmaf(8.f, sk[g], zk[g]);
             // (an infinite key would give scores of either infinity: no number, as its products are)
-            sk[g] = fmaf(sk[g], 0x1p24f, fmaf(0.f, sk[g], 0.f * zk[g]));
+            sk[g] = fmaf(sk[g], KC ? 1.f : 0x1p24f, fmaf(0.f, sk[g], 0.f * zk[g]));
           }
           ring.share(sk, zk);
         }
@@ -825,6 +858,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
         else
           stage(st_out, key0, std::false_type());
         st_out = st_out + 1 == S::STAGES ? 0 : st_out + 1;
+        if (!VC && (key0 / kTile - t0) % kCentreTiles == kCentreTiles - 1) centre();
       }
 
       // ---- the segment's result, or this warp's part of it ----
@@ -877,15 +911,12 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
               }
             }
           };
-          // what a sum counts: n is n 2^-24 in it, odd codes sixteenfold, value scales times v_up
-          const float even = 0x1p24f / v_up, odd = 0x1p20f / v_up;
-          auto moved = [&](int g) {  // what a group's outputs still lack
-            return S::CENTRED ? fmaf(-8.f / v_up, ones[nt][g / 2][(g & 1) * 2 + cc], bsum[nt][cc][g]) : bsum[nt][cc][g];
-          };
+          // what a sum counts: codes 2^-24 in it, odd ones sixteenfold, value scales times v_up
+          const float even = (VC ? 1.f : 0x1p24f) / v_up, odd = even * 0x1p-4f;
           if constexpr (G >= 64) {
 #pragma unroll
             for (int j = 0; j < D / 64; ++j) {
-              const float z = moved(j * 64 / G);
+              const float z = bsum[nt][cc][j * 64 / G];
               float v[8];
 #pragma unroll
               for (int u = 0; u < 4; ++u) {
@@ -897,7 +928,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
           } else {
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-              const float z = moved(g);
+              const float z = bsum[nt][cc][g];
               const float v[4] = {fmaf(acc[nt][g * 2][cc], even, z), fmaf(acc[nt][g * 2 + 1][cc], odd, z),
                                   fmaf(acc[nt][g * 2][2 + cc], even, z), fmaf(acc[nt][g * 2 + 1][2 + cc], odd, z)};
               put((g * 4 + (r8 & 3)) * 8 + (r8 & 4), v, std::integral_constant<int, 4>());

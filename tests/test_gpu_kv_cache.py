@@ -372,6 +372,51 @@ def test_attention_one_long_sequence(mx):
     attend(mx, plan, rand((1, 8, 1, 128), "float16", 12))
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("head_dim,group", [(128, 64), (64, 32), (256, 128)])
+def test_attention_flat_sums(mx, dtype, head_dim, group):
+    """Nearly equal weights over 40000 keys, where sums of codes are hundreds of times what is left of them.
+
+    Norm of the error over the norm of the outputs, which are N keys' mean, sigma / sqrt(N) in size; every error
+    below is independent of the values it meets and of its neighbours, so norms add in squares:
+      * output rounded once, and 16-bit types' weights rounded before their product: a uniform error of at most
+        u, root mean square u / sqrt(3) of a value at the start of its binade: at most sqrt(2 / 3) u together
+      * weights' exponentials: below 2^-20 of each
+      * 32-bit sums: 64 sequences of 2 heads over 1250 tiles of 32 keys leave a warp about 100 tiles, 200
+        additions to an output, each off by at most 2^-24 of the running sum.  That sum holds what the centring
+        leaves, half a code step (4 sigma / 15 / 2 = 0.13 sigma) times its 3200 keys at most, where the outputs
+        hold sigma sqrt(3200): sqrt(200) 2^-24 0.13 sqrt(3200) = 2^-17.4, and the biases' sums the same again."""
+    n, u = 40000, UNIT[dtype]
+    plan = Plan(mx, [n], kv_heads=2, head_dim=head_dim, group=group, page=64, dtype=dtype, seed=3)
+    B = 64
+    q = rand((B, 2, 1, head_dim), dtype, 4, 0.05)
+    scale = head_dim ** -0.5
+    o = mx.fast.quantized_cache_attention(mx.array(q), plan.cache, mx.array(ints([n] * B)),
+                                          block_table=mx.array(plan.table.expand(B, -1)), scale=scale)._t.double()
+    for h in range(2):
+        p = torch.softmax(q[:, h, 0].double() @ plan.values(0, 0)[h].T * scale, -1)
+        want = p @ plan.values(1, 0)[h]
+        worst = float(((o[:, h, 0] - want).norm(dim=-1) / want.norm(dim=-1)).max())
+        assert worst <= u + 2.0 ** -20 + 2 * 2.0 ** -17.4, f"{worst:.3g}"
+
+
+def test_attention_flat_sums_of_a_long_share(mx):
+    """As above where a warp takes 1180 tiles of 32 keys (512 sequences of 131072 on the same pages), and bf16's
+    sums hold the codes themselves: 16 tiles of them at a time, 32 steps that each lose at most 2^-24 of the sum so
+    far on average, always downwards.  That is 7.5 steps times the keys, 1.63 sigma times them, where the outputs
+    hold sigma sqrt(131072) = 362 sigma: 32 2^-24 1.63 362 = 2^-9.8."""
+    n, B = 131072, 512
+    plan = Plan(mx, [n], kv_heads=1, page=256, seed=5)
+    q = rand((B, 1, 1, 128), "bfloat16", 6, 0.05)
+    o = mx.fast.quantized_cache_attention(mx.array(q), plan.cache, mx.array(ints([n] * B)),
+                                          block_table=mx.array(plan.table.expand(B, -1)), scale=128 ** -0.5)._t
+    rows = slice(0, B, 64)
+    p = torch.softmax(q[rows, 0, 0].double() @ plan.values(0, 0)[0].T * 128 ** -0.5, -1)
+    want = p @ plan.values(1, 0)[0]
+    worst = float(((o[rows, 0, 0].double() - want).norm(dim=-1) / want.norm(dim=-1)).max())
+    assert worst <= UNIT["bfloat16"] + 2.0 ** -20 + 2.0 ** -9.8, f"{worst:.3g}"
+
+
 def test_attention_reads_strided_queries(mx):
     plan = Plan(mx, [90, 14], kv_heads=2)
     x = rand((2, 5, 3, 4, 128), "bfloat16", 13)
