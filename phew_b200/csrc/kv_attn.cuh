@@ -28,8 +28,8 @@
 //    is, was tried: mma.sync on that type is expanded into conversions here,
 //    11 instructions each.)
 //  * queries and weights are f16 after a power of two: a row's largest query
-//    element goes to [2^14, 2^15); weights, at most 2^kGrow, times a value scale
-//    kept at most 2^7 by a power of two that follows the largest scale met.
+//    element goes to [2^14, 2^15); weights, at most 1, times a value scale kept
+//    at most 2^15 by a power of two that follows the largest scale met.
 //    What falls below f16's range is then under 2^-38 of the largest.  f32
 //    queries and weights are two f16 terms (22 bits), and its sums leave the
 //    tensor core, which cuts what it adds off, every 16 keys;
@@ -61,7 +61,7 @@ constexpr int kWarps = 4;       // of a block; they share nothing
 constexpr int kTile = 32;       // keys of a tile: one warp's stage
 constexpr int kBegin = 2;       // tiles that the latencies of a segment's begin are worth
 constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;  // codes of a word as pairs of f16
-constexpr float kGrow = 8.0f;                   // log2 units a score may pass the running maximum by
+constexpr float kGrow = 8.0f;                   // log2 units that a row's scores may grow by before its sums are scaled
 constexpr int kCentreTiles = 16;                // tiles of bare codes in one sum
 constexpr float kFloor = -1.0e38f;              // running maximum before the first key
 
@@ -580,11 +580,11 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
       for (int o = 1; o < 4; o <<= 1) lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, o));
 
       float acc[NT][D / 16][4];
-      // a row's weights are 2^(score - m); m moves when a score passes it by `pass`, which is kGrow once the
-      // row has seen a key and below any score before
+      // a row's weights are 2^(score - m), m kGrow above its largest score when it last moved; it moves when a
+      // score passes it by `pass`, which is 0 once the row has seen a key and below any score before
       float m[NT][2], pass[NT][2], l[NT][2], bsum[NT][2][NG];
       float wsum[NT][2][NG];  // of bf16: the weights behind `acc`
-      float v_up = 0x1p60f;          // value scales are taken times this
+      float v_up = 0x1p68f;          // value scales are taken times this
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -650,7 +650,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
                 }
           }
         }
-        // ---- running maximum: moved only when a score passes it by kGrow, so weights stay below 2^kGrow ----
+        // ---- m: moved only when a score passes it; weights stay below 1 ----
         bool grow = false;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -672,9 +672,9 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
 #pragma unroll
               for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
               const bool move = top > pass[nt][cc];
-              const float by = move ? top : 0.f;
+              const float by = move ? top + kGrow : 0.f;
               const float alpha = exp2_fast(fminf(-by, 0.f));  // (a row's first keys find nothing to scale)
-              if (move) pass[nt][cc] = kGrow;
+              if (move) pass[nt][cc] = 0.f;
               m[nt][cc] += by;
               l[nt][cc] *= alpha;
 #pragma unroll
@@ -694,18 +694,18 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
               }
             }
         }
-        // ---- value scales, at most 2^7 times a power of two that only shrinks ----
+        // ---- value scales, at most 2^15 times a power of two that only shrinks ----
         {
           float sv[NG], zv[NG];
           ring.load(st, 1, !EDGE || key0 + lane < ent.end, sv, zv);
           float top = 0.f;
 #pragma unroll
           for (int g = 0; g < NG; ++g) top = fmaxf(top, fabsf(sv[g]));
-          if (__any_sync(0xffffffffu, top * v_up > 128.f && top < INFINITY)) {
+          if (__any_sync(0xffffffffu, top * v_up > 32768.f && top < INFINITY)) {
             if (!(top < INFINITY)) top = 0.f;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float to = __uint_as_float(min(260u - (__float_as_uint(top) >> 23), 187u) << 23);  // top to [64, 128)
+            const float to = __uint_as_float(min(268u - (__float_as_uint(top) >> 23), 195u) << 23);  // top to [2^14, 2^15)
             const float f = to / v_up;
             v_up = to;
 #pragma unroll
@@ -912,7 +912,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
             }
           };
           // what a sum counts: codes 2^-24 in it, odd ones sixteenfold, value scales times v_up
-          const float even = (VC ? 1.f : 0x1p24f) / v_up, odd = even * 0x1p-4f;
+          const float even = VC ? 1.f : 0x1p24f, odd = even * 0x1p-4f, down = 1.f / v_up;
           if constexpr (G >= 64) {
 #pragma unroll
             for (int j = 0; j < D / 64; ++j) {
@@ -920,8 +920,8 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
               float v[8];
 #pragma unroll
               for (int u = 0; u < 4; ++u) {
-                v[u] = fmaf(acc[nt][j * 4 + u][cc], u & 1 ? odd : even, z);
-                v[u + 4] = fmaf(acc[nt][j * 4 + u][2 + cc], u & 1 ? odd : even, z);
+                v[u] = fmaf(acc[nt][j * 4 + u][cc] * (u & 1 ? odd : even), down, z);
+                v[u + 4] = fmaf(acc[nt][j * 4 + u][2 + cc] * (u & 1 ? odd : even), down, z);
               }
               put((j * 8 + r8) * 8, v, std::integral_constant<int, 8>());
             }
@@ -929,8 +929,8 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
               const float z = bsum[nt][cc][g];
-              const float v[4] = {fmaf(acc[nt][g * 2][cc], even, z), fmaf(acc[nt][g * 2 + 1][cc], odd, z),
-                                  fmaf(acc[nt][g * 2][2 + cc], even, z), fmaf(acc[nt][g * 2 + 1][2 + cc], odd, z)};
+              const float v[4] = {fmaf(acc[nt][g * 2][cc] * even, down, z), fmaf(acc[nt][g * 2 + 1][cc] * odd, down, z),
+                                  fmaf(acc[nt][g * 2][2 + cc] * even, down, z), fmaf(acc[nt][g * 2 + 1][2 + cc] * odd, down, z)};
               put((g * 4 + (r8 & 3)) * 8 + (r8 & 4), v, std::integral_constant<int, 4>());
             }
           }

@@ -348,13 +348,15 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
     auto expand = [&](int u, Packed& x) {
       const int j = u >> 3, side = (u >> 2) & 1, row = (u & 3) * 32 + lane, slot = S::slot(j);
       uint32_t sc[NG], bi[NG];  // each twice in a register
-      bool fine = true;
+      bool fine = true, past = false;  // parts finite; values past the type's range (held at its end)
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         sc[g] = __byte_perm(x.sb[0][g / 2], 0, g & 1 ? 0x3232 : 0x1010);
         bi[g] = __byte_perm(x.sb[1][g / 2], 0, g & 1 ? 0x3232 : 0x1010);
         fine = fine && finite16(sc[g], BF16) && finite16(bi[g], BF16);
+        past = past || !finite16(fma_pair<BF16>(sc[g], BF16 ? 0x41704170u : 0x4b804b80u, bi[g]), BF16);  // code 15
       }
+      past = past && fine;
       if (side == 1 && !fine) {
         // a weight of zero times infinity is no number, and a later query's keys may not touch an earlier
         // one: the values count as zero here and as "no number" for every row that sees the key
@@ -368,17 +370,21 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) return;
       const uint32_t dst = smem_u32((side == 0 ? sK : sV) + slot * S::TILE_BYTES) + row * 128;
+      const bool any_past = __any_sync(0xffffffffu, past);
 #pragma unroll
       for (int ch = 0; ch < D / 32; ++ch) {
         const uint32_t word[4] = {x.code[ch].x, x.code[ch].y, x.code[ch].z, x.code[ch].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int g = (ch * 32 + i * 8) / S::G, c16 = ch * 4 + i;
-          store_shared16(dst + (c16 >> 3) * S::HALF_BYTES + (((c16 & 7) ^ (row & 7)) << 4),
-                         fma_pair<BF16>(sc[g], code_pair<BF16, 0>(word[i]), bi[g]),
-                         fma_pair<BF16>(sc[g], code_pair<BF16, 1>(word[i]), bi[g]),
-                         fma_pair<BF16>(sc[g], code_pair<BF16, 2>(word[i]), bi[g]),
-                         fma_pair<BF16>(sc[g], code_pair<BF16, 3>(word[i]), bi[g]));
+          uint32_t v[4] = {fma_pair<BF16>(sc[g], code_pair<BF16, 0>(word[i]), bi[g]),
+                           fma_pair<BF16>(sc[g], code_pair<BF16, 1>(word[i]), bi[g]),
+                           fma_pair<BF16>(sc[g], code_pair<BF16, 2>(word[i]), bi[g]),
+                           fma_pair<BF16>(sc[g], code_pair<BF16, 3>(word[i]), bi[g])};
+          if (any_past)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = past ? hold_pair<BF16>(v[k]) : v[k];
+          store_shared16(dst + (c16 >> 3) * S::HALF_BYTES + (((c16 & 7) ^ (row & 7)) << 4), v[0], v[1], v[2], v[3]);
         }
       }
       fence_async_shared();

@@ -463,6 +463,12 @@ __global__ void __launch_bounds__(kThreads) fetch_kernel(const FetchParams p) {
           set_pair(out, i, fma2(two(s, s), n, two(z, z)));
         }
       }
+      if constexpr (EXPAND) {
+        // scale * code + bias of finite parts may pass the type's largest value: held there
+        const bool held = at[u] != kNoRow && fabsf(to_f32(sc[u][half])) < INFINITY && fabsf(to_f32(bi[u][half])) < INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out.w[i] = held ? hold_pair<std::is_same<T, bf16>::value>(out.w[i]) : out.w[i];
+      }
       store8(dst + half * (D / 2), out);
     }
   }

@@ -136,6 +136,12 @@ def _as_ints(x) -> torch.Tensor:
     return core.array(x, None if isinstance(x, torch.Tensor) else core.int32)._t
 
 
+def _copied(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous copy, made on the tensor's device."""
+    with torch.cuda.device(t.device):
+        return core.contiguous_copy(core.array._wrap(t))._t
+
+
 def _ints(x, batch: int, what: str, cache: QuantizedKVCache) -> torch.Tensor:
     """An int32 [batch] array on the cache's device."""
     t = _as_ints(x)
@@ -145,7 +151,7 @@ def _ints(x, batch: int, what: str, cache: QuantizedKVCache) -> torch.Tensor:
         raise ValueError(f"{what} shape {tuple(t.shape)} != {(batch,)}")
     if t.device != cache.device:
         raise ValueError(f"{what} lies on another device than the cache")
-    return t if t.is_contiguous() else core.contiguous_copy(core.array._wrap(t))._t
+    return t if t.is_contiguous() else _copied(t)
 
 
 def _table(block_table, batch: int, what: str, cache: QuantizedKVCache):
@@ -164,7 +170,7 @@ def _table(block_table, batch: int, what: str, cache: QuantizedKVCache):
         raise ValueError(f"{what}: block_table lies on another device than the cache")
     stride, unit = t.stride()
     if unit != 1 and t.shape[1] > 1:
-        t = core.contiguous_copy(core.array._wrap(t))._t
+        t = _copied(t)
         stride = t.shape[1]
     return t, t.data_ptr(), stride, t.shape[1]
 
@@ -189,7 +195,7 @@ def _rows(x, what: str, cache: QuantizedKVCache):
         raise ValueError(f"{what} lies on another device than the cache")
     b, h, n, unit = t.stride()
     if unit != 1 or (b | h | n) % cache._unit or t.data_ptr() % 16:
-        t = core.contiguous_copy(core.array._wrap(t))._t
+        t = _copied(t)
         b, h, n, unit = t.stride()
     return t, _strides(n, h, b)
 

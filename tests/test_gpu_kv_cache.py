@@ -427,6 +427,57 @@ def test_attention_reads_strided_queries(mx):
     assert torch.equal(same, attend(mx, plan, odd, causal=True))
 
 
+@pytest.mark.parametrize("tokens", [100, 200])  # packed, expanded
+def test_attention_chunk_reads_strided_queries(mx, tokens):
+    plan = Plan(mx, [300, tokens], kv_heads=2)
+    x = rand((2, tokens, 3, 8, 128), "bfloat16", 14)
+    q = x[:, :, 1].transpose(1, 2)
+    same = attend(mx, plan, q, causal=True)
+    assert torch.equal(same, attend(mx, plan, q.contiguous(), causal=True))
+    one = q[:1, :1].expand(2, 8, tokens, 128)  # broadcast over sequences and heads
+    assert torch.equal(attend(mx, plan, one, causal=True), attend(mx, plan, one.contiguous(), causal=True))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("tokens", [2, 100, 200])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_attention_queries_that_are_no_numbers(mx, dtype, tokens, bad):
+    """An odd query's row is no number; its neighbours do not notice."""
+    plan = Plan(mx, [300, 40], kv_heads=2, dtype=dtype)
+    q = rand((2, 8, tokens, 128), dtype, 15)
+    want = attend(mx, plan, q)
+    q[1, 2, 1, 77] = bad
+    got = mx.fast.quantized_cache_attention(mx.array(q), plan.cache, mx.array(ints(plan.lengths)), block_table=mx.array(
+        plan.table), scale=128 ** -0.5)._t
+    assert not torch.isfinite(got[1, 2, 1]).any()
+    got[1, 2, 1] = want[1, 2, 1]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("tokens", [3, 100, 200])
+def test_attention_values_at_the_end_of_the_range(mx, dtype, tokens):
+    """Groups from -top to top: code 15 of such a scale rounds past the type's range in f16 (65536), and the rows
+    that do not see that key must not meet an infinity.  (bf16's range is as large as that of 32-bit sums: a
+    quarter of it.)"""
+    plan = Plan(mx, [tokens + 60], kv_heads=1, dtype=dtype, spare=0)
+    last = tokens + 59
+    page, row = int(plan.table[0, last // plan.page]), last % plan.page
+    top = torch.finfo(DTYPES[dtype]).max * (0.25 if dtype == "bfloat16" else 1.0)
+    plan.dense[1][page, 0, row] = torch.tensor([-top, top], dtype=DTYPES[dtype], device="cuda").repeat(64)
+    sides = [mx.quantize(mx.array(x), group_size=64, bits=4) for x in plan.dense]
+    plan.cache = mx.fast.QuantizedKVCache(*sides, group_size=64, bits=4)
+    v = plan.values(1, 0)[0, -1]
+    assert float(v.max()) >= top  # (65536 > 65504 in f16)
+    q = rand((1, 8, tokens, 128), dtype, 16)
+    o = mx.fast.quantized_cache_attention(mx.array(q), plan.cache, mx.array(ints([tokens + 60])),
+                                          block_table=mx.array(plan.table), scale=128 ** -0.5, mask="causal")._t
+    want, tol = attend64(plan, q, None, 128 ** -0.5, True)
+    check(o[:, :, -1], want[:, :, -1], tol[:, :, -1])
+    plan.lengths = [tokens + 59]  # the bound of the other rows is that of the keys that they see
+    check(o[:, :, :-1], *attend64(plan, q[:, :, :-1], None, 128 ** -0.5, True))
+
+
 def test_attention_far_rows(mx):
     """A cache of more than 2^32 bytes of codes: rows near its end."""
     pages, page = 1100, 16384  # 18 M rows of 2 heads x 128 bytes: 4.6 GB a side
