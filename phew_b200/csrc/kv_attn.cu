@@ -38,6 +38,10 @@ extern "C" int phew_kv_attention(const phew_kv_cache* cache, const void* q, cons
   PHEW_REQUIRE(heads > 0 && heads % cache->kv_heads == 0 && heads < (1ll << 31),
                "phew_kv_attention: heads must be a multiple of the cache's kv_heads");
   PHEW_REQUIRE(heads / cache->kv_heads < ((1ll << 31) - (1 << 16)) / tokens, "phew_kv_attention: too many query rows");
+  // (the kernels count keys a few tiles past the last one, and a sequence's tiles over its heads, in 32 bits)
+  const int64_t cap = kv::capacity(p.c.map);
+  PHEW_REQUIRE(cap <= (1ll << 31) - 1024 && (cap / kv::kTile + 1 + kv::kBegin) * cache->kv_heads < (1ll << 32),
+               "phew_kv_attention: a sequence's pages hold too many tokens");
   PHEW_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o)) & 15) == 0,
                "phew_kv_attention: pointers must be 16-byte aligned");
   for (int i = 0; i < 3; ++i)
@@ -64,7 +68,7 @@ extern "C" int phew_kv_attention(const phew_kv_cache* cache, const void* q, cons
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // (the tcgen05 kernel takes its maxima over unscaled scores)
   if (p.scale_log2 > 0.f && kv::takes_tc(batch, cache->kv_heads, cache->head_dim, cache->dtype,
-                                         static_cast<int64_t>(p.tokens) * p.per, kv::capacity(p.c.map)))
+                                         static_cast<int64_t>(p.tokens) * p.per, cap))
     return kv::run_attn_tc(p, cache->dtype == PHEW_BF16, workspace, st);
   switch (cache->dtype) {
     case PHEW_F32: return kv::run_attn<float>(p, workspace, st);

@@ -154,3 +154,7 @@ def test_entry_points_refuse_bad_arguments(lib):
     refused(attend(c, 3, 1, ok, big), "multiple of the cache's kv_heads")
     refused(attend(c, 4, 0, ok, big), "token count")
     refused(attend(c, 4, 1, odd, big), "strides")
+    wide = lambda cc, heads, columns: lib.phew_kv_attention(  # noqa: E731
+        cc, FAKE, ok, FAKE, 2, heads, 1, FAKE, None, FAKE, columns, columns, 1.0, 0, FAKE, big, FAKE, None)
+    refused(wide(cache(page_size=16), 4, (1 << 27) - 1), "too many tokens")  # 2^31 - 16
+    refused(wide(cache(page_size=16, kv_heads=128), 128, (1 << 27) - 64), "too many tokens")  # 2^26 tiles of 128 heads
