@@ -47,6 +47,12 @@
 // any mix of lengths loads the SMs evenly and no host ever needs the lengths.
 // A segment that lies in one warp is finished there; a cut one leaves partial
 // sums (maximum, sum, output) that the combine kernel joins in a fixed order.
+//
+// Measured: 64 sequences of up to 8192 keys, 32 heads of 128 over 8, bf16:
+// 80 us, 3.8 TB/s of the bytes that must be read (0.59 of a copy).  Three warps
+// to a scheduler (168 registers) issue every other cycle: 613 instructions to
+// a tile, waits on one another's results between them.  Four (128 registers)
+// spill, or read the queries from shared memory, for the same time.
 #pragma once
 
 #include <atomic>
@@ -59,7 +65,9 @@ namespace kv {
 
 constexpr int kWarps = 4;       // of a block; they share nothing
 constexpr int kTile = 32;       // keys of a tile: one warp's stage
-constexpr int kBegin = 2;       // tiles that the latencies of a segment's begin are worth
+// Tiles that the latencies of a segment's begin are worth (1, 2, 4: 41.6, 37.5, 39.9 us for 256 x 8 segments of 300
+// keys; no difference for 128 of 8192)
+constexpr int kBegin = 2;
 constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;  // codes of a word as pairs of f16
 constexpr float kGrow = 8.0f;                   // log2 units that a row's scores may grow by before its sums are scaled
 constexpr int kCentreTiles = 16;                // tiles of bare codes in one sum
@@ -1083,7 +1091,9 @@ template <typename S, typename T> int launch_attn(AttnParams p, void* workspace,
 }
 
 // Row tiles of eight to a block: two for more than eight query rows, where registers allow it (16-bit
-// types with heads up to 128; wider heads and the three terms of f32 would spill the second tile).
+// types with heads up to 128; wider heads and the two terms of f32 would spill the second tile).  Two against one,
+// 8 cache heads of 8192 keys / 16 x 8 of 2048 / 8 of 65536: 12 rows 16 : 16, 26 : 29, 36 : 44 us, 32 rows 17 : 20,
+// 37 : 44, 57 : 75.
 template <typename T> int row_tiles(int head_dim, int64_t rows) {
   return sizeof(T) == 2 && head_dim <= 128 && rows > 8 ? 2 : 1;
 }

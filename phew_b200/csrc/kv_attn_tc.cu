@@ -37,6 +37,15 @@
 // Long caches with few rows are split: a CTA takes a share of the key tiles
 // and leaves partial sums, joined in a fixed order by the combine kernel.
 //
+// Keys and values are rounded to the type, as mx.dequantize gives them, and so
+// are the softmax weights, as in the dense attention: what the tensor core
+// takes.  Together 3.2e-3 to 3.7e-3 of an output's norm in bf16 (1.7e-3 is its
+// own rounding), 4e-4 in f16 (2.1e-4).  Scores, maxima and sums are 32-bit.
+//
+// Measured, causal, heads of 128 in bf16: two prompts of 4096 tokens on 32
+// heads, 334 us (823 TFLOP/s); the last 2048 of 8192 tokens on 32 heads over 8,
+// 248 us (970 TFLOP/s).
+//
 // Every wait is bounded; one that runs out sets error_flag[1] and the CTA
 // winds down with its TMEM freed.
 #include "attn_softmax.cuh"
@@ -613,11 +622,16 @@ __global__ void __launch_bounds__(256) combine_tc_kernel(const TcParams p) {
 // CTAs of a call, how many ways each row block's keys are split (enough to give
 // every SM a CTA, two tiles of the longest possible sequence or more each), and
 // whether the cache is expanded first.
-// Query rows to a cache head from which the kernel is taken: below, the mma.sync kernel's passes of 8 or 16
-// rows over the cache cost less than a tile of 128 that is mostly empty.  Heads of 256 (always expanded: their
-// packed tiles would find no room for a second ring slot either) from 128 on.
-constexpr int64_t kTcMinRows = 64, kTcMinRowsWide = 128;
-constexpr int64_t kExpandBlocks = 3;               // row blocks from which one expansion beats one per CTA
+// Query rows to a cache head above which the kernel is taken: up to there the mma.sync kernel's passes of 16 rows
+// (8 of heads of 256) over the cache cost less than a tile of 128 that is mostly empty.  Measured, mma.sync against
+// this kernel, 8 cache heads of 8192 keys / 16 x 8 of 2048 / 8 of 65536: at 48 rows 22 : 31, 49 : 57, 81 : 106 us,
+// at 64 rows 24 : 31, 61 : 57, 103 : 106, at 96 rows 30 : 32, 84 : 57, 146 : 107.  Heads of 256, 8 of 8192 keys /
+// 8 x 8 of 2048: at 64 rows 44 : 55, 77 : 82, at 96 rows 58 : 56, 105 : 84.
+constexpr int64_t kTcAbove = 64;
+// Row blocks from which one expansion beats one per CTA.  Expanded against packed, the same three caches: 2 blocks
+// 44 : 45, 126 : 123, 216 : 209 us, 3 blocks 50 : 56, 162 : 180, 274 : 306, 4 blocks 59 : 69, 198 : 234, 357 : 428.
+// Heads of 256 are always expanded.
+constexpr int64_t kExpandBlocks = 3;
 constexpr int64_t kExpandBytes = int64_t(1) << 30;  // scratch that a call may take for it
 
 int rows_of(int head_dim) { return head_dim <= 128 ? TcShape<128, 128>::ROWS : TcShape<256, 128>::ROWS; }
@@ -706,8 +720,7 @@ int dispatch_tc(const Maps& m, const TcParams& p, unsigned grid, cudaStream_t st
 
 bool takes_tc(int64_t batch, int kv_heads, int head_dim, int dtype, int64_t rows, int64_t cap) {
   if (dtype == PHEW_F32) return false;
-  if (head_dim <= 128) return rows >= kTcMinRows;
-  return rows >= kTcMinRowsWide && tc_plan(batch, kv_heads, head_dim, rows, cap).rows > 0;
+  return rows > kTcAbove && (head_dim <= 128 || tc_plan(batch, kv_heads, head_dim, rows, cap).rows > 0);
 }
 
 size_t tc_bytes(int64_t batch, int kv_heads, int head_dim, int64_t rows, int64_t cap) {
