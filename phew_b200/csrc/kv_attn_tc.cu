@@ -19,6 +19,14 @@
 // from the softmax, which is why the dense form exists; more producer warps
 // (7 for 3) did not help.
 //
+// A pair of tiles takes 3600 clocks: each query tile's chain of 1750 in the
+// softmax (1024 of them the exponentials), 360 until its warps are heard, 1560
+// in its two products; the tensor core, which serves both tiles, is busy for
+// 2100.  Measured without gain (247 us for the chunk below): two threads to a
+// row (244), the output product begun on the first half of the weights (258),
+// a quarter of the exponentials as polynomials (274), spinning on barriers
+// (273).
+//
 //   warp 0        TMEM owner and MMA issuer: per key tile j and query tile t,
 //                 O_t += P_t V_j, then S_t = Q_t K_{j+1}^T
 //   next warps    dense: one, TMA.  Packed: three producers; the line of units
@@ -423,6 +431,10 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_addr = tmem + lane_addr + t * 128;
     const uint32_t o_addr = tmem + lane_addr + 256 + t * 128;
+    // (all lanes or none: one that gave up alone would leave the others in a vote)
+    auto wait = [&](uint64_t* bar, uint32_t phase) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, phase, wait_flag, p.wait_ns));
+    };
     const int nkv = t ? n_t[1] : n_t[0];
     const float c = p.scale_log2;
     int lim;
@@ -452,7 +464,7 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
     }
     float m_ref = kTcFloor, l = 0.f;
     for (int j = 0; j < nkv && ok; ++j) {
-      if (!mbar_wait(&s_full[t], j & 1, wait_flag, p.wait_ns)) { ok = false; break; }
+      if (!wait(&s_full[t], j & 1)) { ok = false; break; }
       fence_after_sync();
       uint32_t raw[128];
 #pragma unroll
@@ -482,7 +494,7 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
       if (__any_sync(0xffffffffu, rescale)) {
         tmem_st_wait();
         tile_sum = compute_p<BF16>(raw, c, m_ref, s_addr);
-        if (!mbar_wait(&o_done[t], (j - 1) & 1, wait_flag, p.wait_ns)) ok = false;
+        if (!wait(&o_done[t], (j - 1) & 1)) ok = false;
         fence_after_sync();
         if (ok) {
 #pragma unroll
@@ -503,7 +515,7 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[t]);
     }
-    if (ok && nkv > 0 && !mbar_wait(&o_done[t], (nkv - 1) & 1, wait_flag, p.wait_ns)) ok = false;
+    if (ok && nkv > 0 && !wait(&o_done[t], (nkv - 1) & 1)) ok = false;
     fence_after_sync();
     if (ok) {
       // (where the row lies is worked out again: the loop has no registers to keep it in)
