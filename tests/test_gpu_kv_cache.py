@@ -537,6 +537,42 @@ def test_step_in_a_graph_with_moving_lengths(mx):
         check(o, *attend64(plan, q, None, 0.1, False))
 
 
+@pytest.mark.parametrize("tokens", [100, 300])  # packed and split along the keys; expanded
+def test_chunks_in_a_graph_with_moving_lengths(mx, tokens):
+    """A captured chunk (write, attend, read back) replays with other lengths and counts, against the eager calls."""
+    plan = Plan(mx, [900, 500], kv_heads=2)
+    table, lengths, counts = mx.array(plan.table), ints([tokens, tokens]), ints([tokens, tokens])
+    offsets = ints([0, 0])
+    k, v = (rand((2, 2, tokens, 128), "bfloat16", 40 + i) for i in range(2))
+    q = rand((2, 8, tokens, 128), "bfloat16", 42)
+
+    def step():
+        mx.fast.quantized_cache_update(plan.cache, mx.array(k), mx.array(v), mx.array(offsets), block_table=table,
+                                       counts=mx.array(counts))
+        o = mx.fast.quantized_cache_attention(mx.array(q), plan.cache, mx.array(lengths), block_table=table,
+                                              counts=mx.array(counts), scale=0.1, mask="causal")
+        kv = mx.fast.quantized_cache_fetch(plan.cache, mx.array(lengths), block_table=table, max_length=700)
+        return o._t, kv[0]._t, kv[1]._t
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for n, c in [((900, 500), (tokens, tokens)), ((tokens, 1), (tokens, 1)), ((77, 333), (5, 0)), ((640, 0), (90, 0))]:
+        lengths.copy_(ints(list(n)))
+        counts.copy_(ints(list(c)))
+        offsets.copy_(lengths - counts)
+        k.copy_(rand(k.shape, "bfloat16", 50 + n[0]))
+        g.replay()
+        plan.lengths = list(n)
+        check(out[0], *attend64(plan, q, list(c), 0.1, True))
+        assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
 def test_two_streams_at_once(mx):
     """Calls on two streams share nothing but the cache they read."""
     plan = Plan(mx, [3000] * 4, kv_heads=4, page=64)
