@@ -202,7 +202,9 @@ struct UpdateParams {
 // The group's scale and bias, and the reciprocal that codes are taken with.
 struct Affine {
   float sc, bi, inv;
-  bool plain;  // quotients lie in [0, top + 1/2), and the reciprocal's steps below give them
+  bool plain;  // quotients lie in [0, top + 1/2), or with `over` in [0, top + 3/2), and the reciprocal's steps give them
+  bool over;   // the largest codes are to be held at top: bf16 rounds a scale by 2^-8 of it, one code in 255 (7 % of
+               // groups of 64 normals; the other types' roundings stay below half a code)
 };
 template <typename T, int BITS> __device__ __forceinline__ Affine affine_of(const Range<T>& r) {
   constexpr float top = (1 << BITS) - 1, part = 1.f / top;
@@ -225,7 +227,10 @@ template <typename T, int BITS> __device__ __forceinline__ Affine affine_of(cons
   } else {
     a.inv = __frcp_rn(a.sc);
   }
-  a.plain = d * a.inv < top + 0.4999f;
+  constexpr bool holds = std::is_same<T, bf16>::value && BITS == 8;
+  const float most = d * a.inv;
+  a.plain = most < top + (holds ? 1.4999f : 0.4999f);
+  a.over = holds && most >= top + 0.4999f;
   if (sizeof(T) == 4) a.plain = a.plain && (__float_as_uint(a.sc) & 0x7fffffu) != 0x7fffffu;
   return a;
 }
@@ -253,6 +258,13 @@ __device__ __forceinline__ void codes8(const Eight<T>& x, const Affine& a, uint3
     t[i] = add2(v, up);
     q[i] = add2(t[i], down);
   }
+  if (a.over) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      t[i] = two(fminf(lo_of(t[i]), kRound + top), fminf(hi_of(t[i]), kRound + top));
+      q[i] = add2(t[i], down);
+    }
+  }
   if (!a.plain || !(lo_of(any) + hi_of(any) < INFINITY)) {  // odd scales, or a value that is no number (code 0)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -278,15 +290,17 @@ __device__ __forceinline__ void codes8(const Eight<T>& x, const Affine& a, uint3
 }
 
 // Bound by HBM (update of 4 x 32 heads x 8192 tokens of 128 bf16 values with
-// the values written back: 1.22 GB in 237 us, 5.2 TB/s, 0.79 of the copy rate).  A thread takes eight neighbouring values
-// of either half of a row, so that every load and store of a warp is
-// contiguous and the row's address is worked out once for sixteen values; a
-// group is G / 8 neighbouring lanes, or both halves of D / 16.
+// the values written back: 1.22 GB in 225 us, 5.4 TB/s, 0.83 of the copy rate)
+// and by issue slots (0.74 of them).  A thread takes sixteen neighbouring
+// values of a row, so that its address and the group's scale are worked out once
+// for them; a group is G / 16 neighbouring lanes.  (Eight of either half of the
+// row make every access of a warp contiguous: 4 % faster for f32 with its values
+// written back, 4 to 10 % slower for the 16-bit types and without values.)
 template <typename T, int BITS, int D, int G>
 __global__ void __launch_bounds__(kThreads) update_kernel(const UpdateParams p) {
   constexpr int LANES = D / 16;                 // threads to a row
   constexpr int PER_PASS = kThreads / LANES;    // rows to a pass of the block
-  constexpr int LG = G < D ? G / 8 : LANES;     // lanes of a group
+  constexpr int LG = G / 16;                    // lanes of a group
   constexpr int NG = D / G;
   const int side = blockIdx.y;
   const int c = threadIdx.x % LANES;
@@ -306,9 +320,9 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const UpdateParams p) 
     in[u][0] = in[u][1] = Eight<T>{};
     if (have[u]) {
       const Row r = row_after(p.split, first, first_row, row - first_row, PER_PASS * kRows);
-      const T* x = xs + r.b * p.st[side][2] + r.h * p.st[side][1] + r.i * p.st[side][0] + c * 8;
+      const T* x = xs + r.b * p.st[side][2] + r.h * p.st[side][1] + r.i * p.st[side][0] + c * 16;
       in[u][0] = load8(x);
-      in[u][1] = load8(x + D / 2);
+      in[u][1] = load8(x + 8);
       live[u] = !p.counts || r.i < __ldg(p.counts + r.b);
       if (live[u]) {
         at[u] = row_of(p.c.map, r.b, r.h, static_cast<int64_t>(__ldg(p.offsets + r.b)) + r.i);
@@ -318,48 +332,44 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const UpdateParams p) 
   }
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
-    Range<T> r[2];
-    r[0].of(in[u][0]);
-    r[1].of(in[u][1]);
-    if (G == D) r[0].with(r[1]);
-    r[0].across(LG);
-    if (G < D)
-      r[1].across(LG);
-    else
-      r[1] = r[0];
+    Range<T> r, r1;
+    r.of(in[u][0]);
+    r1.of(in[u][1]);
+    r.with(r1);
+    r.across(LG);
     if (!have[u]) continue;
     T* dense = nullptr;
-    if (p.dense[side]) dense = static_cast<T*>(p.dense[side]) + static_cast<int64_t>(row0 + u * PER_PASS) * D + c * 8;
+    if (p.dense[side]) dense = static_cast<T*>(p.dense[side]) + static_cast<int64_t>(row0 + u * PER_PASS) * D + c * 16;
     if (!live[u]) {
       if (dense) {
         store8(dense, Eight<T>{});
-        store8(dense + D / 2, Eight<T>{});
+        store8(dense + 8, Eight<T>{});
       }
       continue;
     }
+    const Affine a = affine_of<T, BITS>(r);
+    uint32_t words[2][BITS / 4];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const Affine a = affine_of<T, BITS>(r[half]);
-      uint32_t words[BITS / 4];
       uint64_t q[4];
-      codes8<T, BITS>(in[u][half], a, words, q);
-      if (at[u] != kNoRow) {
-        uint32_t* dst = p.c.codes[side] + static_cast<int64_t>(at[u]) * (D * BITS / 32) + (half * (D / 16) + c) * (BITS / 4);
-        if (BITS == 4)
-          dst[0] = words[0];
-        else
-          *reinterpret_cast<uint2*>(dst) = make_uint2(words[0], words[BITS / 4 - 1]);
-        if (c % LG == 0 && (G < D || half == 0)) {
-          const int64_t s_at = static_cast<int64_t>(at[u]) * NG + (half * (D / 2) + c * 8) / G;
-          static_cast<T*>(p.c.scales[side])[s_at] = from_f32<T>(a.sc);
-          static_cast<T*>(p.c.biases[side])[s_at] = from_f32<T>(a.bi);
-        }
-      }
+      codes8<T, BITS>(in[u][half], a, words[half], q);
       if (dense) {
         Eight<T> out;
 #pragma unroll
         for (int i = 0; i < 4; ++i) set_pair(out, i, fma2(two(a.sc, a.sc), q[i], two(a.bi, a.bi)));
-        store8(dense + half * (D / 2), out);
+        store8(dense + half * 8, out);
+      }
+    }
+    if (at[u] != kNoRow) {
+      uint32_t* dst = p.c.codes[side] + static_cast<int64_t>(at[u]) * (D * BITS / 32) + c * (BITS / 2);
+      if (BITS == 4)
+        *reinterpret_cast<uint2*>(dst) = make_uint2(words[0][0], words[1][0]);
+      else
+        *reinterpret_cast<uint4*>(dst) = make_uint4(words[0][0], words[0][BITS / 4 - 1], words[1][0], words[1][BITS / 4 - 1]);
+      if (c % LG == 0) {
+        const int64_t s_at = static_cast<int64_t>(at[u]) * NG + c / LG;
+        static_cast<T*>(p.c.scales[side])[s_at] = from_f32<T>(a.sc);
+        static_cast<T*>(p.c.biases[side])[s_at] = from_f32<T>(a.bi);
       }
     }
   }
@@ -376,7 +386,7 @@ struct FetchParams {
 
 // Bound by HBM, mostly by the values written (16 ragged sequences of up to
 // 8192 tokens, 8 heads of 128 in bf16: 99 us, 0.96 of the copy rate).  Eight codes of either half of
-// a row to a thread, as in update_kernel.  A code becomes a float by a byte
+// a row to a thread.  A code becomes a float by a byte
 // permutation into 2^23 + code (conversions run at an eighth of the rate),
 // two values to an instruction from there.
 // EXPAND: as expand() says.
