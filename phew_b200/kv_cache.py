@@ -254,7 +254,8 @@ def quantized_cache_update(cache: QuantizedKVCache, k, v, offsets, *, block_tabl
     the inputs (``mx.dequantize``'s, zero behind ``counts``), e.g. for a prompt's
     own attention.  Two tokens of one call must not land in the same row.
     A position or page outside the cache is left unwritten and reported by
-    ``ops.check_device_errors``.
+    ``ops.check_device_errors``.  Inside ``mx.compile`` pending arrays that
+    read the cache's arrays are computed before the write.
     """
     k, ks = _rows(k, "quantized_cache_update: k", cache)
     v, vs = _rows(v, "quantized_cache_update: v", cache)
@@ -268,6 +269,7 @@ def quantized_cache_update(cache: QuantizedKVCache, k, v, offsets, *, block_tabl
     off = _ints(offsets, batch, "quantized_cache_update: offsets", cache)
     cnt = None if counts is None else _ints(counts, batch, "quantized_cache_update: counts", cache)
     keep, table, stride, columns = _table(block_table, batch, "quantized_cache_update", cache)
+    core.settle_readers([a._t for a in (*cache.keys, *cache.values)])
     out = None
     if fetch:
         out = (_empty_like(k), _empty_like(k))

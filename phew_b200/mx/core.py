@@ -445,8 +445,20 @@ def _elementwise(op: str, operands: list, out_dtype: Dtype | None = None,
 # evaluation) and keeps the result.  A pending node read by two different
 # materialisations is computed in both (elementwise recompute is cheaper
 # than a round trip through HBM).
+#
+# A pending node holds its operands, not their values, so an op that writes
+# into an array calls `settle_readers` first: op-by-op evaluation would have
+# read the array before the write.
 
 _trace = threading.local()
+
+# Deferred nodes that are alive, by id (each removes itself when it dies).
+_deferred: dict[int, weakref.ref] = {}
+
+
+def _note_deferred(a: "_Lazy") -> None:
+    key = id(a)
+    _deferred[key] = weakref.ref(a, lambda _, key=key: _deferred.pop(key, None))
 
 
 def _tracing() -> bool:
@@ -465,6 +477,7 @@ class _Lazy(array):
         object.__setattr__(a, "_shape", tuple(int(x) for x in shape))
         object.__setattr__(a, "_dtype", node_dt)
         object.__setattr__(a, "_mt", None)
+        _note_deferred(a)
         return a
 
     @property
@@ -731,6 +744,33 @@ def trace_exit() -> None:
     _trace.depth = getattr(_trace, "depth", 1) - 1
 
 
+def _storage_range(t: torch.Tensor) -> tuple[int, int]:
+    st = t.untyped_storage()
+    return st.data_ptr(), st.data_ptr() + st.nbytes()
+
+
+def settle_readers(tensors) -> None:
+    """Materialise every pending array that reads the memory of one of
+    `tensors`, views of it included: called before an op writes into them.
+    (Nodes that only read such an array then hold its computed value.)"""
+    if not _deferred:
+        return
+    written = [_storage_range(t) for t in tensors]
+    for key, ref in list(_deferred.items()):
+        a = ref()
+        if a is None or not a.pending:
+            _deferred.pop(key, None)  # dead or computed: nothing to settle any more
+            continue
+        op = a._op
+        for x in ((op[2],) if op[0] == _ROW_REDUCE else op[1]):
+            if not isinstance(x, array) or (isinstance(x, _Lazy) and x.pending):
+                continue
+            lo, hi = _storage_range(x._t)
+            if builtins.any(lo < w_hi and w_lo < hi for w_lo, w_hi in written):
+                a._t  # noqa: B018  (materialises)
+                break
+
+
 def settle(x):
     """Materialise every pending array in `x` (an array or nested list /
     tuple / dict of them) and return the same structure of plain arrays."""
@@ -974,6 +1014,7 @@ def _reduce(opname: str, a, axis=None, keepdims=False) -> array:
         object.__setattr__(m, "_shape", tuple(a.shape[:-1]) + (1,))
         object.__setattr__(m, "_dtype", a.dtype)
         object.__setattr__(m, "_mt", None)
+        _note_deferred(m)
         return m
     return _reduce_now(opname, a, axis, keepdims)
 
