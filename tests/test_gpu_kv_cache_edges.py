@@ -42,3 +42,122 @@ def test_pending_readers_of_the_cache_see_it_before_the_update(mx):
         got.append([a._t.clone() for a in f(plan.cache, mx.array(plan.table))])
     assert not torch.equal(got[0][0], got[0][3])  # the update changed what is read
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+# --- attention, row by row and group by group -------------------------------------------
+
+
+def bounds(plan, q, counts, scale, causal, tensor_core=False):
+    """(output, bound of its error's norm, what a lost tile of 32 keys would change) in 64 bits, the last two
+    per row and group of the head dimension.
+
+    Errors are independent from key to key, so norms add in squares.  With w_j a row's softmax weights, s_j and
+    n_j a value's scale and codes, v'_j = s_j (n_j - 8), or s_j n_j where bf16 sums hold bare codes, or the
+    values rounded to the type on the tcgen05 path (more than 64 rows, where keys are too):
+      * the output rounded once: u |o|
+      * weights times scales rounded by at most h of them (2^-11 as one f16 term, 2^-22 as two, u on the tcgen05
+        path): h N, N = sqrt(sum w_j^2 |v'_j|^2); 1.5 of it, the most that two keys can give
+      * scores off by e: e N.  Products of bare key codes are cut at 2^-14 of the largest query times a code's
+        step: 6 sqrt(D / 3) 2^-14 max|q| max s scale at six sigma; of codes less 8, and in f32's sums and
+        queries of 22 bits, 2^-19 |q| |k| scale by Cauchy and Schwarz
+      * f16's smallest steps: 2^-23 of the largest weight times scale, for each key: sqrt(keys) of that
+      * 32-bit sums: 2^-21 of the sum of the magnitudes, 2^-19 where bare codes pile up over 32 additions."""
+    u = 2.0 ** {"bfloat16": -8, "float16": -11, "float32": -24}[plan.dtype]
+    B, H, L, D = q.shape
+    G, per = plan.group, H // plan.kv_heads
+    ng = D // G
+    out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    tol = torch.zeros((B, H, L, ng), dtype=torch.float64, device="cuda")
+    tile = torch.zeros_like(tol)
+    rounded = (lambda x: x.float().to(DTYPES[plan.dtype]).double()) if tensor_core else (lambda x: x)
+    h = u if tensor_core else 2.0 ** (-22 if plan.dtype == "float32" else -11)
+    bare = plan.dtype == "bfloat16" and not tensor_core
+    for b, n in enumerate(plan.lengths):
+        c = L if counts is None else counts[b]
+        if n == 0 or c == 0:
+            continue
+        K, V = rounded(plan.values(0, b)), rounded(plan.values(1, b))
+        cols = plan.table[b, : -(-n // plan.page)].long()
+        pick = lambda t: t._t[cols].transpose(0, 1).flatten(1, 2)[:, :n].double()  # noqa: E731
+        sk, sv, zv = pick(plan.parts(0)[1]).abs(), pick(plan.parts(1)[1]), pick(plan.parts(1)[2])
+        for head in range(H):
+            k, v, s_v, z_v = K[head // per], V[head // per], sv[head // per], zv[head // per]
+            x = q[b, head, :c].double()
+            s = (x @ k.T) * scale
+            if causal:
+                i = torch.arange(c, device="cuda")[:, None]
+                s = s.masked_fill(torch.arange(n, device="cuda")[None] > n - c + i, -torch.inf)
+            w = torch.where((s > -torch.inf).any(-1, keepdim=True), torch.softmax(s, -1), 0.0)
+            o = w @ v
+            vg = v.unflatten(-1, (ng, G))
+            centre = z_v[..., None] if bare else z_v[..., None] + 8 * s_v[..., None]
+            lone = (vg if tensor_core else vg - centre).norm(dim=-1)  # |v'_j| of a group
+            N = (w.square() @ lone.square()).sqrt()
+            seen = (w > 0).double()
+            qk = x.norm(dim=-1, keepdim=True) * (seen * k.norm(dim=-1)).amax(-1, keepdim=True) * abs(scale)
+            cut = 0.0 if plan.dtype == "float32" else (
+                6 * (D / 3) ** 0.5 * 2.0 ** -14 * abs(scale) * x.abs().amax(-1, keepdim=True)
+                * (seen * sk[head // per].amax(-1)).amax(-1, keepdim=True))
+            e = qk * 2.0 ** -19 + cut
+            step = s_v.abs()
+            top = torch.stack([(w * step[:, g]).amax(-1) for g in range(ng)], -1)
+            piles = w @ (8 * step + (vg.abs().amax(-1) if tensor_core else centre[..., 0].abs()))
+            og = o.unflatten(-1, (ng, G)).norm(dim=-1)
+            out[b, head, :c] = o
+            tol[b, head, :c] = (u * og + (1.5 * h + e) * N + n ** 0.5 * 2.0 ** -23 * 8 * G ** 0.5 * top
+                                + 2.0 ** (-19 if bare else -21) * G ** 0.5 * piles)
+            lost = w.clone()
+            lost[:, max(0, n // 2 - 16) : n // 2 + 16] = 0
+            total = lost.sum(-1, keepdim=True)
+            lost = lost / torch.where(total > 0, total, 1.0)
+            tile[b, head, :c] = (o - lost @ v).unflatten(-1, (ng, G)).norm(dim=-1)
+    return out, tol, tile
+
+
+def groups_err(got, want, group):
+    return (got.double() - want).unflatten(-1, (-1, group)).norm(dim=-1)
+
+
+def attend_closely(mx, plan, q, counts=None, causal=False, scale=None, sharp=True):
+    """Attention within the bound above, and where `sharp`, that the bound would notice a lost tile or zeros."""
+    scale = plan.head_dim ** -0.5 if scale is None else scale
+    rows = q.shape[2] * (q.shape[1] // plan.kv_heads)
+    tensor_core = plan.dtype != "float32" and rows > 64 and scale > 0
+    o = mx.fast.quantized_cache_attention(
+        mx.array(q), plan.cache, mx.array(ints(plan.lengths)), block_table=mx.array(plan.table),
+        counts=None if counts is None else mx.array(ints(counts)), scale=scale, mask="causal" if causal else None)._t
+    want, tol, tile = bounds(plan, q, counts, scale, causal, tensor_core)
+    if sharp:
+        n = torch.tensor(plan.lengths, device="cuda")[:, None, None, None].expand_as(tol)
+        live = (tol > 0) & (n >= 64)
+        assert live.any()
+        assert float((want.unflatten(-1, (-1, plan.group)).norm(dim=-1) > 4 * tol)[live].double().mean()) > 0.99
+        assert float((tile > 2 * tol)[live].double().mean()) > (0.4 if causal else 0.99)
+    err = groups_err(o, want, plan.group)
+    worst = float((err / tol.clamp_min(1e-300)).nan_to_num(torch.inf).masked_fill((tol == 0) & (err == 0), 0.0).max())
+    assert worst <= 1.0, f"{worst:.3g} of the bound"
+    return o
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("head_dim,group,heads", [(64, 32, 4), (64, 64, 24), (128, 32, 8), (128, 64, 2), (128, 64, 24),
+                                                  (128, 128, 10), (256, 32, 2), (256, 64, 16), (256, 128, 6)])
+def test_tokens_closely(mx, dtype, head_dim, group, heads):
+    plan = Plan(mx, [1, 2500, 130, 0, 700], kv_heads=2, head_dim=head_dim, group=group, dtype=dtype, seed=heads)
+    attend_closely(mx, plan, rand((5, heads, 1, head_dim), dtype, 3))
+    attend_closely(mx, plan, rand((5, heads, 3, head_dim), dtype, 4), [1, 3, 2, 3, 0], causal=True)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_long_histories_closely(mx, dtype):
+    plan = Plan(mx, [9000, 1, 4096], kv_heads=1, page=64, dtype=dtype, seed=2)
+    attend_closely(mx, plan, rand((3, 4, 1, 128), dtype, 5))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("head_dim,group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128), (256, 64)])
+@pytest.mark.parametrize("tokens,heads", [(40, 4), (150, 4), (300, 8)])  # packed and split; packed; expanded
+@pytest.mark.parametrize("causal", [False, True])
+def test_chunks_closely(mx, dtype, head_dim, group, tokens, heads, causal):
+    plan = Plan(mx, [1500, tokens, 0, 131], kv_heads=2, head_dim=head_dim, group=group, dtype=dtype, page=24, seed=tokens)
+    attend_closely(mx, plan, rand((4, heads, tokens, head_dim), dtype, 7), [tokens, tokens, 3, 31], causal=causal)
