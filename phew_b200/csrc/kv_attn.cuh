@@ -27,12 +27,17 @@
 //    e4m3, which holds a nibble in a byte as it
 //    is, was tried: mma.sync on that type is expanded into conversions here,
 //    11 instructions each.)
-//  * queries and weights are f16 after a power of two: a row's largest query
-//    element goes to [2^14, 2^15); weights, at most 1, times a value scale kept
-//    at most 2^15 by a power of two that follows the largest scale met.
-//    What falls below f16's range is then under 2^-38 of the largest.  f32
-//    queries and weights are two f16 terms (22 bits), and its sums leave the
-//    tensor core, which cuts what it adds off, every 16 keys;
+//  * queries and weights times value scales are f16 after a power of two.  A
+//    row's largest query element goes to [2^14, 2^15): what falls below f16's
+//    range is under 2^-38 of it.  Weights times scales have a factor for each
+//    row and group, set by the largest of them that the row has met, so that
+//    neither another group's values nor a key that the row does not attend
+//    to cost it bits: f16's smallest step is at most 2^-22 of that largest
+//    one.  The factors lie in shared memory and are looked at again only when a
+//    row's maximum moves, or a scale itself would pass f16's range under one of
+//    them (one comparison a tile; a segment's first tile always: 0.5 us of a
+//    short call, 1.8 with two row tiles).  f32 queries and weights are two f16 terms (22 bits), and its
+//    sums leave the tensor core, which cuts what it adds off, every 16 keys;
 //  * a word's eight codes stay with the thread that loads it: the order of
 //    the head dimension inside a product is free, so queries are arranged to
 //    match and nothing is shuffled; weights move from the score fragment
@@ -72,6 +77,8 @@ constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;  // codes of a word 
 constexpr float kGrow = 8.0f;                   // log2 units that a row's scores may grow by before its sums are scaled
 constexpr int kCentreTiles = 16;                // tiles of bare codes in one sum
 constexpr float kFloor = -1.0e38f;              // running maximum before the first key
+constexpr float kF16Most = 32768.f;             // what weights times scales are held below
+constexpr float kNoFactor = 0x1p68f;            // a row's and group's factor before its first weight
 
 struct AttnParams {
   Cache c;
@@ -133,13 +140,14 @@ template <typename T, int D_, int G_, int NT_> struct Shape {
   static constexpr int CODE_BYTES = kTile * D / 2;         // one side's codes of a stage
   static constexpr int STAGE = 2 * CODE_BYTES + 4 * kTile * SROW;
   static constexpr int AFFINE = kTile * NG * 8;            // scales and biases of a stage's side as float pairs
+  static constexpr int FACTORS = ((ROWS + 1) * NG * 4 + 127) / 128 * 128;  // of rows and groups; their largest to a group
   // blocks to an SM (their registers: 65536 / (128 CTAS) to a thread), and as many stages as their share of
   // the SM's 228 KB holds beside the 1 KB that each block costs
   static constexpr int CTAS = D == 256 ? 2 : D == 128 ? (F32 || NT == 2 ? 2 : 3) : (F32 || NT == 2 ? 3 : 4);
   static constexpr int SHARE = (228 / CTAS - 1) * 1024 / kWarps;
-  static constexpr int STAGES = (SHARE - AFFINE) / STAGE < 4 ? (SHARE - AFFINE) / STAGE : 4;
+  static constexpr int STAGES = (SHARE - AFFINE - FACTORS) / STAGE < 4 ? (SHARE - AFFINE - FACTORS) / STAGE : 4;
   static_assert(STAGES >= 2, "a ring needs two stages");
-  static constexpr int RING = STAGE * STAGES + AFFINE;          // per warp
+  static constexpr int RING = STAGE * STAGES + AFFINE + FACTORS;  // per warp
   static constexpr int SMEM = RING * kWarps;
 };
 
@@ -169,6 +177,9 @@ template <int N> __device__ __forceinline__ void load_words(uint32_t addr, uint3
   else
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
 }
+
+// 1 / x of a power of two between 2^-126 and 2^126.
+__device__ __forceinline__ float inverse_pow2(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -343,6 +354,46 @@ template <typename S, typename T> struct Ring {
         else
           out[g] = to_f32(T{static_cast<uint16_t>(g & 1 ? w[g / 2] >> 16 : w[g / 2])});
       }
+    }
+  }
+  // Factors of rows 2 t4 and 2 t4 + 1 of row tile nt, [group][row].
+  __device__ __forceinline__ uint32_t factors(int nt) const {
+    return pairs() + S::AFFINE + (nt * 4 + (lane & 3)) * S::NG * 8;
+  }
+  __device__ __forceinline__ void load_factors(int nt, float (*up)[2]) const {
+    const uint32_t at = factors(nt);
+    if constexpr (S::NG == 1) {
+      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(up[0][0]), "=f"(up[0][1]) : "r"(at));
+    } else {
+#pragma unroll
+      for (int g = 0; g < S::NG; g += 2)
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(up[g][0]), "=f"(up[g][1]), "=f"(up[g + 1][0]), "=f"(up[g + 1][1])
+                     : "r"(at + g * 8));
+    }
+  }
+  // ... called by every lane, which hold the same for the same rows.
+  __device__ __forceinline__ void store_factors(int nt, const float (*up)[2]) const {
+    if (lane < 4) {
+#pragma unroll
+      for (int g = 0; g < S::NG; ++g)
+        asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(factors(nt) + g * 8), "f"(up[g][0]), "f"(up[g][1]) : "memory");
+    }
+  }
+  // The largest of all rows' factors, to a group.
+  __device__ __forceinline__ uint32_t most() const { return pairs() + S::AFFINE + S::ROWS * S::NG * 4; }
+  __device__ __forceinline__ void load_most(float* v) const {
+    uint32_t w[S::NG];
+    constexpr int N = S::NG < 4 ? S::NG : 4;
+#pragma unroll
+    for (int g = 0; g < S::NG; g += N) load_words<N>(most() + g * 4, w + g);
+#pragma unroll
+    for (int g = 0; g < S::NG; ++g) v[g] = __uint_as_float(w[g]);
+  }
+  __device__ __forceinline__ void store_most(const float* v) const {
+    if (lane == 0) {
+#pragma unroll
+      for (int g = 0; g < S::NG; ++g) asm volatile("st.shared.f32 [%0], %1;" ::"r"(most() + g * 4), "f"(v[g]) : "memory");
     }
   }
   // Scales and biases of key `key` on the side shared last.
@@ -591,8 +642,24 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
       // a row's weights are 2^(score - m), m kGrow above its largest score when it last moved; it moves when a
       // score passes it by `pass`, which is 0 once the row has seen a key and below any score before
       float m[NT][2], pass[NT][2], l[NT][2], bsum[NT][2][NG];
-      float wsum[NT][2][NG];  // of bf16: the weights behind `acc`
-      float v_up = 0x1p68f;          // value scales are taken times this
+      float wsum[NT][2][NG];  // of bf16: the weights times scales behind `acc`
+      __syncwarp();           // (the last segment's factors have been read)
+      {
+        float most[NG];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          // a row that sees none of these keys has no weights to fit
+          float up[NG][2];
+#pragma unroll
+          for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) up[g][cc] = lim[nt][cc] > t0 * kTile ? kNoFactor : 1.f;
+          ring.store_factors(nt, up);
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) most[g] = kNoFactor;
+        ring.store_most(most);
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -610,6 +677,74 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
       }
 
       const int my_key = key_of_slot(r8);
+
+      // Factors of the rows and groups whose weights times scales pass f16's range in this tile, are their first, or
+      // are taken against a new m (`moved`, a bit to a row): what was large before may be nothing now.  The tile's largest scale goes to [2^12, 2^13), unless that left less than 2^-2 of the row's
+      // largest weight times scale: then the scales that pass the range have next to no weight.
+      auto fit = [&](float (*s)[NT][4], const float* sv, uint32_t moved) {
+        uint32_t top[NG];
+        float most[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const uint32_t bits = __float_as_uint(fabsf(sv[g]));  // (magnitudes order as their bits)
+          top[g] = __reduce_max_sync(0xffffffffu, bits < 0x7f800000u ? bits : 0u);
+          most[g] = 0.f;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float part[NG][2], up[NG][2];  // the row's largest weight times scale
+#pragma unroll
+          for (int g = 0; g < NG; ++g) part[g][0] = part[g][1] = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float a[NG], z[NG];
+            ring.affine(k * 8 + my_key, a, z);
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) {
+              const float w = exp2_fast(s[k >> 1][nt][2 * (k & 1) + cc]);
+#pragma unroll
+              for (int g = 0; g < NG; ++g) {
+                const float f = w * fabsf(a[g]);
+                if (f < INFINITY) part[g][cc] = fmaxf(part[g][cc], f);
+              }
+            }
+          }
+          ring.load_factors(nt, up);
+#pragma unroll
+          for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) {
+              float f = part[g][cc];
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) f = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, o));
+              float by = 1.f;
+              const bool again = up[g][cc] == kNoFactor || (moved >> (2 * nt + cc) & 1);
+              if (f * up[g][cc] > kF16Most || (again && f > 0.f)) {
+                const int e = max(266 - static_cast<int>(top[g] >> 23),
+                                  252 - static_cast<int>(__float_as_uint(f) >> 23));
+                const float to = __int_as_float(min(e, 195) << 23);  // (at most kNoFactor)
+                by = to / up[g][cc];
+                up[g][cc] = to;
+              }
+              most[g] = fmaxf(most[g], up[g][cc]);
+              wsum[nt][cc][g] *= by;
+#pragma unroll
+              for (int i = g * G / 16; i < (g + 1) * G / 16; ++i) {
+                acc[nt][i][cc] *= by;
+                acc[nt][i][2 + cc] *= by;
+              }
+            }
+          __syncwarp();
+          ring.store_factors(nt, up);
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          most[g] = fmaxf(most[g], __shfl_xor_sync(0xffffffffu, most[g], 1));
+          most[g] = fmaxf(most[g], __shfl_xor_sync(0xffffffffu, most[g], 2));
+        }
+        ring.store_most(most);
+        __syncwarp();
+      };
 
       // One stage of 32 keys; EDGE: some row does not see all of them.
       auto stage = [&](int st, int key0, auto edge_c) {
@@ -660,6 +795,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
         }
         // ---- m: moved only when a score passes it; weights stay below 1 ----
         bool grow = false;
+        uint32_t moved = 0;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -683,6 +819,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
               const float by = move ? top + kGrow : 0.f;
               const float alpha = exp2_fast(fminf(-by, 0.f));  // (a row's first keys find nothing to scale)
               if (move) pass[nt][cc] = 0.f;
+              if (move) moved |= 1u << (2 * nt + cc);
               m[nt][cc] += by;
               l[nt][cc] *= alpha;
 #pragma unroll
@@ -702,46 +839,29 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
               }
             }
         }
-        // ---- value scales, at most 2^15 times a power of two that only shrinks ----
+        // ---- value scales and biases for the whole warp ----
         {
-          float sv[NG], zv[NG];
+          float sv[NG], zv[NG], most[NG];
           ring.load(st, 1, !EDGE || key0 + lane < ent.end, sv, zv);
-          float top = 0.f;
-#pragma unroll
-          for (int g = 0; g < NG; ++g) top = fmaxf(top, fabsf(sv[g]));
-          if (__any_sync(0xffffffffu, top * v_up > 32768.f && top < INFINITY)) {
-            if (!(top < INFINITY)) top = 0.f;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float to = __uint_as_float(min(268u - (__float_as_uint(top) >> 23), 195u) << 23);  // top to [2^14, 2^15)
-            const float f = to / v_up;
-            v_up = to;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-              for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc[nt][i][k] *= f;
-#pragma unroll
-              for (int g = 0; g < NG; ++g) {
-                wsum[nt][0][g] *= f;
-                wsum[nt][1][g] *= f;
-              }
-            }
-          }
+          ring.load_most(most);
+          bool over = false;
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
+            over = over || (fabsf(sv[g]) * most[g] > kF16Most && fabsf(sv[g]) < INFINITY);
             if (VC) zv[g] = fmaf(8.f, sv[g], zv[g]);
-            sv[g] *= v_up;
           }
           __syncwarp();
           ring.share(sv, zv);
           __syncwarp();
+          if (__any_sync(0xffffffffu, over || moved)) fit(s, sv, moved);
         }
         // ---- weights, their sums, and the second product ----
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
           uint32_t pb[NT][NG][TERMS][2];
+          float up[NT][NG][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) ring.load_factors(nt, up[nt]);
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             float sv[NG], zv[NG];
@@ -761,7 +881,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
                 for (int cc = 0; cc < 2; ++cc) {
                   // a key that this row does not see may hold anything
                   const bool none = EDGE && w[cc] == 0.f;
-                  f[cc] = none ? 0.f : w[cc] * sv[g];
+                  f[cc] = none ? 0.f : w[cc] * sv[g] * up[nt][g][cc];
                   if (!VC) wsum[nt][cc][g] += f[cc];
                   bsum[nt][cc][g] = none ? bsum[nt][cc][g] : fmaf(w[cc], zv[g], bsum[nt][cc][g]);
                 }
@@ -824,13 +944,15 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
       // the weights go over to the biases' side before a sum is kCentreTiles long.
       auto centre = [&]() {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+          float up[NG][2];
+          ring.load_factors(nt, up);
 #pragma unroll
           for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int cc = 0; cc < 2; ++cc) {
               float& w = wsum[nt][cc][g];
-              bsum[nt][cc][g] = fmaf(8.f / v_up, w, bsum[nt][cc][g]);
+              bsum[nt][cc][g] = fmaf(8.f * inverse_pow2(up[g][cc]), w, bsum[nt][cc][g]);
 #pragma unroll
               for (int o = 4; o < 32; o <<= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
 #pragma unroll
@@ -841,6 +963,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
               }
               w = 0.f;
             }
+        }
       };
 
       for (int key0 = t0 * kTile; key0 < t1 * kTile; key0 += kTile) {
@@ -879,7 +1002,9 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
         if (t1 == ent.tiles) p.span[segment].y = static_cast<int>(self);
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        float up[NG][2];
+        ring.load_factors(nt, up);
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
           const int row = nt * 8 + 2 * t4 + cc;
@@ -919,12 +1044,12 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
               }
             }
           };
-          // what a sum counts: codes 2^-24 in it, odd ones sixteenfold, value scales times v_up
-          const float even = VC ? 1.f : 0x1p24f, odd = even * 0x1p-4f, down = 1.f / v_up;
+          // what a sum counts: codes 2^-24 in it, odd ones sixteenfold, weights times scales with their factor
+          const float even = VC ? 1.f : 0x1p24f, odd = even * 0x1p-4f;
           if constexpr (G >= 64) {
 #pragma unroll
             for (int j = 0; j < D / 64; ++j) {
-              const float z = bsum[nt][cc][j * 64 / G];
+              const float z = bsum[nt][cc][j * 64 / G], down = inverse_pow2(up[j * 64 / G][cc]);
               float v[8];
 #pragma unroll
               for (int u = 0; u < 4; ++u) {
@@ -936,7 +1061,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
           } else {
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-              const float z = bsum[nt][cc][g];
+              const float z = bsum[nt][cc][g], down = inverse_pow2(up[g][cc]);
               const float v[4] = {fmaf(acc[nt][g * 2][cc] * even, down, z), fmaf(acc[nt][g * 2 + 1][cc] * odd, down, z),
                                   fmaf(acc[nt][g * 2][2 + cc] * even, down, z), fmaf(acc[nt][g * 2 + 1][2 + cc] * odd, down, z)};
               put((g * 4 + (r8 & 3)) * 8 + (r8 & 4), v, std::integral_constant<int, 4>());
@@ -947,6 +1072,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
             p.part_ml[slot * 2 + 1] = sum;
           }
         }
+      }
     }
     base += static_cast<uint64_t>(kv_heads) * units;
     ++e;

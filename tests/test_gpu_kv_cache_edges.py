@@ -54,7 +54,8 @@ def bounds(plan, q, counts, scale, causal, tensor_core=False):
     Errors are independent from key to key, so norms add in squares.  With w_j a row's softmax weights, s_j and
     n_j a value's scale and codes, v'_j = s_j (n_j - 8), or s_j n_j where bf16 sums hold bare codes, or the
     values rounded to the type on the tcgen05 path (more than 64 rows, where keys are too):
-      * the output rounded once: u |o|
+      * the output rounded once: u |o|, and below 2^-14, where f16's steps stay 2^-24, half a step for each of a
+        group's values: 2^-25 sqrt(group)
       * weights times scales rounded by at most h of them (2^-11 as one f16 term, 2^-22 as two, u on the tcgen05
         path): h N, N = sqrt(sum w_j^2 |v'_j|^2); 1.5 of it, the most that two keys can give
       * scores off by e: e N.  Products of bare key codes are cut at 2^-14 of the largest query times a code's
@@ -104,7 +105,8 @@ def bounds(plan, q, counts, scale, causal, tensor_core=False):
             piles = w @ (8 * step + (vg.abs().amax(-1) if tensor_core else centre[..., 0].abs()))
             og = o.unflatten(-1, (ng, G)).norm(dim=-1)
             out[b, head, :c] = o
-            tol[b, head, :c] = (u * og + (1.5 * h + e) * N + n ** 0.5 * 2.0 ** -23 * 8 * G ** 0.5 * top
+            floor = 2.0 ** -25 * G ** 0.5 if plan.dtype == "float16" else 0.0
+            tol[b, head, :c] = (u * og + floor + (1.5 * h + e) * N + n ** 0.5 * 2.0 ** -23 * 8 * G ** 0.5 * top
                                 + 2.0 ** (-19 if bare else -21) * G ** 0.5 * piles)
             lost = w.clone()
             lost[:, max(0, n // 2 - 16) : n // 2 + 16] = 0
@@ -161,3 +163,77 @@ def test_long_histories_closely(mx, dtype):
 def test_chunks_closely(mx, dtype, head_dim, group, tokens, heads, causal):
     plan = Plan(mx, [1500, tokens, 0, 131], kv_heads=2, head_dim=head_dim, group=group, dtype=dtype, page=24, seed=tokens)
     attend_closely(mx, plan, rand((4, heads, tokens, head_dim), dtype, 7), [tokens, tokens, 3, 31], causal=causal)
+
+
+# --- values of very different magnitude ---------------------------------------------------
+
+
+def spread(dtype, bits):
+    """Two factors 2^bits apart (24 at most in f16) whose values, and the steps between them, every type holds."""
+    if dtype == "float16":
+        bits = min(bits, 24)
+        return 2.0 ** (bits // 2), 2.0 ** (bits // 2 - bits)
+    return 2.0 ** bits, 1.0
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("bits", [10, 20, 36])
+@pytest.mark.parametrize("head_dim,group,heads", [(64, 32, 2), (128, 64, 8), (128, 32, 20), (256, 32, 2)])
+def test_groups_of_different_magnitude(mx, dtype, bits, head_dim, group, heads):
+    """Small values beside large ones: each group to its own precision."""
+    plan = Plan(mx, [1200, 90], kv_heads=2, head_dim=head_dim, group=group, dtype=dtype, seed=bits)
+    large, small = spread(dtype, bits)
+    factor = torch.full((head_dim // group,), large, device="cuda")
+    factor[1::2] = small
+    for part in plan.cache.values[1:]:
+        part._t.copy_(part._t.float() * factor)
+    attend_closely(mx, plan, rand((2, heads, 1, head_dim), dtype, 6))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("heads,tokens", [(2, 1), (8, 2), (16, 3), (30, 3)])
+@pytest.mark.parametrize("at", [0, 5, 700])
+def test_a_large_value_of_no_weight(mx, dtype, heads, tokens, at):
+    """A key that no query attends to may have values of any size, wherever a warp meets it."""
+    plan = Plan(mx, [1200], kv_heads=2, dtype=dtype, page=1200, spare=0)
+    large, small = spread(dtype, 36)
+    k, v = plan.dense
+    k[:, :, at] = -8.0
+    v *= small
+    v[:, :, at] *= large / small
+    sides = [mx.quantize(mx.array(x), group_size=64, bits=4) for x in plan.dense]
+    plan.cache = mx.fast.QuantizedKVCache(*sides, group_size=64, bits=4)
+    attend_closely(mx, plan, rand((1, heads, tokens, 128), dtype, 8).abs(), scale=0.125)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("heads,kv_heads,tokens", [(2, 2, 3), (4, 2, 7), (2, 1, 30), (4, 2, 80)])
+def test_a_large_value_that_later_tokens_alone_see(mx, dtype, heads, kv_heads, tokens):
+    plan = Plan(mx, [200], kv_heads=kv_heads, dtype=dtype, page=200, spare=0)
+    large, small = spread(dtype, 60)
+    v = plan.dense[1]
+    v *= small
+    v[:, :, 199] *= large / small
+    sides = [mx.quantize(mx.array(x), group_size=64, bits=4) for x in plan.dense]
+    plan.cache = mx.fast.QuantizedKVCache(*sides, group_size=64, bits=4)
+    q = rand((1, heads, tokens, 128), dtype, 9)
+    o = attend_closely(mx, plan, q, causal=True, sharp=False)
+    plan.lengths = [199]  # without that key the other rows have a bound of their own
+    want, tol, _ = bounds(plan, q[:, :, :-1], None, 128 ** -0.5, True, dtype != "float32" and tokens * heads // kv_heads > 64)
+    assert bool((groups_err(o[:, :, :-1], want, 64) <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("heads,tokens", [(2, 1), (8, 2), (30, 3)])
+def test_large_values_whose_weight_fades(mx, dtype, heads, tokens):
+    """Scores rise along the keys; the first keys, whose values are large, weigh nothing in the end."""
+    plan = Plan(mx, [700], kv_heads=2, dtype=dtype, page=700, spare=0)
+    large, small = spread(dtype, 36)
+    k, v = plan.dense
+    k.copy_(torch.linspace(-4, 4, 700, device="cuda")[:, None] + 0.02 * k)
+    v *= small
+    v[:, :, :64] *= large / small
+    sides = [mx.quantize(mx.array(x), group_size=64, bits=4) for x in plan.dense]
+    plan.cache = mx.fast.QuantizedKVCache(*sides, group_size=64, bits=4)
+    q = torch.ones((1, heads, tokens, 128), device="cuda").to(DTYPES[dtype])
+    attend_closely(mx, plan, q, scale=0.5, sharp=False)
