@@ -323,7 +323,9 @@ int phew_quantize(const void* w, void* wq, void* scales, void* biases, int64_t r
  * table live on the device, so that a captured graph replays with new ones;
  * table entries behind a sequence's last page are not read.  A position
  * outside a sequence's pages or a table entry that is no page of the cache
- * is not accessed: it sets error_flag[0] to PHEW_ERR_INVALID.  error_flag is
+ * is not accessed: it sets error_flag[0] to PHEW_ERR_INVALID, and its keys
+ * and values count as zeros (a length past a sequence's pages ends at them).
+ * error_flag is
  * two device ints; a pipeline wait of phew_kv_attention that runs out sets
  * error_flag[1] to PHEW_ERR_TIMEOUT. */
 typedef struct phew_kv_cache {

@@ -156,15 +156,15 @@ template <typename T, int D_, int G_, int NT_> struct Shape {
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
-template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
-  if constexpr (N == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-// four bytes of which `valid` are read, the rest zero
-__device__ __forceinline__ void copy_async_upto4(uint32_t dst, const void* src, int valid) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+// N bytes of which `valid` are read, the rest zero
+template <int N> __device__ __forceinline__ void copy_async_upto(uint32_t dst, const void* src, int valid) {
+  if constexpr (N == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(valid) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -266,8 +266,9 @@ template <typename S, typename T> struct Ring {
 
   __device__ __forceinline__ uint32_t pairs() const { return base + S::STAGE * S::STAGES; }
 
-  // Starts the copy of the 32 rows that the lanes hold into stage `s`; EIGHTS: rows of eight keys lie side by side.
-  template <bool EIGHTS> __device__ __forceinline__ void issue(int s, uint32_t row) {
+  // Starts the copy of the 32 rows that the lanes hold into stage `s`, zeros for the scales and biases of a lane
+  // that has no `page`; EIGHTS: rows of eight keys lie side by side.
+  template <bool EIGHTS> __device__ __forceinline__ void issue(int s, uint32_t row, bool page) {
     const uint32_t at = base + s * S::STAGE;
     const int ch = lane % CH, sub = lane / CH;
     constexpr uint32_t ROW = S::D / 2;
@@ -280,8 +281,8 @@ template <typename S, typename T> struct Ring {
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const uint32_t src = __shfl_sync(0xffffffffu, row, i * RP + (RP == 8 ? 0 : sub & ~7));
-        copy_async<16>(dst + i * RP * ROW, k + static_cast<uint64_t>(src) * ROW);
-        copy_async<16>(dst + S::CODE_BYTES + i * RP * ROW, v + static_cast<uint64_t>(src) * ROW);
+        copy_async16(dst + i * RP * ROW, k + static_cast<uint64_t>(src) * ROW);
+        copy_async16(dst + S::CODE_BYTES + i * RP * ROW, v + static_cast<uint64_t>(src) * ROW);
       }
     } else {
 #pragma unroll
@@ -291,8 +292,8 @@ template <typename S, typename T> struct Ring {
         for (int i = 0; i < CH; ++i) {
           const int r = i * RP + sub;
           const uint32_t src = __shfl_sync(0xffffffffu, row, side == 0 ? key_of_slot(r) : r);
-          copy_async<16>(at + side * S::CODE_BYTES + r * ROW + swizzle<S::D>(r, ch) * 16,
-                         codes + static_cast<uint64_t>(src) * ROW);
+          copy_async16(at + side * S::CODE_BYTES + r * ROW + swizzle<S::D>(r, ch) * 16,
+                       codes + static_cast<uint64_t>(src) * ROW);
         }
       }
     }
@@ -304,11 +305,12 @@ template <typename S, typename T> struct Ring {
         // the aligned word around the two bytes; the array's last row alone has no partner behind it
         const uint32_t rows = static_cast<uint32_t>(c.map.pages) * static_cast<uint32_t>(c.map.kv_heads) *
                               static_cast<uint32_t>(c.map.page_size);
-        copy_async_upto4(dst, arr + static_cast<uint64_t>(row & ~1u) * 2, (row | 1u) < rows ? 4 : 2);
+        copy_async_upto<4>(dst, arr + static_cast<uint64_t>(row & ~1u) * 2, !page ? 0 : (row | 1u) < rows ? 4 : 2);
       } else {
         constexpr int N = S::SB < 16 ? S::SB : 16;
 #pragma unroll
-        for (int i = 0; i < S::SB; i += N) copy_async<N>(dst + i, arr + static_cast<uint64_t>(row) * S::SB + i);
+        for (int i = 0; i < S::SB; i += N)
+          copy_async_upto<N>(dst + i, arr + static_cast<uint64_t>(row) * S::SB + i, page ? N : 0);
       }
     }
     if constexpr (S::SB == 2) odd = (odd & ~(1u << s)) | ((row & 1u) << s);
@@ -509,7 +511,9 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
       if (t1 <= t0) continue;  // units of the begin alone
 
       // ---- the ring: page numbers one stage ahead of the copies, copies STAGES - 1 ahead of the products.
-      // A lane without a key copies row 0 of the cache: whatever it holds is masked. ----
+      // A lane without a key copies row 0 of the cache: whatever it holds is masked.  So does one whose page is none
+      // of the cache's, with zeros for scales and biases: its key and value count as zeros, as in the tcgen05
+      // kernel. ----
       struct Look {
         int page;  // -1: no key
         uint32_t row;
@@ -538,16 +542,18 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
       auto start_copy = [&](const Look& k) {
         if (left > 0) {
           uint32_t row = 0;
+          bool page = true;
           if (k.row != kNoRow) {
-            if (page_ok(p.c.map, k.page))
+            page = page_ok(p.c.map, k.page);
+            if (page)
               row = static_cast<uint32_t>(k.page) * p.page_rows + k.row;
             else
               atomicExch(p.error_flag, PHEW_ERR_INVALID);
           }
           if (p.eights)
-            ring.template issue<true>(st_in, row);
+            ring.template issue<true>(st_in, row, page);
           else
-            ring.template issue<false>(st_in, row);
+            ring.template issue<false>(st_in, row, page);
           st_in = st_in + 1 == S::STAGES ? 0 : st_in + 1;
           --left;
         } else {

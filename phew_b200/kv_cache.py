@@ -314,7 +314,9 @@ def quantized_cache_attention(q, cache: QuantizedKVCache, lengths, *, block_tabl
     tokens included; ``counts`` (int32 ``[batch]``, default all) its query
     tokens in a padded batch.  ``mask`` None, or ``"causal"``: the last query
     token sits at the sequence's last key.  Rows that see no key, and rows
-    behind ``counts``, are zero.
+    behind ``counts``, are zero.  A block table entry that is no page of the
+    cache stands for keys and values of zero, a length past a sequence's pages
+    ends at them; both are reported by ``ops.check_device_errors``.
     """
     if mask is not None and not (isinstance(mask, str) and mask == "causal"):
         raise ValueError(f"quantized_cache_attention: mask must be None or 'causal', got {mask!r}")

@@ -237,3 +237,31 @@ def test_large_values_whose_weight_fades(mx, dtype, heads, tokens):
     plan.cache = mx.fast.QuantizedKVCache(*sides, group_size=64, bits=4)
     q = torch.ones((1, heads, tokens, 128), device="cuda").to(DTYPES[dtype])
     attend_closely(mx, plan, q, scale=0.5, sharp=False)
+
+
+# --- pages that are none of the cache's ------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("page,head_dim,group", [(16, 128, 64), (8, 64, 32), (40, 256, 32), (3, 128, 128)])
+@pytest.mark.parametrize("tokens", [1, 40, 100, 300])
+@pytest.mark.parametrize("entry", [-1, 1 << 30])
+def test_keys_of_a_bad_page_count_as_zeros(mx, dtype, page, head_dim, group, tokens, entry):
+    """Nothing of the cache's first page, or any other, reaches the output."""
+    from phew_b200._native import PhewError
+    from phew_b200.ops import check_device_errors
+
+    plan = Plan(mx, [170], kv_heads=2, head_dim=head_dim, group=group, page=page, dtype=dtype, spare=1)
+    free = (set(range(plan.cache.pages)) - set(plan.table[0].tolist())).pop()
+    for part in (*plan.cache.keys, *plan.cache.values):
+        part._t[free].zero_()
+    q = rand((1, 4, tokens, head_dim), dtype, 10)
+    run = lambda: mx.fast.quantized_cache_attention(  # noqa: E731
+        mx.array(q), plan.cache, [170], block_table=mx.array(plan.table), scale=head_dim ** -0.5, mask="causal")._t
+    plan.table[0, 1] = free
+    want = run()
+    plan.table[0, 1] = entry
+    got = run()
+    with pytest.raises(PhewError, match="outside a sequence's pages"):
+        check_device_errors()
+    assert torch.equal(got, want)
