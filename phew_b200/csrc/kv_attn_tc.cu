@@ -293,8 +293,10 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
     }
   } else if (DENSE && warp == 1) {
     // ---------------- TMA ----------------
-    if (lane == 0 && n_max > 0) {
-      asm volatile("griddepcontrol.wait;" ::: "memory");  // the expanded keys and values are there
+    if (lane == 0) {
+      // the expanded keys and values are there.  Every CTA waits, one without keys too: a grid of which none did
+      // could end before the expansion, and what follows it on the stream would find that still writing.
+      asm volatile("griddepcontrol.wait;" ::: "memory");
       const int first = bh * p.rows + j0 * kTcTile;
       auto load = [&](const CUtensorMap* tm, uint64_t* bar, uint8_t* dst, int row) {
         mbar_expect_tx(bar, S::TILE_BYTES);

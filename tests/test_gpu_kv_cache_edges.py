@@ -265,3 +265,36 @@ def test_keys_of_a_bad_page_count_as_zeros(mx, dtype, page, head_dim, group, tok
     with pytest.raises(PhewError, match="outside a sequence's pages"):
         check_device_errors()
     assert torch.equal(got, want)
+
+
+# --- nothing asked ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_no_queries_over_long_histories(mx, captured):
+    """A chunk step in which no sequence has a token: zeros, and the scratch is free for what comes next."""
+    B, tokens = 8, 300
+    plan = Plan(mx, [20000] * B, kv_heads=2, page=256)
+    q, table = mx.array(rand((B, 8, tokens, 128), "bfloat16", 13)), mx.array(plan.table)
+    n, counts = mx.array(ints(plan.lengths)), mx.array(ints([0] * B))
+    scratch = 2 * B * 2 * 20096 * 128  # 16-bit values of both sides
+
+    def step():
+        o = mx.fast.quantized_cache_attention(q, plan.cache, n, block_table=table, counts=counts, scale=0.1, mask="causal")._t
+        return o, [torch.full((scratch // 2,), 3.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+
+    step()
+    torch.cuda.synchronize()
+    replay = None
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        replay = graph.replay
+    for _ in range(10):
+        if replay:
+            replay()
+        else:
+            out = step()
+        o, after = out
+        assert not o.any() and all(bool((a == 3.0).all()) for a in after)
