@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import threading
 
 import torch
 
@@ -19,16 +20,26 @@ from . import dtypes as dt
 from .mx import core
 
 _error_flags: dict[int, torch.Tensor] = {}
+_error_flags_lock = threading.Lock()
 _Strides = ctypes.c_int64 * 3
 
 
 def cache_error_flag(device: torch.device) -> torch.Tensor:
     """Two device ints (0 = clean): [0] set when a position or a page lies
-    outside the cache, [1] when a bounded wait ran out."""
+    outside the cache, [1] when a bounded wait ran out.  One pair to a device,
+    made once, and zero on every stream when it is returned."""
     f = _error_flags.get(device.index)
     if f is None:
-        f = torch.zeros(2, dtype=torch.int32, device=device)
-        _error_flags[device.index] = f
+        with _error_flags_lock:
+            f = _error_flags.get(device.index)
+            if f is None:
+                with torch.cuda.device(device):
+                    if torch.cuda.is_current_stream_capturing():
+                        # (it would be the graph's memory, and zeroed by every replay)
+                        raise RuntimeError("QuantizedKVCache: a device's first cache cannot be made inside a capture")
+                    f = torch.zeros(2, dtype=torch.int32, device=device)
+                    torch.cuda.current_stream().synchronize()
+                _error_flags[device.index] = f
     return f
 
 
@@ -36,7 +47,7 @@ def check_cache_errors() -> None:
     """Raise if a kernel of the cache met a position outside a sequence's
     pages or a block table entry that is no page, or gave up a wait
     (synchronises)."""
-    for f in _error_flags.values():
+    for f in list(_error_flags.values()):
         code, waited = f.tolist()
         if code or waited:
             f.zero_()
@@ -59,11 +70,12 @@ class QuantizedKVCache:
     ``bits`` 4 or 8 (attention reads 4), ``head_dim`` 64, 128 or 256,
     ``group_size`` 32, 64 or 128.  The arrays are the caller's: ``update``
     writes into them.  A block table ``[batch, columns]`` names each sequence's
-    pages in order; without one page b belongs to sequence b.
+    pages in order; without one page b belongs to sequence b.  A device's first
+    cache synchronises with it once, and cannot be made inside a graph capture.
     """
 
     __slots__ = ("keys", "values", "pages", "kv_heads", "page_size", "head_dim", "group_size", "bits",
-                 "dtype", "device", "_torch_dtype", "_unit", "_struct", "_flag")
+                 "dtype", "device", "_torch_dtype", "_unit", "_struct", "_flag", "_flag_tensor")
 
     def __init__(self, keys, values, *, group_size: int = 64, bits: int = 4) -> None:
         if len(keys) != 3 or len(values) != 3:
@@ -110,7 +122,8 @@ class QuantizedKVCache:
         self._struct = _native.KVCache(*(ctypes.c_void_p(a._t.data_ptr()) for a in parts), self.pages,
                                        self.page_size, self.kv_heads, dim, g, nb, self.dtype.code)
         self._torch_dtype, self._unit = self.dtype.torch, 16 // self.dtype.size
-        self._flag = cache_error_flag(self.device).data_ptr()
+        self._flag_tensor = cache_error_flag(self.device)  # (kernels get its address: it lives as long as the cache)
+        self._flag = self._flag_tensor.data_ptr()
 
     @classmethod
     def zeros(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, dtype="bfloat16", *,

@@ -298,3 +298,54 @@ def test_no_queries_over_long_histories(mx, captured):
             out = step()
         o, after = out
         assert not o.any() and all(bool((a == 3.0).all()) for a in after)
+
+
+# --- the first cache of a device -----------------------------------------------------------------
+
+
+def test_first_cache_inside_a_capture_is_refused(mx, monkeypatch):
+    """Its error flag would be the graph's memory, zeroed by every replay.  Later caches may be made there."""
+    from phew_b200 import kv_cache
+
+    plan = Plan(mx, [40], page=16)
+    q, n, table = mx.array(rand((1, 4, 1, 128), "bfloat16", 14)), mx.array(ints([40])), mx.array(plan.table)
+
+    def attend():
+        cache = mx.fast.QuantizedKVCache(plan.cache.keys, plan.cache.values)
+        return mx.fast.quantized_cache_attention(q, cache, n, block_table=table, scale=0.1)._t
+
+    want = attend().clone()
+    torch.cuda.synchronize()
+    with monkeypatch.context() as m:
+        m.setattr(kv_cache, "_error_flags", {})
+        with pytest.raises(RuntimeError, match="inside a capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                attend()
+        assert not kv_cache._error_flags
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = attend()
+    graph.replay()
+    assert torch.equal(o, want)
+
+
+def test_caches_made_by_threads_report_to_one_flag(mx, monkeypatch):
+    import threading
+
+    from phew_b200 import kv_cache
+
+    monkeypatch.setattr(kv_cache, "_error_flags", {})
+    plan, caches, start = Plan(mx, [40]), [], threading.Barrier(8)
+    kv_cache._error_flags.clear()
+
+    def make():
+        start.wait()
+        caches.append(mx.fast.QuantizedKVCache(plan.cache.keys, plan.cache.values))
+
+    threads = [threading.Thread(target=make) for _ in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    flag = kv_cache._error_flags[plan.cache.device.index]
+    assert len(caches) == 8 and all(c._flag == flag.data_ptr() for c in caches) and not flag.any()

@@ -1,9 +1,13 @@
 """Host side of the quantised cache on the CPU: pending arrays that read what
-an op is about to write."""
+an op is about to write, the error flag that all of a device's caches share."""
 
 from __future__ import annotations
 
+import contextlib
 import gc
+import threading
+import time
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -65,3 +69,57 @@ def test_deferred_nodes_are_forgotten_when_they_die(core):
     finally:
         core.trace_exit()
     assert not core.order
+
+
+@pytest.fixture()
+def flags(monkeypatch):
+    """kv_cache with no flag made yet; tensors lie on the CPU and take a while."""
+    from phew_b200 import kv_cache
+
+    made, zeros = [], torch.zeros
+
+    def slow_zeros(*a, device=None, **k):
+        time.sleep(0.02)
+        made.append(zeros(*a, **k))
+        return made[-1]
+
+    events = []
+    stream = SimpleNamespace(synchronize=lambda: events.append("synchronised"))
+    state = SimpleNamespace(made=made, events=events, capturing=False, get=kv_cache.cache_error_flag, module=kv_cache)
+    monkeypatch.setattr(kv_cache, "_error_flags", {})
+    monkeypatch.setattr(torch, "zeros", slow_zeros)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: stream)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state.capturing)
+    return state
+
+
+def test_threads_share_one_error_flag(flags):
+    """A second flag would be freed while a cache still hands its address to kernels."""
+    device, got, start = torch.device("cuda", 0), [], threading.Barrier(8)
+
+    def make():
+        start.wait()
+        got.append(flags.get(device))
+
+    threads = [threading.Thread(target=make) for _ in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 8 and all(f is got[0] for f in got)
+    assert len(flags.made) == 1 and flags.events == ["synchronised"]
+    assert flags.module._error_flags == {0: got[0]}
+    other = flags.get(torch.device("cuda", 1))
+    assert other is not got[0] and flags.get(torch.device("cuda", 1)) is other
+
+
+def test_no_error_flag_is_made_inside_a_capture(flags):
+    flags.capturing = True
+    with pytest.raises(RuntimeError, match="inside a capture"):
+        flags.get(torch.device("cuda", 0))
+    assert not flags.made and not flags.module._error_flags
+    flags.capturing = False
+    f = flags.get(torch.device("cuda", 0))
+    flags.capturing = True
+    assert flags.get(torch.device("cuda", 0)) is f
