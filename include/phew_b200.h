@@ -347,7 +347,8 @@ typedef struct phew_kv_cache {
 /* Quantises tokens [0, counts[b]) of k[b], v[b] ([batch][kv_heads][tokens]
  * [head_dim] views of the cache's dtype; strides {token, head, batch} in
  * elements, multiples of 16 bytes) into positions offsets[b] + token, with the
- * arithmetic of phew_quantize; counts NULL = all tokens.  Other rows of the
+ * arithmetic of phew_quantize, but for a group that holds a NaN: its scale
+ * and bias are NaN and its codes 0.  counts NULL = all tokens.  Other rows of the
  * cache stay as they were.  With k_out / v_out (contiguous) it also writes
  * the values the cache now stands for (phew_dequantize's), zero for tokens
  * behind counts[b].  Two tokens of one call must not name the same row.

@@ -11,7 +11,9 @@
 //   code  = clamp(rint((x - bias) / scale), 0, 2^bits - 1)       (fp32, IEEE divide)
 //   value = T(scale * code + bias)                               (fp32 fma)
 // so a written row is bit for bit what phew_quantize gives for it and a read
-// row what phew_dequantize gives.
+// row what phew_dequantize gives.  But a group that holds a NaN gets NaN for
+// scale and bias (codes 0), so that it reads back as NaN, where phew_quantize
+// passes over it.
 #include <type_traits>
 
 #include "common.cuh"
@@ -98,16 +100,16 @@ template <typename T> __device__ __forceinline__ void set_pair(Eight<T>& e, int 
   }
 }
 
-// Smallest and largest of the eight.  The 16-bit types keep (min, -max) as one
+// Smallest and largest of the eight, NaN if one of them is.  The 16-bit types keep (min, -max) as one
 // packed pair, so a step across lanes is one shuffle and one packed minimum.
 template <typename T> struct Range {
   uint32_t p;
   static __device__ __forceinline__ uint32_t min_of(uint32_t a, uint32_t b) {
     uint32_t d;
     if constexpr (std::is_same<T, bf16>::value)
-      asm("min.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+      asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     else
-      asm("min.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+      asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
   }
   __device__ __forceinline__ void of(const Eight<T>& e) {
@@ -126,23 +128,33 @@ template <typename T> struct Range {
 };
 template <> struct Range<float> {
   float a, b;
+  static __device__ __forceinline__ float min_of(float x, float y) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(x), "f"(y));
+    return d;
+  }
+  static __device__ __forceinline__ float max_of(float x, float y) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(x), "f"(y));
+    return d;
+  }
   __device__ __forceinline__ void of(const Eight<float>& e) {
     a = b = __uint_as_float(e.w[0]);
 #pragma unroll
     for (int i = 1; i < 8; ++i) {
-      a = fminf(a, __uint_as_float(e.w[i]));
-      b = fmaxf(b, __uint_as_float(e.w[i]));
+      a = min_of(a, __uint_as_float(e.w[i]));
+      b = max_of(b, __uint_as_float(e.w[i]));
     }
   }
   __device__ __forceinline__ void with(const Range& o) {
-    a = fminf(a, o.a);
-    b = fmaxf(b, o.b);
+    a = min_of(a, o.a);
+    b = max_of(b, o.b);
   }
   __device__ __forceinline__ void across(int lanes) {
 #pragma unroll
     for (int o = lanes / 2; o > 0; o >>= 1) {
-      a = fminf(a, __shfl_xor_sync(0xffffffffu, a, o));
-      b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, o));
+      a = min_of(a, __shfl_xor_sync(0xffffffffu, a, o));
+      b = max_of(b, __shfl_xor_sync(0xffffffffu, b, o));
     }
   }
   __device__ __forceinline__ float lo() const { return a; }
@@ -217,7 +229,7 @@ template <typename T, int BITS> __device__ __forceinline__ Affine affine_of(cons
   float q = d * part;
   q = fmaf(fmaf(-top, q, d), part, q);
   if (!(d < 1e38f)) q = __fdiv_rn(d, top);
-  a.sc = round_to<T>(fmaxf(q, 1e-8f));
+  a.sc = lo == lo ? round_to<T>(fmaxf(q, 1e-8f)) : lo;
   a.bi = lo;  // a value of type T
   if (sizeof(T) == 2) {
     // one Newton step from one unit in the last place: the rounded reciprocal of a mantissa of 8 or 11 bits

@@ -262,7 +262,8 @@ def quantized_cache_update(cache: QuantizedKVCache, k, v, offsets, *, block_tabl
 
     ``counts`` (int32 ``[batch]``, default all) limits a padded batch to its
     first tokens; every other row of the cache stays as it was.  A row's codes,
-    scales and biases are those of ``mx.quantize`` on it.  With ``fetch`` the
+    scales and biases are those of ``mx.quantize`` on it, but a group that holds
+    a NaN reads back as NaN (scale and bias NaN, codes 0).  With ``fetch`` the
     values that the new tokens now stand for are returned as ``(k, v)`` like
     the inputs (``mx.dequantize``'s, zero behind ``counts``), e.g. for a prompt's
     own attention.  Two tokens of one call must not land in the same row.

@@ -267,6 +267,40 @@ def test_keys_of_a_bad_page_count_as_zeros(mx, dtype, page, head_dim, group, tok
     assert torch.equal(got, want)
 
 
+# --- writing what is no number ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("bits,head_dim,group", [(4, 128, 64), (8, 64, 32), (4, 256, 128), (8, 128, 128)])
+def test_update_keeps_what_is_no_number(mx, dtype, bits, head_dim, group):
+    """A group with a NaN reads back as NaN; its neighbours, and infinities, are mx.quantize's."""
+    x = rand((1, 2, 9, head_dim), dtype, 11)
+    nan = torch.zeros((1, 2, 9, head_dim // group), dtype=torch.bool, device="cuda")
+    for head, row, col, bad in [(0, 0, 0, float("nan")), (0, 3, head_dim - 1, -float("nan")), (1, 4, group - 1, float("nan")),
+                                (1, 1, 3, float("inf")), (1, 2, 17, -float("inf"))]:
+        x[0, head, row, col] = bad
+        nan[0, head, row, col // group] |= bad != bad
+    x[0, 1, 8] = float("nan")
+    nan[0, 1, 8] = True
+    x[0, 0, 7] = float("inf")
+    cache = mx.fast.QuantizedKVCache.zeros(1, 2, 9, head_dim, dtype, group_size=group, bits=bits)
+    got = mx.fast.quantized_cache_update(cache, mx.array(x), mx.array(-x), [0], fetch=True)
+    for y, side, dense in ((x, cache.keys, got[0]._t), (-x, cache.values, got[1]._t)):
+        want = [a._t for a in mx.quantize(mx.array(y), group_size=group, bits=bits)]
+        assert torch.isnan(side[1]._t[nan]).all() and torch.isnan(side[2]._t[nan]).all()
+        for a, w in zip(side[1:], want[1:]):
+            assert torch.equal(a._t[~nan].view(torch.uint8), w[~nan].view(torch.uint8))
+        codes = lambda t: t.view(torch.int32).unflatten(-1, (head_dim // group, -1))  # noqa: E731
+        assert torch.equal(codes(side[0]._t)[~nan], codes(want[0])[~nan])
+        assert not codes(side[0]._t)[nan].any()
+        plain = mx.dequantize(*(mx.array(a) for a in want), group_size=group, bits=bits)._t.unflatten(-1, (-1, group))
+        read = mx.fast.quantized_cache_fetch(cache, [9])[0 if y is x else 1]._t
+        for v in (dense, read):
+            v = v.unflatten(-1, (-1, group))
+            assert torch.isnan(v[nan]).all()
+            assert torch.equal(v[~nan].nan_to_num(7.0), plain[~nan].nan_to_num(7.0))
+
+
 # --- nothing asked ---------------------------------------------------------------------------
 
 
