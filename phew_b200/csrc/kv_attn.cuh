@@ -611,15 +611,14 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
 #pragma unroll
           for (int i = 0; i < WPT; ++i)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) sum[g] += v[g * WPT + i][k];
+            for (int k = 0; k < 8; ++k) sum[g] += v[g * WPT + i][k] *= up;  // (unscaled, a sum may pass fp32's range)
           sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
           sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
-          sum[g] *= up;
         }
 #pragma unroll
         for (int w = 0; w < WT; ++w) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[w][k] *= k & 1 ? up * 0.0625f : up;  // odd codes count sixteenfold
+          for (int k = 1; k < 8; k += 2) v[w][k] *= 0.0625f;  // odd codes count sixteenfold
 #pragma unroll
           for (int t = 0; t < TERMS; ++t)
 #pragma unroll

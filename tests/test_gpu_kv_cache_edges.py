@@ -301,6 +301,21 @@ def test_update_keeps_what_is_no_number(mx, dtype, bits, head_dim, group):
             assert torch.equal(v[~nan].nan_to_num(7.0), plain[~nan].nan_to_num(7.0))
 
 
+# --- large queries -------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("tokens", [1, 3, 100])
+def test_queries_whose_sum_passes_the_range(mx, dtype, tokens):
+    """Finite scores of queries of up to 2^126: their sum over the head dimension alone is past 32 bits."""
+    plan = Plan(mx, [300], dtype=dtype, kv_heads=1)
+    for part in plan.cache.keys[1:]:
+        part._t.mul_(2.0 ** -20)
+    q = rand((1, 2, tokens, 128), dtype, 12).abs()
+    for up in (1.0, 2.0 ** 124):
+        attend_closely(mx, plan, q * up, scale=2.0 ** 17 / up)
+
+
 # --- nothing asked ---------------------------------------------------------------------------
 
 
@@ -337,6 +352,7 @@ def test_no_queries_over_long_histories(mx, captured):
 # --- the first cache of a device -----------------------------------------------------------------
 
 
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
 def test_first_cache_inside_a_capture_is_refused(mx, monkeypatch):
     """Its error flag would be the graph's memory, zeroed by every replay.  Later caches may be made there."""
     from phew_b200 import kv_cache
