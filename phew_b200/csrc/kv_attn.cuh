@@ -684,9 +684,11 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
       const int my_key = key_of_slot(r8);
 
       // Factors of the rows and groups whose weights times scales pass f16's range in this tile, are their first, or
-      // are taken against a new m (`moved`, a bit to a row): what was large before may be nothing now.  The tile's largest scale goes to [2^12, 2^13), unless that left less than 2^-2 of the row's
+      // are taken against a new m (a row's moved by `moved`, 0 where it stayed): what was large before may be nothing
+      // now, and a factor may grow again, by 2^60 more than the sums have shrunk at most (of 2^31 keys they are below
+      // 2^58 before).  The tile's largest scale goes to [2^12, 2^13), unless that left less than 2^-2 of the row's
       // largest weight times scale: then the scales that pass the range have next to no weight.
-      auto fit = [&](float (*s)[NT][4], const float* sv, uint32_t moved) {
+      auto fit = [&](float (*s)[NT][4], const float* sv, const float (*moved)[2]) {
         uint32_t top[NG];
         float most[NG];
 #pragma unroll
@@ -722,21 +724,24 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
               float f = part[g][cc];
 #pragma unroll
               for (int o = 4; o < 32; o <<= 1) f = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, o));
-              float by = 1.f;
-              const bool again = up[g][cc] == kNoFactor || (moved >> (2 * nt + cc) & 1);
+              float by = 1.f, rest = 1.f;  // two halves of the step: it may be 2^183
+              const bool again = up[g][cc] == kNoFactor || moved[nt][cc] != 0.f;
               if (f * up[g][cc] > kF16Most || (again && f > 0.f)) {
                 const int e = max(266 - static_cast<int>(top[g] >> 23),
                                   252 - static_cast<int>(__float_as_uint(f) >> 23));
-                const float to = __int_as_float(min(e, 195) << 23);  // (at most kNoFactor)
-                by = to / up[g][cc];
-                up[g][cc] = to;
+                const int from = static_cast<int>(__float_as_uint(up[g][cc]) >> 23);
+                const int most_step = 60 + static_cast<int>(fminf(fmaxf(moved[nt][cc], 0.f), 200.f));
+                const int step = min(min(e, 195) - from, most_step);  // (195: kNoFactor)
+                by = __int_as_float(((step >> 1) + 127) << 23);
+                rest = __int_as_float((step - (step >> 1) + 127) << 23);
+                up[g][cc] = __int_as_float((from + step) << 23);
               }
               most[g] = fmaxf(most[g], up[g][cc]);
-              wsum[nt][cc][g] *= by;
+              wsum[nt][cc][g] = wsum[nt][cc][g] * by * rest;
 #pragma unroll
               for (int i = g * G / 16; i < (g + 1) * G / 16; ++i) {
-                acc[nt][i][cc] *= by;
-                acc[nt][i][2 + cc] *= by;
+                acc[nt][i][cc] = acc[nt][i][cc] * by * rest;
+                acc[nt][i][2 + cc] = acc[nt][i][2 + cc] * by * rest;
               }
             }
           __syncwarp();
@@ -800,7 +805,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
         }
         // ---- m: moved only when a score passes it; weights stay below 1 ----
         bool grow = false;
-        uint32_t moved = 0;
+        float moved[NT][2] = {};
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -812,7 +817,8 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
               if (EDGE && key0 + kb * 16 + (k >> 1) * 8 + my_key >= lim[nt][k & 1]) y = -INFINITY;
               grow = grow || y > pass[nt][k & 1];
             }
-        if (__any_sync(0xffffffffu, grow)) {
+        grow = __any_sync(0xffffffffu, grow);
+        if (grow) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -824,7 +830,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
               const float by = move ? top + kGrow : 0.f;
               const float alpha = exp2_fast(fminf(-by, 0.f));  // (a row's first keys find nothing to scale)
               if (move) pass[nt][cc] = 0.f;
-              if (move) moved |= 1u << (2 * nt + cc);
+              moved[nt][cc] = by;
               m[nt][cc] += by;
               l[nt][cc] *= alpha;
 #pragma unroll
@@ -858,7 +864,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
           __syncwarp();
           ring.share(sv, zv);
           __syncwarp();
-          if (__any_sync(0xffffffffu, over || moved)) fit(s, sv, moved);
+          if (__any_sync(0xffffffffu, over) || grow) fit(s, sv, moved);
         }
         // ---- weights, their sums, and the second product ----
 #pragma unroll

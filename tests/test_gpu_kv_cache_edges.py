@@ -61,6 +61,8 @@ def bounds(plan, q, counts, scale, causal, tensor_core=False):
       * scores off by e: e N.  Products of bare key codes are cut at 2^-14 of the largest query times a code's
         step: 6 sqrt(D / 3) 2^-14 max|q| max s scale at six sigma; of codes less 8, and in f32's sums and
         queries of 22 bits, 2^-19 |q| |k| scale by Cauchy and Schwarz
+      * weights in 32 bits: the largest is 2^-8 or more, and 2^(s - m) below fp32's 2^-126 is zero, so keys of less
+        than 2^-118 of the largest weight may count as nothing: sum w_j |v_j| over those
       * f16's smallest steps: 2^-23 of the largest weight times scale, for each key: sqrt(keys) of that
       * 32-bit sums: 2^-21 of the sum of the magnitudes, 2^-19 where bare codes pile up over 32 additions."""
     u = 2.0 ** {"bfloat16": -8, "float16": -11, "float32": -24}[plan.dtype]
@@ -105,7 +107,8 @@ def bounds(plan, q, counts, scale, causal, tensor_core=False):
             piles = w @ (8 * step + (vg.abs().amax(-1) if tensor_core else centre[..., 0].abs()))
             og = o.unflatten(-1, (ng, G)).norm(dim=-1)
             out[b, head, :c] = o
-            floor = 2.0 ** -25 * G ** 0.5 if plan.dtype == "float16" else 0.0
+            none = w * (w < 2.0 ** -118 * w.amax(-1, keepdim=True))
+            floor = none @ vg.norm(dim=-1) + (2.0 ** -25 * G ** 0.5 if plan.dtype == "float16" else 0.0)
             tol[b, head, :c] = (u * og + floor + (1.5 * h + e) * N + n ** 0.5 * 2.0 ** -23 * 8 * G ** 0.5 * top
                                 + 2.0 ** (-19 if bare else -21) * G ** 0.5 * piles)
             lost = w.clone()
@@ -120,14 +123,17 @@ def groups_err(got, want, group):
     return (got.double() - want).unflatten(-1, (-1, group)).norm(dim=-1)
 
 
-def attend_closely(mx, plan, q, counts=None, causal=False, scale=None, sharp=True):
-    """Attention within the bound above, and where `sharp`, that the bound would notice a lost tile or zeros."""
+def attend_closely(mx, plan, q, counts=None, causal=False, scale=None, sharp=True, copies=1):
+    """Attention within the bound above, and where `sharp`, that the bound would notice a lost tile or zeros.
+    `copies` of the batch in one call: enough of them leave a warp whole sequences instead of a tile or two."""
     scale = plan.head_dim ** -0.5 if scale is None else scale
     rows = q.shape[2] * (q.shape[1] // plan.kv_heads)
     tensor_core = plan.dtype != "float32" and rows > 64 and scale > 0
     o = mx.fast.quantized_cache_attention(
-        mx.array(q), plan.cache, mx.array(ints(plan.lengths)), block_table=mx.array(plan.table),
-        counts=None if counts is None else mx.array(ints(counts)), scale=scale, mask="causal" if causal else None)._t
+        mx.array(q.repeat(copies, 1, 1, 1)), plan.cache, mx.array(ints(plan.lengths * copies)),
+        block_table=mx.array(plan.table.repeat(copies, 1)),
+        counts=None if counts is None else mx.array(ints(counts * copies)), scale=scale,
+        mask="causal" if causal else None)._t.unflatten(0, (copies, -1))
     want, tol, tile = bounds(plan, q, counts, scale, causal, tensor_core)
     if sharp:
         n = torch.tensor(plan.lengths, device="cuda")[:, None, None, None].expand_as(tol)
@@ -138,7 +144,7 @@ def attend_closely(mx, plan, q, counts=None, causal=False, scale=None, sharp=Tru
     err = groups_err(o, want, plan.group)
     worst = float((err / tol.clamp_min(1e-300)).nan_to_num(torch.inf).masked_fill((tol == 0) & (err == 0), 0.0).max())
     assert worst <= 1.0, f"{worst:.3g} of the bound"
-    return o
+    return o[0]
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
@@ -190,10 +196,11 @@ def test_groups_of_different_magnitude(mx, dtype, bits, head_dim, group, heads):
     attend_closely(mx, plan, rand((2, heads, 1, head_dim), dtype, 6))
 
 
+@pytest.mark.parametrize("copies", [1, 1500])
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("heads,tokens", [(2, 1), (8, 2), (16, 3), (30, 3)])
 @pytest.mark.parametrize("at", [0, 5, 700])
-def test_a_large_value_of_no_weight(mx, dtype, heads, tokens, at):
+def test_a_large_value_of_no_weight(mx, dtype, heads, tokens, at, copies):
     """A key that no query attends to may have values of any size, wherever a warp meets it."""
     plan = Plan(mx, [1200], kv_heads=2, dtype=dtype, page=1200, spare=0)
     large, small = spread(dtype, 36)
@@ -203,12 +210,13 @@ def test_a_large_value_of_no_weight(mx, dtype, heads, tokens, at):
     v[:, :, at] *= large / small
     sides = [mx.quantize(mx.array(x), group_size=64, bits=4) for x in plan.dense]
     plan.cache = mx.fast.QuantizedKVCache(*sides, group_size=64, bits=4)
-    attend_closely(mx, plan, rand((1, heads, tokens, 128), dtype, 8).abs(), scale=0.125)
+    attend_closely(mx, plan, rand((1, heads, tokens, 128), dtype, 8).abs(), scale=0.125, copies=copies)
 
 
+@pytest.mark.parametrize("copies", [1, 1500])
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("heads,kv_heads,tokens", [(2, 2, 3), (4, 2, 7), (2, 1, 30), (4, 2, 80)])
-def test_a_large_value_that_later_tokens_alone_see(mx, dtype, heads, kv_heads, tokens):
+def test_a_large_value_that_later_tokens_alone_see(mx, dtype, heads, kv_heads, tokens, copies):
     plan = Plan(mx, [200], kv_heads=kv_heads, dtype=dtype, page=200, spare=0)
     large, small = spread(dtype, 60)
     v = plan.dense[1]
@@ -217,15 +225,16 @@ def test_a_large_value_that_later_tokens_alone_see(mx, dtype, heads, kv_heads, t
     sides = [mx.quantize(mx.array(x), group_size=64, bits=4) for x in plan.dense]
     plan.cache = mx.fast.QuantizedKVCache(*sides, group_size=64, bits=4)
     q = rand((1, heads, tokens, 128), dtype, 9)
-    o = attend_closely(mx, plan, q, causal=True, sharp=False)
+    o = attend_closely(mx, plan, q, causal=True, sharp=False, copies=copies)
     plan.lengths = [199]  # without that key the other rows have a bound of their own
     want, tol, _ = bounds(plan, q[:, :, :-1], None, 128 ** -0.5, True, dtype != "float32" and tokens * heads // kv_heads > 64)
     assert bool((groups_err(o[:, :, :-1], want, 64) <= tol).all())
 
 
+@pytest.mark.parametrize("copies", [1, 1500])
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("heads,tokens", [(2, 1), (8, 2), (30, 3)])
-def test_large_values_whose_weight_fades(mx, dtype, heads, tokens):
+def test_large_values_whose_weight_fades(mx, dtype, heads, tokens, copies):
     """Scores rise along the keys; the first keys, whose values are large, weigh nothing in the end."""
     plan = Plan(mx, [700], kv_heads=2, dtype=dtype, page=700, spare=0)
     large, small = spread(dtype, 36)
@@ -236,7 +245,27 @@ def test_large_values_whose_weight_fades(mx, dtype, heads, tokens):
     sides = [mx.quantize(mx.array(x), group_size=64, bits=4) for x in plan.dense]
     plan.cache = mx.fast.QuantizedKVCache(*sides, group_size=64, bits=4)
     q = torch.ones((1, heads, tokens, 128), device="cuda").to(DTYPES[dtype])
-    attend_closely(mx, plan, q, scale=0.5, sharp=False)
+    attend_closely(mx, plan, q, scale=0.5, sharp=False, copies=copies)
+
+
+@pytest.mark.parametrize("copies", [1, 1500])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("heads,tokens", [(2, 1), (8, 2), (30, 3)])
+@pytest.mark.parametrize("drop", [20.0, 100.0, 400.0])
+def test_values_of_the_whole_range(mx, dtype, heads, tokens, drop, copies):
+    """The first 64 keys' values are 2^140 of the others', with scores `drop` below theirs: by 2^29 of their weight,
+    and they decide the output, by 2^144, and both count, by 2^577, and they are nothing."""
+    plan = Plan(mx, [700], kv_heads=2, dtype=dtype, page=700, spare=0)
+    k, v = plan.dense
+    k *= 0.02
+    k[:, :, :64] -= drop / 64
+    v *= 2.0 ** -20
+    v[:, :, :64] *= 2.0 ** 70
+    v[:, :, :64] *= 2.0 ** 70
+    sides = [mx.quantize(mx.array(x), group_size=64, bits=4) for x in plan.dense]
+    plan.cache = mx.fast.QuantizedKVCache(*sides, group_size=64, bits=4)
+    q = torch.ones((1, heads, tokens, 128), device="cuda").to(DTYPES[dtype])
+    attend_closely(mx, plan, q, scale=0.5, sharp=False, copies=copies)
 
 
 # --- pages that are none of the cache's ------------------------------------------------------
