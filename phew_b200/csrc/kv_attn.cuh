@@ -603,7 +603,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
         // the row's largest magnitude to [2^14, 2^15)
         const uint32_t e = max(__float_as_uint(top) >> 23, 20u);
         const float up = __uint_as_float((268u - e) << 23);
-        const float row_unit = p.scale_log2 * __uint_as_float((e - 14u) << 23);  // scale / up
+        const float row_unit = p.scale_log2 * 0x1p24f * __uint_as_float((e - 14u) << 23);  // 2^24 scale / up
         float sum[NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -989,8 +989,10 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attn_kernel(const AttnPa
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
             if (KC) zk[g] = fmaf(8.f, sk[g], zk[g]);
-            // (an infinite key would give scores of either infinity: no number, as its products are)
-            sk[g] = fmaf(sk[g], KC ? 1.f : 0x1p24f, fmaf(0.f, sk[g], 0.f * zk[g]));
+            // (2^-24 of a score, so that a large key's bias times a query's sum of 2^21 stays in range; an infinite
+            // key would give scores of either infinity: no number, as its products are)
+            sk[g] = fmaf(sk[g], KC ? 0x1p-24f : 1.f, fmaf(0.f, sk[g], 0.f * zk[g]));
+            zk[g] *= 0x1p-24f;
           }
           ring.share(sk, zk);
         }

@@ -330,7 +330,7 @@ def test_update_keeps_what_is_no_number(mx, dtype, bits, head_dim, group):
             assert torch.equal(v[~nan].nan_to_num(7.0), plain[~nan].nan_to_num(7.0))
 
 
-# --- large queries -------------------------------------------------------------------------------
+# --- large queries and keys -------------------------------------------------------------------------------
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
@@ -343,6 +343,17 @@ def test_queries_whose_sum_passes_the_range(mx, dtype, tokens):
     q = rand((1, 2, tokens, 128), dtype, 12).abs()
     for up in (1.0, 2.0 ** 124):
         attend_closely(mx, plan, q * up, scale=2.0 ** 17 / up)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("tokens", [1, 3, 100])
+@pytest.mark.parametrize("up", [2.0 ** 118, 2.0 ** -70])
+def test_large_and_small_keys(mx, dtype, tokens, up):
+    """Keys near the ends of the range, whose scores are finite."""
+    plan = Plan(mx, [300], dtype=dtype, kv_heads=1)
+    for part in plan.cache.keys[1:]:
+        part._t.mul_(up)
+    attend_closely(mx, plan, rand((1, 2, tokens, 128), dtype, 15), scale=0.1 / up)
 
 
 # --- nothing asked ---------------------------------------------------------------------------
