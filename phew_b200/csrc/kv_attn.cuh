@@ -1193,8 +1193,6 @@ template <typename S, typename T> int launch_attn(AttnParams p, void* workspace,
   const int64_t blocks = blocks_of<S>(static_cast<int64_t>(p.tokens) * p.per);
   const int64_t segments = p.batch * blocks * p.c.map.kv_heads;
   PHEW_REQUIRE(segments < (1ll << 31), "phew_kv_attention: too many query rows");
-  PHEW_REQUIRE((capacity(p.c.map) / kTile + kBegin + 1) * p.c.map.kv_heads < (1ll << 32),
-               "phew_kv_attention: too many tokens for a sequence");
   p.blocks = static_cast<int>(blocks);
   p.by_blocks = fast_div(static_cast<uint32_t>(blocks));
   const int page = p.c.map.page_size;

@@ -75,7 +75,7 @@ class QuantizedKVCache:
     """
 
     __slots__ = ("keys", "values", "pages", "kv_heads", "page_size", "head_dim", "group_size", "bits",
-                 "dtype", "device", "_torch_dtype", "_unit", "_struct", "_flag", "_flag_tensor")
+                 "dtype", "device", "_torch_dtype", "_unit", "_struct", "_flag", "_flag_tensor", "_written")
 
     def __init__(self, keys, values, *, group_size: int = 64, bits: int = 4) -> None:
         if len(keys) != 3 or len(values) != 3:
@@ -116,6 +116,7 @@ class QuantizedKVCache:
         if codes.size == 0:
             raise ValueError("QuantizedKVCache: empty cache")
         self.keys, self.values = tuple(parts[:3]), tuple(parts[3:])
+        self._written = tuple(a._t for a in parts)  # what an update writes into
         self.pages, self.kv_heads, self.page_size = codes.shape[:3]
         self.head_dim, self.group_size, self.bits, self.dtype = dim, g, nb, scales.dtype
         self.device = codes._t.device
@@ -283,7 +284,7 @@ def quantized_cache_update(cache: QuantizedKVCache, k, v, offsets, *, block_tabl
     off = _ints(offsets, batch, "quantized_cache_update: offsets", cache)
     cnt = None if counts is None else _ints(counts, batch, "quantized_cache_update: counts", cache)
     keep, table, stride, columns = _table(block_table, batch, "quantized_cache_update", cache)
-    core.settle_readers([a._t for a in (*cache.keys, *cache.values)])
+    core.settle_readers(cache._written)
     out = None
     if fetch:
         out = (_empty_like(k), _empty_like(k))
