@@ -4,15 +4,33 @@
 // The rows of a cache head are r = token * per + head over its `per` query
 // heads; a CTA takes 256 of them (two 128-row tiles a and b) and walks the
 // keys in tiles of 128.  Bound by the chain score product - softmax - output
-// product of each tile, at about the rate of the exponentials.  Two forms:
+// product of each tile, at about the rate of the exponentials.
+//
+// Operands are f16 whatever the type: a tile's keys and its values (dense; those
+// of a quarter of it, 32 keys, where tiles are packed) in units of a power of
+// two, the largest magnitude at [2^14, 2^15); a query in units of its own,
+// exactly.  With ke, ve the units' exponents
+//   t_ij = c_i 2^ke (q'_i . k'_j) + ve,  p_ij = 2^(t_ij - m_i),  o_i = sum_j p_ij v'_j,
+//   l_i = sum_j p_ij 2^-ve
+// so units cost an element nothing: they enter with the constants of a tile.
+// m_i is 7 below a row's largest t when it moves, which leaves f16's smallest
+// weight 2^-31 of the largest.  Keys, values and weights are rounded to 11 bits
+// this way, for bf16 too (whose own 8 bits cost 3.2e-3 of an output's norm, 1.7e-3
+// of them its rounding).  Scores, maxima and sums are 32-bit.  Where magnitudes in
+// a tile lie further apart than f16 holds (Reach::odd) its rows are computed again
+// by plain_rows_kernel, in one thread's fp32 arithmetic: slow, for caches that no
+// model writes.  (A launch of its own, 2 us; at the end of this kernel its code
+// cost 10 to 20.)
+//
+// Two forms:
 //
 // Dense (kExpandBlocks row blocks or more, whose every CTA would expand the
-// same keys again): the cache is expanded once to 16 bits in scratch, as
-// phew_kv_fetch does, and tiles arrive by TMA.  One pass of HBM over the keys
-// against 0.5 us for each CTA and tile (measured: 256 CTAs x 56 tiles).
+// same keys again): the cache is expanded once to scratch, and tiles arrive by
+// TMA.  One pass of HBM over the keys against 0.5 us for each CTA and tile
+// (measured: 256 CTAs x 56 tiles).
 //
 // Packed (few row blocks): producer warps load packed rows (two units of 32
-// keys ahead, in registers), expand them as T(scale * code + bias) - two
+// keys ahead, in registers), expand them as f16(scale * code + bias) - two
 // instructions a value: a shift and a logic operation per pair of codes, an
 // exact subtraction, a packed multiply-add - and store them in the 128-byte
 // swizzle that the tensor core reads.  Those instructions take issue slots
@@ -33,7 +51,7 @@
 //                 K_0, V_0, K_1, ... in quarters of 32 keys, every third one to
 //                 a warp.  Both fill two-deep rings of K and V
 //   last 8 warps  softmax of tile a and b, one query row per thread; they also
-//                 load Q and write O
+//                 convert Q and write O
 //
 // TMEM: S_a, S_b, O_a, O_b of 128 columns each.  Heads of 256 have one query
 // tile to a CTA (O takes 256 columns), rings one deep and always the dense form.
@@ -45,14 +63,10 @@
 // Long caches with few rows are split: a CTA takes a share of the key tiles
 // and leaves partial sums, joined in a fixed order by the combine kernel.
 //
-// Keys and values are rounded to the type, as mx.dequantize gives them, and so
-// are the softmax weights, as in the dense attention: what the tensor core
-// takes.  Together 3.2e-3 to 3.7e-3 of an output's norm in bf16 (1.7e-3 is its
-// own rounding), 4e-4 in f16 (2.1e-4).  Scores, maxima and sums are 32-bit.
-//
 // Measured, causal, heads of 128 in bf16: two prompts of 4096 tokens on 32
-// heads, 334 us (823 TFLOP/s); the last 2048 of 8192 tokens on 32 heads over 8,
-// 248 us (970 TFLOP/s).
+// heads, 332 us (828 TFLOP/s); the last 2048 of 8192 tokens on 32 heads over 8,
+// 246 us (977 TFLOP/s).  Errors of an output's norm: 1.7e-3 in bf16, 3.9e-4 in
+// f16 (2.1e-4 its own rounding).
 //
 // Every wait is bounded; one that runs out sets error_flag[1] and the CTA
 // winds down with its TMEM freed.
@@ -64,17 +78,24 @@ namespace kv {
 namespace {
 
 using namespace tc;
-using attn::compute_p;
+using attn::add2;
 using attn::ex2;
+using attn::f2;
+using attn::fma2;
+using attn::hi_of;
+using attn::lo_of;
+using attn::max3;
 using attn::pack2;
-using attn::row_max;
 
 constexpr int kTileRows = 128;
 constexpr int kTcTile = 128;       // keys of a tile
 constexpr int kProducers = 3;      // warps 1 .. 3 of the packed form
 constexpr int kTmemCols = 512;
 constexpr float kTcFloor = -1.0e38f;
-constexpr float kTcGrow = 8.0f;    // log2 units: the running maximum moves when a tile passes it by more
+constexpr float kTcUnder = 7.0f;   // log2 units that m lies below a row's largest t when it moves
+constexpr float kTcMost = 15.0f;   // ... that t may pass it by (weights up to 2^15 are f16)
+constexpr int kUnitMin = -60;      // their smallest exponent: l, in units of values, stays in fp32's range
+constexpr int kUnits = 4;          // tiles whose units are kept: a softmax warp is at most two behind the loads
 
 template <int D_, int G_> struct TcShape {
   static constexpr int D = D_, G = G_, NG = D / G;
@@ -84,13 +105,22 @@ template <int D_, int G_> struct TcShape {
   static constexpr int QT = D <= 128 ? 2 : 1;                // query tiles of a CTA
   static constexpr int ROWS = QT * kTileRows;
   static constexpr int RING = D <= 128 ? 2 : 1;              // tiles of K, and of V, in flight
-  static constexpr int SMEM = (QT + 2 * RING) * TILE_BYTES + 1024 + 256;
+  static constexpr int SMEM = (QT + 2 * RING) * TILE_BYTES + 1024 + 512;
   // slot and phase of key tile j in the rings
   static __device__ __forceinline__ int slot(int j) { return RING == 2 ? j & 1 : 0; }
   static __device__ __forceinline__ uint32_t phase(int j) { return (RING == 2 ? j >> 1 : j) & 1; }
 };
 
 constexpr int tc_threads(bool dense, int tiles) { return 32 * ((dense ? 2 : 1 + kProducers) + 4 * tiles); }
+
+// A tile's units, as softmax threads take them: of its quarters, or in the dense form of the whole tile ([0]).
+struct alignas(16) Units {
+  float k[4];       // 2^ke
+  float v[4], l[4]; // ve, 2^-ve
+  uint8_t odd[8];   // of keys, of values
+  uint32_t pad[2];
+};
+static_assert(sizeof(Units) == 64, "copied in 16-byte pieces");
 
 struct TcParams {
   Cache c;
@@ -103,7 +133,8 @@ struct TcParams {
   int blocks;  // 256-row blocks of a cache head
   int splits;
   int rows;    // dense: token rows of a cache head in the expanded keys and values
-  bool q_tma;  // dense: tiles of queries arrive by TMA too
+  const Units* units;  // dense: [batch * kv_heads][rows / 128]
+  int* odd;            // of every CTA, a bit to a query tile: keys were met that f16 does not hold
   FastDiv by_per;
   float scale_log2;  // > 0
   bool causal;
@@ -114,43 +145,263 @@ struct TcParams {
   int withhold;  // test hook: the V tile of this key tile is never announced (-1: none)
 };
 
-// code pairs (U, U + 4) of a word as 16-bit floats, exactly
-template <bool BF16, int U> __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+// code pairs (U, U + 4) of a word as f16, exactly
+template <int U> __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
   uint32_t d, x;
-  if constexpr (BF16) {
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w >> (4 * U)), "r"(0x000f000fu), "r"(0x43004300u));
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(0x43004300u));  // 128 + n - 128
-  } else {
-    const uint32_t y = U == 0 ? w << 4 : w >> (U == 0 ? 0 : 4 * U - 4);
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(y), "r"(0x00f000f0u), "r"(0x54005400u));
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(0x54005400u));  // 64 + n - 64
-  }
+  const uint32_t y = U == 0 ? w << 4 : w >> (U == 0 ? 0 : 4 * U - 4);
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(y), "r"(0x00f000f0u), "r"(0x54005400u));
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(0x54005400u));  // 64 + n - 64
   return d;
 }
-template <bool BF16> __device__ __forceinline__ uint32_t fma_pair(uint32_t a, uint32_t b, uint32_t c) {
+__device__ __forceinline__ uint32_t fma_pair(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
-  if constexpr (BF16)
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  else
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
-__device__ __forceinline__ bool finite16(uint32_t bits, bool bf16) {
-  const uint32_t e = bf16 ? 0x7f80u : 0x7c00u;
-  return (bits & e) != e;
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }  // -126 .. 127
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+
+// Magnitudes that a part of a tile's codes reach, as bits (which order as the magnitudes do), 0 where there is none.
+struct Reach {
+  uint32_t far = 0;                                       // the largest
+  uint32_t key = 0x7f7fffffu, group = 0x7f7fffffu;        // the smallest key's largest, the smallest group's
+
+  // A key's groups, one after the other, then `done`.  Parts that are no finite numbers count as nothing; a group of
+  // zeros (bias 0, the smallest scale there is) has no magnitude to lose.
+  uint32_t now = 0;
+  __device__ __forceinline__ void add(float s, float z) {
+    if (!(finite(s) && finite(z))) return;
+    const uint32_t r = min(max(__float_as_uint(fabsf(z)), __float_as_uint(fabsf(fmaf(15.f, s, z)))), 0x7f7fffffu);
+    far = max(far, r);
+    if (z == 0.f && fabsf(s) < 1.1e-8f) return;
+    now = max(now, r);
+    if (r) group = min(group, r);
+  }
+  __device__ __forceinline__ void done() {
+    if (now) key = min(key, now);
+  }
+  __device__ __forceinline__ void across_warp() {
+    far = __reduce_max_sync(0xffffffffu, far);
+    key = __reduce_min_sync(0xffffffffu, key);
+    group = __reduce_min_sync(0xffffffffu, group);
+  }
+  __device__ __forceinline__ int unit() const { return max(static_cast<int>(far >> 23) - 127 - 14, kUnitMin); }
+  // Whether f16 does not hold the part.  In its units a group's values keep 11 bits down to 2^-14; `finest`: what its
+  // magnitude has to be for that (packed tiles round the scale too, a fifteenth of it or less).  A row that gives the
+  // largest value no weight has its m from the other keys of the part, as far too high for the rest of the sequence as
+  // the largest lies above them; down to 2^-2 that leaves weights steps of 2^-16 of the largest.
+  __device__ __forceinline__ bool odd(int side, int finest) const {
+    const auto below = [&](uint32_t bits, int e) { return static_cast<int>(bits >> 23) - 127 - unit() < e; };
+    return far && (below(group, finest) || (side && below(key, -2)));
+  }
+};
+
+// Units of a side: of `part` of NU parts of a tile.
+template <int NU> __device__ __forceinline__ void set_units(Units* u, int side, int part, int e, bool odd) {
+  if (side == 0) {
+    u->k[part] = pow2(e);
+  } else {
+    u->v[part] = static_cast<float>(e);
+    u->l[part] = pow2(-e);
+  }
+  if (NU == 1)
+    *reinterpret_cast<uint32_t*>(u->odd + side * 4) = odd;
+  else
+    u->odd[side * 4 + part] = odd;
 }
+
+// Exponent of a row of queries: in units of it the row's largest magnitude, `top`, lies at [2^14, 2^15).
+__device__ __forceinline__ int query_unit(float top) { return static_cast<int>(max(__float_as_uint(top) >> 23, 20u)) - 127 - 14; }
+
+template <bool BF16> __device__ __forceinline__ float half_of(uint32_t w, int i) {
+  const uint32_t x = i ? w >> 16 : w & 0xffffu;
+  return BF16 ? __uint_as_float(x << 16) : to_f32(f16{static_cast<uint16_t>(x)});
+}
+
+// What a row's scores are worth, and the exponents of its values, in each of a tile's NU parts.
+template <int NU> struct Row {
+  float c[NU], v[NU];
+};
+// `query`: 2^qe.  A worth is more than nothing, so that a masked score stays -infinity.
+template <int NU> __device__ __forceinline__ Row<NU> row_units(float scale_log2, float query, uint32_t units) {
+  Row<NU> r;
+  uint32_t k[NU], v[NU];
+  load_words<NU>(units, k);
+  load_words<NU>(units + 16, v);
+#pragma unroll
+  for (int h = 0; h < NU; ++h) {
+    r.c[h] = fmaxf(scale_log2 * (query * __uint_as_float(k[h])), 0x1p-126f);
+    r.v[h] = __uint_as_float(v[h]);
+  }
+  return r;
+}
+
+// Weights of a row's 128 scores, packed into 64 pairs of f16 and stored to TMEM at s_addr (columns 0..63 of the S
+// buffer).  Returns the row sum of this tile's (unrounded) weights.
+template <int NU>
+__device__ __forceinline__ float weights(const uint32_t* raw, const Row<NU>& r, float m, uint32_t units, uint32_t s_addr) {
+  float sum = 0.f;
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    uint32_t down;
+    load_words<1>(units + 32 + (NU == 1 ? 0 : 4 * h), &down);
+    const float c = r.c[NU == 1 ? 0 : h], off = r.v[NU == 1 ? 0 : h] - m;
+    const uint64_t c2 = f2(c, c), o2 = f2(off, off);
+    uint64_t l2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+    uint32_t pk[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int pi = 16 * h + i;
+      const uint64_t x = fma2(f2(__uint_as_float(raw[2 * pi]), __uint_as_float(raw[2 * pi + 1])), c2, o2);
+      const uint64_t e = f2(ex2(lo_of(x)), ex2(hi_of(x)));
+      l2[i & 1] = add2(l2[i & 1], e);
+      pk[i] = pack2<false>(lo_of(e), hi_of(e));
+    }
+    tmem_st16(s_addr + 16 * h, pk);
+    const uint64_t l = add2(l2[0], l2[1]);
+    sum = fmaf(lo_of(l) + hi_of(l), __uint_as_float(down), sum);
+  }
+  return sum;
+}
+
+// Largest t of a row's 128 scores (NaN ones aside).
+template <int NU> __device__ __forceinline__ float largest(const uint32_t* raw, const Row<NU>& r) {
+  float top[4];
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    float m4[4];
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+      m4[a] = max3(__uint_as_float(raw[32 * h + 2 * a]), __uint_as_float(raw[32 * h + 2 * a + 1]),
+                   __uint_as_float(raw[32 * h + 8 + a]));
+#pragma unroll
+    for (int i = 12; i + 8 <= 32; i += 8)
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+        m4[a] = max3(m4[a], __uint_as_float(raw[32 * h + i + 2 * a]), __uint_as_float(raw[32 * h + i + 2 * a + 1]));
+    const float m = max3(max3(m4[0], m4[1], __uint_as_float(raw[32 * h + 28])), max3(m4[2], m4[3], __uint_as_float(raw[32 * h + 29])),
+                         fmaxf(__uint_as_float(raw[32 * h + 30]), __uint_as_float(raw[32 * h + 31])));
+    top[h] = NU == 1 ? m : fmaf(m, r.c[NU == 1 ? 0 : h], r.v[NU == 1 ? 0 : h]);
+  }
+  const float m = max3(top[0], top[1], fmaxf(top[2], top[3]));
+  return NU == 1 ? fmaf(m, r.c[0], r.v[0]) : m;
+}
+
 __device__ __forceinline__ void store_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, int bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
 }
 // shared-memory writes of this thread become visible to the tensor core
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// A CTA's rows of queries and key tiles, by its number.
+struct Share {
+  int bh, b, h, rb, split, count, length, row0;
+  int j0, n_max, n_t[2];  // first key tile, how many from it on, for both query tiles and each
+};
+template <typename S> __device__ __forceinline__ Share share_of(const TcParams& p) {
+  Share s;
+  // Cache heads in groups of 16, so that the CTAs running at one time share few heads' keys in the L2; within a
+  // group row blocks from the last (the longest under a causal mask) down, a block's heads and splits together.
+  const int kv_heads = p.c.map.kv_heads;
+  const int all_heads = p.batch * kv_heads, in_group = 16 * p.blocks * p.splits;
+  const int group = static_cast<int>(blockIdx.x) / in_group, rem = static_cast<int>(blockIdx.x) % in_group;
+  const int wide = min(16, all_heads - 16 * group) * p.splits;
+  s.rb = p.blocks - 1 - rem / wide;
+  s.split = rem % wide % p.splits;
+  s.bh = 16 * group + rem % wide / p.splits;
+  s.b = s.bh / kv_heads;
+  s.h = s.bh % kv_heads;
+  s.count = p.counts ? clamp_count(__ldg(p.counts + s.b), p.tokens) : p.tokens;
+  s.length = clamp_count(__ldg(p.lengths + s.b), capacity(p.c.map));
+  s.row0 = s.rb * S::ROWS;
+  int need[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int first = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(s.row0 + t * kTileRows)));
+    const int last = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(s.row0 + t * kTileRows + kTileRows - 1)));
+    const int end = first >= s.count ? 0 : seen_end(s.length, s.count, last < s.count ? last : s.count - 1, p.causal);
+    need[t] = t < S::QT ? (end + kTcTile - 1) / kTcTile : 0;
+  }
+  const int all = max(need[0], need[1]);
+  s.j0 = static_cast<int>(static_cast<int64_t>(all) * s.split / p.splits);
+  s.n_max = static_cast<int>(static_cast<int64_t>(all) * (s.split + 1) / p.splits) - s.j0;
+  for (int t = 0; t < 2; ++t) s.n_t[t] = min(max(need[t] - s.j0, 0), s.n_max);
+  return s;
+}
+
+// A row's keys [k0, k1) in fp32, from the cache as it lies, by one thread: where a quarter's magnitudes differ by more
+// than f16 holds.  To `out`, or as a partial to `part` and `ml`.  Every 32 head dimensions go through the keys again,
+// so that no thread needs more memory of its own than registers.
+template <typename T, int D>
+__device__ __forceinline__ void plain_row(const TcParams& p, int b, int h, int head, int tok, int k0, int k1, T* out,
+                                       float* part, float* ml) {
+  const T* q = static_cast<const T*>(p.q) + b * p.st[2] + head * p.st[1] + tok * p.st[0];
+  const int ng = D / p.c.group;
+  float top = 0.f;
+  for (int d = 0; d < D; ++d) top = fmaxf(top, fabsf(to_f32(q[d])));
+  const int qe = query_unit(top);
+  const float up = pow2(-qe);  // (qe is -121 .. 114)
+  for (int d0 = 0; d0 < D; d0 += 32) {
+    float o[32], m = kTcFloor, l = 0.f;
+#pragma unroll
+    for (int d = 0; d < 32; ++d) o[d] = 0.f;
+    for (int key = k0; key < k1; ++key) {
+      const uint32_t at = row_of(p.c.map, b, h, key);
+      float s = 0.f, sv = 0.f, zv = 0.f;  // (a bad page's: zeros; it is reported already)
+      uint32_t word[4] = {};
+      if (at != kNoRow) {
+        const int64_t g0 = static_cast<int64_t>(at) * ng;
+        const uint32_t* k = p.c.codes[0] + static_cast<int64_t>(at) * (D / 8);
+        for (int g = 0; g < ng; ++g) {
+          float dot = 0.f, sum = 0.f;
+          for (int d = g * p.c.group; d < (g + 1) * p.c.group; ++d) {
+            const float x = to_f32(q[d]) * up;
+            dot = fmaf(x, static_cast<float>(k[d >> 3] >> (4 * (d & 7)) & 15), dot);
+            sum += x;
+          }
+          // (2^-24: a large key's bias times the sum stays in range)
+          s = fmaf(to_f32(static_cast<const T*>(p.c.scales[0])[g0 + g]) * 0x1p-24f, dot,
+                   fmaf(to_f32(static_cast<const T*>(p.c.biases[0])[g0 + g]) * 0x1p-24f, sum, s));
+        }
+        s = s * (p.scale_log2 * 0x1p24f) * pow2(qe);
+        sv = to_f32(static_cast<const T*>(p.c.scales[1])[g0 + d0 / p.c.group]);
+        zv = to_f32(static_cast<const T*>(p.c.biases[1])[g0 + d0 / p.c.group]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) word[i] = p.c.codes[1][static_cast<int64_t>(at) * (D / 8) + d0 / 8 + i];
+      }
+      const float m_new = fmaxf(m, s), was = ex2(m - m_new), w = ex2(s - m_new);
+      m = m_new;
+      l = fmaf(l, was, w);
+#pragma unroll
+      for (int d = 0; d < 32; ++d)
+        o[d] = fmaf(w, fmaf(sv, static_cast<float>(word[d >> 3] >> (4 * (d & 7)) & 15), zv), o[d] * was);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int d = 0; d < 32; ++d) {
+      if (part)
+        part[d0 + d] = o[d];
+      else
+        out[d0 + d] = from_f32<T>(o[d] * inv);
+    }
+    if (part) {
+      ml[0] = m;
+      ml[1] = l;
+    }
+  }
+}
+
 template <typename S, bool BF16, bool DENSE>
 __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
-    attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                   const __grid_constant__ CUtensorMap tm_v, const TcParams p) {
+    attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const TcParams p) {
   constexpr int D = S::D, NG = S::NG;
   constexpr int FIRST = DENSE ? 2 : 1 + kProducers;  // softmax warp
+  constexpr int NU = DENSE ? 1 : 4;                  // units to a tile
   using T = typename std::conditional<BF16, bf16, f16>::type;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -167,43 +418,25 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
   uint64_t* p_full = bars + 12;   // [2]
   uint64_t* o_done = bars + 14;   // [2]
   uint64_t* drain = bars + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+  uint64_t* u_full = bars + 17;   // [kUnits]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
   int* s_poison = reinterpret_cast<int*>(tmem_slot + 1);  // first key whose values are not finite
+  int* s_odd = reinterpret_cast<int*>(bars + 22);         // [2] a tile of keys that f16 does not hold was met
+  Units* s_units = reinterpret_cast<Units*>(bars + 24);   // [kUnits]
   int* wait_flag = p.error_flag + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // ---- which rows and which keys ----
-  // Cache heads in groups of 16, so that the CTAs running at one time share few heads' keys in the L2; within a
-  // group row blocks from the last (the longest under a causal mask) down, a block's heads and splits together.
-  const int kv_heads = p.c.map.kv_heads;
-  const int all_heads = p.batch * kv_heads, in_group = 16 * p.blocks * p.splits;
-  const int group = static_cast<int>(blockIdx.x) / in_group, rem = static_cast<int>(blockIdx.x) % in_group;
-  const int wide = min(16, all_heads - 16 * group) * p.splits;
-  const int rb = p.blocks - 1 - rem / wide;
-  const int split = rem % wide % p.splits, bh = 16 * group + rem % wide / p.splits;
-  const int b = bh / kv_heads, h = bh % kv_heads;
-  const int count = p.counts ? clamp_count(__ldg(p.counts + b), p.tokens) : p.tokens;
-  const int length = clamp_count(__ldg(p.lengths + b), capacity(p.c.map));
+  const Share sh = share_of<S>(p);
+  const int b = sh.b, h = sh.h, bh = sh.bh, rb = sh.rb, split = sh.split, count = sh.count, length = sh.length;
+  const int row0 = sh.row0, j0 = sh.j0, n_max = sh.n_max;
+  const int n_t[2] = {sh.n_t[0], sh.n_t[1]};
   if (threadIdx.x == 0 && length != __ldg(p.lengths + b)) atomicExch(p.error_flag, PHEW_ERR_INVALID);
-  const int row0 = rb * S::ROWS;
-  // key tiles that each query tile needs, and this CTA's share of them
-  int need[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int first = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(row0 + t * kTileRows)));
-    const int last = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(row0 + t * kTileRows + kTileRows - 1)));
-    const int end = first >= count ? 0 : seen_end(length, count, last < count ? last : count - 1, p.causal);
-    need[t] = t < S::QT ? (end + kTcTile - 1) / kTcTile : 0;
-  }
-  const int all = max(need[0], need[1]);
-  const int j0 = static_cast<int>(static_cast<int64_t>(all) * split / p.splits);
-  const int n_max = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / p.splits) - j0;
-  const int n_t[2] = {min(max(need[0] - j0, 0), n_max), min(max(need[1] - j0, 0), n_max)};
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], DENSE && p.q_tma ? 1 : 4);
+      mbar_init(&q_full[i], 4);
       mbar_init(&k_full[i], DENSE ? 1 : 4);
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], DENSE ? 1 : 4);
@@ -213,20 +446,10 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
       mbar_init(&o_done[i], 1);
     }
     mbar_init(drain, 1);
+    for (int i = 0; i < kUnits; ++i) mbar_init(&u_full[i], DENSE ? 1 : 8);
     *s_poison = 0x7fffffff;
+    s_odd[0] = s_odd[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (DENSE && p.q_tma) {
-      // rows token * per + head: boxes of `per` heads x 128 / per tokens
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (n_t[t] > 0) {
-          mbar_expect_tx(&q_full[t], S::TILE_BYTES);
-          const int tok = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(row0 + t * kTileRows)));
-#pragma unroll
-          for (int i = 0; i < S::HALVES; ++i)
-            tma_load_4d(sQ + t * S::TILE_BYTES + i * S::HALF_BYTES, &tm_q, &q_full[t], i * 64, h * p.per, tok, b);
-        }
-    }
   }
   if (warp == 0) tmem_alloc(tmem_slot, kTmemCols);
   fence_before_sync();
@@ -235,12 +458,13 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
   int k_last[2] = {-1, -1}, v_last[2] = {-1, -1};  // dense: the key tile whose load each ring slot received last
+  int u_last = -1;                                 // ... whose units were loaded last
 
   if (warp == 0) {
     if (lane == 0) {
       // ---------------- MMA issuer ----------------
-      constexpr uint32_t id_qk = instr_desc_f16(BF16 ? 1 : 0, 0, kTileRows, kTcTile);
-      constexpr uint32_t id_pv = instr_desc_f16(BF16 ? 1 : 0, 1, kTileRows, D);
+      constexpr uint32_t id_qk = instr_desc_f16(0, 0, kTileRows, kTcTile);
+      constexpr uint32_t id_pv = instr_desc_f16(0, 1, kTileRows, D);
       auto issue_s = [&](int t, uint32_t k_addr) {
         const uint32_t q_addr = smem_u32(sQ + t * S::TILE_BYTES);
 #pragma unroll
@@ -308,6 +532,11 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
         const uint32_t ph = S::phase(j) ^ 1;
         if (!mbar_wait(&k_empty[s], ph, wait_flag, p.wait_ns)) { ok = false; break; }
         load(&tm_k, &k_full[s], sK + s * S::TILE_BYTES, first + j * kTcTile);
+        // (the softmax has read the units of tile j - 4: scores of j - 2 were made after its weights of j - 3)
+        u_last = j;
+        uint64_t* bar = &u_full[j & (kUnits - 1)];
+        mbar_expect_tx(bar, sizeof(Units));
+        bulk_load(&s_units[j & (kUnits - 1)], p.units + static_cast<int64_t>(bh) * (p.rows / kTcTile) + j0 + j, sizeof(Units), bar);
         (s ? k_last[1] : k_last[0]) = j;
         if (!mbar_wait(&v_empty[s], ph, wait_flag, p.wait_ns)) { ok = false; break; }
         if (j == p.withhold) continue;  // test hook: this V tile never lands
@@ -366,22 +595,40 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
     };
     auto expand = [&](int u, Packed& x) {
       const int j = u >> 3, side = (u >> 2) & 1, row = (u & 3) * 32 + lane, slot = S::slot(j);
-      uint32_t sc[NG], bi[NG];  // each twice in a register
-      bool fine = true, past = false;  // parts finite; values past the type's range (held at its end)
+      // in units of the quarter's own power of two
+      float s[NG], z[NG];
+      Reach reach;
+      bool fine = true;  // parts finite
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        sc[g] = __byte_perm(x.sb[0][g / 2], 0, g & 1 ? 0x3232 : 0x1010);
-        bi[g] = __byte_perm(x.sb[1][g / 2], 0, g & 1 ? 0x3232 : 0x1010);
-        fine = fine && finite16(sc[g], BF16) && finite16(bi[g], BF16);
-        past = past || !finite16(fma_pair<BF16>(sc[g], BF16 ? 0x41704170u : 0x4b804b80u, bi[g]), BF16);  // code 15
+        s[g] = half_of<BF16>(x.sb[0][g / 2], g & 1);
+        z[g] = half_of<BF16>(x.sb[1][g / 2], g & 1);
+        reach.add(s[g], z[g]);
+        fine = fine && finite(s[g]) && finite(z[g]);
       }
-      past = past && fine;
+      reach.done();
+      reach.across_warp();
+      const int unit = reach.unit();
+      const float down = pow2(-unit);
+      if (lane == 0) {
+        // (read by the softmax when the scores are there; it has read those of tile j - 4: this warp's unit before
+        // this one found its slot empty of tile j - 3's)
+        uint64_t* bar = &u_full[j & (kUnits - 1)];
+        set_units<NU>(&s_units[j & (kUnits - 1)], side, u & 3, unit, reach.odd(side, -10));
+        mbar_arrive(bar);
+      }
       if (side == 1 && !fine) {
         // a weight of zero times infinity is no number, and a later query's keys may not touch an earlier
         // one: the values count as zero here and as "no number" for every row that sees the key
         atomicMin(s_poison, (j0 + j) * kTcTile + row);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) sc[g] = bi[g] = 0;
+        for (int g = 0; g < NG; ++g) s[g] = z[g] = 0.f;
+      }
+      uint32_t sc[NG], bi[NG];  // each twice in a register
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        sc[g] = pack2<false>(s[g] * down, s[g] * down);
+        bi[g] = pack2<false>(z[g] * down, z[g] * down);
       }
       uint64_t* full = side == 0 ? &k_full[slot] : &v_full[slot];
       uint64_t* empty = side == 0 ? &k_empty[slot] : &v_empty[slot];
@@ -389,20 +636,14 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) return;
       const uint32_t dst = smem_u32((side == 0 ? sK : sV) + slot * S::TILE_BYTES) + row * 128;
-      const bool any_past = __any_sync(0xffffffffu, past);
 #pragma unroll
       for (int ch = 0; ch < D / 32; ++ch) {
         const uint32_t word[4] = {x.code[ch].x, x.code[ch].y, x.code[ch].z, x.code[ch].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int g = (ch * 32 + i * 8) / S::G, c16 = ch * 4 + i;
-          uint32_t v[4] = {fma_pair<BF16>(sc[g], code_pair<BF16, 0>(word[i]), bi[g]),
-                           fma_pair<BF16>(sc[g], code_pair<BF16, 1>(word[i]), bi[g]),
-                           fma_pair<BF16>(sc[g], code_pair<BF16, 2>(word[i]), bi[g]),
-                           fma_pair<BF16>(sc[g], code_pair<BF16, 3>(word[i]), bi[g])};
-          if (any_past)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = past ? hold_pair<BF16>(v[k]) : v[k];
+          const uint32_t v[4] = {fma_pair(sc[g], code_pair<0>(word[i]), bi[g]), fma_pair(sc[g], code_pair<1>(word[i]), bi[g]),
+                                 fma_pair(sc[g], code_pair<2>(word[i]), bi[g]), fma_pair(sc[g], code_pair<3>(word[i]), bi[g])};
           store_shared16(dst + (c16 >> 3) * S::HALF_BYTES + (((c16 & 7) ^ (row & 7)) << 4), v[0], v[1], v[2], v[3]);
         }
       }
@@ -438,26 +679,59 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
       return __all_sync(0xffffffffu, mbar_wait(bar, phase, wait_flag, p.wait_ns));
     };
     const int nkv = t ? n_t[1] : n_t[0];
-    const float c = p.scale_log2;
     int lim;
+    float query = 1.f;  // 2^qe
     {
       const int r = row0 + t * kTileRows + row;
       const int tok = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(r)));
       lim = seen_end(length, count, tok, p.causal) - j0 * kTcTile;
-      if (nkv > 0 && !(DENSE && p.q_tma)) {
-        const bool have = tok < count;
-        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.st[2] +
-                                                        (h * p.per + (r - tok * p.per)) * p.st[1] + tok * p.st[0]);
-        const uint32_t dst = smem_u32(sQ + t * S::TILE_BYTES) + row * 128;
+      if (nkv > 0) {
+        // sixteen lanes to a row, two rows at a time: their largest magnitudes (NaN ones aside), then the rows in units
+        // of those (exactly, but for what lies 2^-29 below)
+        const int half = lane >> 4, c16 = lane & 15;
+        constexpr int CHUNKS = D / 8, STEPS = CHUNKS > 16 ? CHUNKS / 16 : 1;  // 16-byte pieces of a row, of a lane
+        uint4 x[16][STEPS];
 #pragma unroll
-        for (int c16 = 0; c16 < D / 8; ++c16) {
-          const uint4 x = have ? __ldg(q + c16) : make_uint4(0, 0, 0, 0);
-          const uint32_t at = dst + (c16 >> 3) * S::HALF_BYTES + (((c16 & 7) ^ (row & 7)) << 4);
-          if constexpr (DENSE)
-            store_shared16(at, x.x, x.y, x.z, x.w);
-          else
-            store_shared16(at, __byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410),
-                           __byte_perm(x.y, x.w, 0x7632));
+        for (int i = 0; i < 16; ++i) {
+          const int rr = row0 + t * kTileRows + quarter * 32 + 2 * i + half;
+          const int tt = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(rr)));
+          const uint4* q = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.st[2] +
+                                                          (h * p.per + (rr - tt * p.per)) * p.st[1] + tt * p.st[0]);
+#pragma unroll
+          for (int k = 0; k < STEPS; ++k)
+            x[i][k] = tt < count && c16 + 16 * k < CHUNKS ? __ldg(q + c16 + 16 * k) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float top = 0.f;
+#pragma unroll
+          for (int k = 0; k < STEPS; ++k) {
+            const uint32_t w[4] = {x[i][k].x, x[i][k].y, x[i][k].z, x[i][k].w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              top = fmaxf(top, fmaxf(fabsf(half_of<BF16>(w[y], 0)), fabsf(half_of<BF16>(w[y], 1))));
+          }
+#pragma unroll
+          for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const int qe = query_unit(top);
+          const float up = pow2(-qe);
+          const int mine = __shfl_sync(0xffffffffu, qe, (lane & 1) * 16);
+          if (lane >> 1 == i) query = pow2(mine);
+          const int rw = quarter * 32 + 2 * i + half;
+#pragma unroll
+          for (int k = 0; k < STEPS; ++k) {
+            uint32_t w[4] = {x[i][k].x, x[i][k].y, x[i][k].z, x[i][k].w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y) w[y] = pack2<false>(half_of<BF16>(w[y], 0) * up, half_of<BF16>(w[y], 1) * up);
+            const int ch = c16 + 16 * k;
+            if (ch >= CHUNKS) continue;
+            const uint32_t at = smem_u32(sQ + t * S::TILE_BYTES) + rw * 128 + (ch >> 3) * S::HALF_BYTES + (((ch & 7) ^ (rw & 7)) << 4);
+            if constexpr (DENSE)
+              store_shared16(at, w[0], w[1], w[2], w[3]);
+            else
+              store_shared16(at, __byte_perm(w[0], w[2], 0x5410), __byte_perm(w[0], w[2], 0x7632), __byte_perm(w[1], w[3], 0x5410),
+                             __byte_perm(w[1], w[3], 0x7632));
+          }
         }
         fence_async_shared();
         __syncwarp();
@@ -466,6 +740,15 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
     }
     float m_ref = kTcFloor, l = 0.f;
     for (int j = 0; j < nkv && ok; ++j) {
+      // the tile's units: there long before its scores
+      if (!wait(&u_full[j & (kUnits - 1)], (j / kUnits) & 1)) { ok = false; break; }
+      const uint32_t units = smem_u32(&s_units[j & (kUnits - 1)]);
+      {
+        uint32_t bad[2];
+        load_words<2>(units + 48, bad);
+        if (bad[0] | bad[1]) s_odd[t] = 1;
+      }
+      const Row<NU> ru = row_units<NU>(p.scale_log2, query, units);
       if (!wait(&s_full[t], j & 1)) { ok = false; break; }
       fence_after_sync();
       uint32_t raw[128];
@@ -481,13 +764,13 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
       bool rescale = false;
       float alpha = 1.f;
       if (j == 0) {
-        m_ref = fmaxf(row_max(raw) * c, kTcFloor);
-        tile_sum = compute_p<BF16>(raw, c, m_ref, s_addr);
+        m_ref = fmaxf(largest<NU>(raw, ru) - kTcUnder, kTcFloor);
+        tile_sum = weights<NU>(raw, ru, m_ref, units, s_addr);
       } else {
         // weights against the running maximum while this tile's is reduced, redone if it grew too far
-        tile_sum = compute_p<BF16>(raw, c, m_ref, s_addr);
-        const float m_tile = row_max(raw) * c;
-        if (m_tile > m_ref + kTcGrow) {
+        tile_sum = weights<NU>(raw, ru, m_ref, units, s_addr);
+        const float m_tile = largest<NU>(raw, ru) - kTcUnder;
+        if (m_tile > m_ref + (kTcMost - kTcUnder)) {
           alpha = ex2(m_ref - m_tile);
           m_ref = m_tile;
           rescale = true;
@@ -495,7 +778,7 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
       }
       if (__any_sync(0xffffffffu, rescale)) {
         tmem_st_wait();
-        tile_sum = compute_p<BF16>(raw, c, m_ref, s_addr);
+        tile_sum = weights<NU>(raw, ru, m_ref, units, s_addr);
         if (!wait(&o_done[t], (j - 1) & 1)) ok = false;
         fence_after_sync();
         if (ok) {
@@ -577,9 +860,6 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
   if (__syncthreads_or(!ok)) {
     // a wait ran out somewhere: let the issued products and loads finish before the TMEM and shared memory go
     if (warp == 0 && lane == 0) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (DENSE && p.q_tma && n_t[t] > 0) mbar_wait(&q_full[t], 0, nullptr, p.wait_ns);
       commit(drain);
       mbar_wait(drain, 0, nullptr, p.wait_ns);
     } else if (DENSE && warp == 1 && lane == 0) {
@@ -588,6 +868,8 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
         if (k_last[i] >= 0) mbar_wait(&k_full[i], S::phase(k_last[i]), nullptr, p.wait_ns);
         if (v_last[i] >= 0) mbar_wait(&v_full[i], S::phase(v_last[i]), nullptr, p.wait_ns);
       }
+      for (int j = max(u_last - kUnits + 1, 0); j <= u_last; ++j)
+        mbar_wait(&u_full[j & (kUnits - 1)], (j / kUnits) & 1, nullptr, p.wait_ns);
     }
     fence_before_sync();
     __syncthreads();
@@ -596,6 +878,26 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
     fence_after_sync();
     tmem_dealloc(tmem, kTmemCols);
   }
+  if (threadIdx.x == 0) p.odd[blockIdx.x] = s_odd[0] | s_odd[1] << 1;
+}
+
+// Rows that met keys that f16 does not hold, again: CTA by CTA of attn_tc_kernel, a thread to a row.
+template <typename S, bool BF16> __global__ void __launch_bounds__(S::ROWS) plain_rows_kernel(const TcParams p) {
+  using T = typename std::conditional<BF16, bf16, f16>::type;
+  constexpr int D = S::D;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int t = threadIdx.x / kTileRows;
+  if (!(p.odd[blockIdx.x] >> t & 1)) return;
+  const Share s = share_of<S>(p);
+  const int r = s.row0 + static_cast<int>(threadIdx.x);
+  const int tok = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(r)));
+  const int head = s.h * p.per + (r - tok * p.per);
+  const int end = min(seen_end(s.length, s.count, tok, p.causal), (s.j0 + (t ? s.n_t[1] : s.n_t[0])) * kTcTile);
+  if (end <= 0) return;
+  const int64_t slot = ((static_cast<int64_t>(s.bh) * p.blocks + s.rb) * p.splits + s.split) * S::ROWS + threadIdx.x;
+  T* out = static_cast<T*>(p.o) + ((static_cast<int64_t>(s.b) * p.heads + head) * p.tokens + tok) * D;
+  plain_row<T, D>(p, s.b, s.h, head, tok, s.j0 * kTcTile, end, out, p.splits > 1 ? p.part + slot * D : nullptr,
+                  p.part_ml + slot * 2);
 }
 
 // Joins the splits of a row: one warp per row, splits in their order.
@@ -633,6 +935,112 @@ __global__ void __launch_bounds__(256) combine_tc_kernel(const TcParams p) {
   for (int i = 0; i < E; ++i) out[i * 32 + lane] = from_f32<T>(o[i] * inv);
 }
 
+struct ExpandParams {
+  Cache c;
+  void* dense[2];  // [batch * kv_heads][rows][D] f16
+  Units* units;    // [batch * kv_heads][rows / 128]
+  const int32_t* lengths;
+  FastDiv by_tiles, by_heads;  // tiles of a head, heads
+  int* error_flag;
+};
+
+// The dense form's keys and values, a tile and a side to a block: written up to a sequence's last tile, zero behind its
+// last key.  A weight of zero would make a NaN of an infinity, so a key whose value's scale or bias is not finite gets
+// zero for a value and NaN for a key: rows that see it get one through their score.
+// Bound by HBM and latencies: two prompts of 4096 tokens on 32 heads of 128, 38 MB read and 134 MB written in 31 us.
+// Launched so that a programmatic dependent may be set up meanwhile.
+template <int D> constexpr int kExpandThreads = D <= 128 ? 128 : 256;
+template <typename T, int D> __global__ void __launch_bounds__(kExpandThreads<D>) expand_kernel(const ExpandParams p) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  constexpr int THREADS = kExpandThreads<D>, WORDS = D / 8;  // words of eight codes to a row
+  constexpr int W = kTcTile * WORDS / THREADS;               // to a thread
+  __shared__ uint32_t s_row[kTcTile];
+  __shared__ Reach s_reach[kTcTile / 32];
+  __shared__ float2 s_affine[kTcTile][D / 32];  // scale and bias of a key's groups
+  const int side = blockIdx.y, tid = threadIdx.x;
+  const uint32_t bh = div_by(p.by_tiles, blockIdx.x);
+  const int tile = static_cast<int>(blockIdx.x - bh * p.by_tiles.d);
+  const int b = static_cast<int>(div_by(p.by_heads, bh)), h = static_cast<int>(bh - b * p.by_heads.d);
+  const int length = __ldg(p.lengths + b);
+  if (tile * kTcTile >= length) return;
+  const int ng = D / p.c.group, shift = p.c.group == 32 ? 2 : p.c.group == 64 ? 3 : 4;  // words to a group: 2^shift
+  if (tid < kTcTile) {
+    const int key = tile * kTcTile + tid;
+    uint32_t at = kNoRow;
+    if (key < length) {
+      at = row_of(p.c.map, b, h, key);
+      if (at == kNoRow) atomicExch(p.error_flag, PHEW_ERR_INVALID);
+    }
+    s_row[tid] = at;
+    Reach reach;
+#pragma unroll 4
+    for (int g = 0; g < ng; ++g) {
+      float2 a = make_float2(0.f, 0.f);
+      if (at != kNoRow) {
+        const int64_t i = static_cast<int64_t>(at) * ng + g;
+        const float vs = to_f32(static_cast<const T*>(p.c.scales[1])[i]), vz = to_f32(static_cast<const T*>(p.c.biases[1])[i]);
+        if (finite(vs) && finite(vz))
+          a = side ? make_float2(vs, vz)
+                   : make_float2(to_f32(static_cast<const T*>(p.c.scales[0])[i]), to_f32(static_cast<const T*>(p.c.biases[0])[i]));
+        else
+          a.y = side ? 0.f : __int_as_float(0x7fc00000);
+      }
+      s_affine[tid][g] = a;
+      reach.add(a.x, a.y);
+    }
+    reach.done();
+    reach.across_warp();
+    if (tid % 32 == 0) s_reach[tid / 32] = reach;
+  }
+  __syncthreads();
+  uint32_t word[W];
+#pragma unroll
+  for (int u = 0; u < W; ++u) {
+    const int i = u * THREADS + tid;
+    const uint32_t at = s_row[i / WORDS];
+    word[u] = at == kNoRow ? 0 : __ldg(p.c.codes[side] + static_cast<int64_t>(at) * WORDS + i % WORDS);
+  }
+  Reach reach = s_reach[0];
+#pragma unroll
+  for (int i = 1; i < kTcTile / 32; ++i) {
+    reach.far = max(reach.far, s_reach[i].far);
+    reach.key = min(reach.key, s_reach[i].key);
+    reach.group = min(reach.group, s_reach[i].group);
+  }
+  const int unit = reach.unit();
+  if (tid == 0) set_units<1>(p.units + blockIdx.x, side, 0, unit, reach.odd(side, -14));
+  const float down = pow2(-unit);
+  uint4* dst = static_cast<uint4*>(p.dense[side]) + static_cast<int64_t>(blockIdx.x) * (kTcTile * WORDS) + tid;
+#pragma unroll
+  for (int u = 0; u < W; ++u) {
+    const int w = u * THREADS + tid;
+    const float2 a = s_affine[w / WORDS][w % WORDS >> shift];
+    const uint64_t s2 = f2(a.x * down, a.x * down), z2 = f2(a.y * down, a.y * down);
+    // a code as a float: a byte of it under 2^23
+    constexpr uint32_t base = 0x4B000000u;
+    const uint32_t even = word[u] & 0x0f0f0f0fu, other = (word[u] >> 4) & 0x0f0f0f0fu;
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t n = add2(f2(__uint_as_float(__byte_perm(even, base, 0x7540 + i)), __uint_as_float(__byte_perm(other, base, 0x7540 + i))),
+                              f2(-8388608.f, -8388608.f));
+      const uint64_t x = fma2(s2, n, z2);
+      v[i] = pack2<false>(lo_of(x), hi_of(x));
+    }
+    dst[u * THREADS] = make_uint4(v[0], v[1], v[2], v[3]);
+  }
+}
+
+template <typename T> int launch_expand(const ExpandParams& p, unsigned tiles, cudaStream_t st) {
+  const dim3 grid(tiles, 2);
+  switch (p.c.head_dim) {
+    case 64: expand_kernel<T, 64><<<grid, kExpandThreads<64>, 0, st>>>(p); break;
+    case 128: expand_kernel<T, 128><<<grid, kExpandThreads<128>, 0, st>>>(p); break;
+    default: expand_kernel<T, 256><<<grid, kExpandThreads<256>, 0, st>>>(p); break;
+  }
+  return launch_status("kv expand_kernel");
+}
+
 // CTAs of a call, how many ways each row block's keys are split (enough to give
 // every SM a CTA, two tiles of the longest possible sequence or more each), and
 // whether the cache is expanded first.
@@ -653,7 +1061,7 @@ int rows_of(int head_dim) { return head_dim <= 128 ? TcShape<128, 128>::ROWS : T
 struct TcPlan {
   int64_t blocks, splits, ctas;
   int64_t rows;  // token rows of a cache head in the expanded cache; 0: packed
-  size_t part_bytes, side_bytes;
+  size_t part_bytes, side_bytes, unit_bytes;
 };
 TcPlan tc_plan(int64_t batch, int kv_heads, int head_dim, int64_t q_rows, int64_t cap) {
   TcPlan t;
@@ -673,19 +1081,20 @@ TcPlan tc_plan(int64_t batch, int kv_heads, int head_dim, int64_t q_rows, int64_
     t.rows = 0;
     t.side_bytes = 0;
   }
+  t.unit_bytes = static_cast<size_t>(batch) * kv_heads * (t.rows / kTcTile) * sizeof(Units);
   return t;
 }
 
-// [batch * kv_heads * rows][D] of 16-bit values; box of 64 columns x 128 rows, 128-byte swizzle.
-int dense_map(CUtensorMap* tm, const void* base, bool bf16_type, int64_t rows, int D) {
+// [batch * kv_heads * rows][D] of f16; box of 64 columns x 128 rows, 128-byte swizzle.
+int dense_map(CUtensorMap* tm, const void* base, int64_t rows, int D) {
   const uint64_t dims[2] = {static_cast<uint64_t>(D), static_cast<uint64_t>(rows)};
   const uint64_t strides[1] = {static_cast<uint64_t>(D) * 2};
   const uint32_t box[2] = {64, static_cast<uint32_t>(kTcTile)};
-  return make_map_16bit(tm, base, bf16_type, 2, dims, strides, box);
+  return make_map_16bit(tm, base, false, 2, dims, strides, box);
 }
 
 struct Maps {
-  CUtensorMap q, k, v;  // dense
+  CUtensorMap k, v;  // dense
 };
 
 template <typename S, bool BF16, bool DENSE>
@@ -702,15 +1111,19 @@ int launch_tc(const Maps& m, const TcParams& p, unsigned grid, cudaStream_t st) 
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = DENSE ? 1 : 0;  // set up while the cache is expanded
-  PHEW_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_tc_kernel<S, BF16, DENSE>, m.q, m.k, m.v, p));
+  PHEW_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_tc_kernel<S, BF16, DENSE>, m.k, m.v, p));
   if (int s = launch_status("kv attn_tc_kernel")) return s;
-  if (p.splits == 1) return PHEW_OK;
   cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.batch) * p.c.map.kv_heads * p.blocks * (S::ROWS / 8)));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(S::ROWS);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  PHEW_CHECK_CUDA(cudaLaunchKernelEx(&cfg, plain_rows_kernel<S, BF16>, p));
+  if (int s = launch_status("kv plain_rows_kernel")) return s;
+  if (p.splits == 1) return PHEW_OK;
+  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.batch) * p.c.map.kv_heads * p.blocks * (S::ROWS / 8)));
+  cfg.blockDim = dim3(256);
   PHEW_CHECK_CUDA(cudaLaunchKernelEx(&cfg, combine_tc_kernel<S, BF16>, p));
   return launch_status("kv combine_tc_kernel");
 }
@@ -739,7 +1152,7 @@ bool takes_tc(int64_t batch, int kv_heads, int head_dim, int dtype, int64_t rows
 
 size_t tc_bytes(int64_t batch, int kv_heads, int head_dim, int64_t rows, int64_t cap) {
   const TcPlan t = tc_plan(batch, kv_heads, head_dim, rows, cap);
-  return 2 * t.side_bytes + t.part_bytes;
+  return 2 * t.side_bytes + t.unit_bytes + t.part_bytes + (static_cast<size_t>(t.ctas) * 4 + 15) / 16 * 16;
 }
 
 int run_attn_tc(const AttnParams& a, bool bf16_type, void* workspace, cudaStream_t st) {
@@ -765,25 +1178,26 @@ int run_attn_tc(const AttnParams& a, bool bf16_type, void* workspace, cudaStream
   p.causal = a.causal;
   char* scratch = static_cast<char*>(workspace);
   Maps m = {};
-  p.q_tma = false;
+  p.units = nullptr;
   if (t.rows) {
     const int64_t rows = static_cast<int64_t>(a.batch) * a.c.map.kv_heads * t.rows;
-    if (int s = dense_map(&m.k, scratch, bf16_type, rows, D)) return s;
-    if (int s = dense_map(&m.v, scratch + t.side_bytes, bf16_type, rows, D)) return s;
-    // tiles of queries are boxes where a tile holds whole tokens and every axis has a stride
-    p.q_tma = kTileRows % a.per == 0 && a.st[0] > 0 && a.st[1] > 0 && a.st[2] > 0;
-    if (p.q_tma) {
-      const uint64_t dims[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(a.heads), static_cast<uint64_t>(a.tokens),
-                                static_cast<uint64_t>(a.batch)};
-      const uint64_t strides[3] = {static_cast<uint64_t>(a.st[1]) * 2, static_cast<uint64_t>(a.st[0]) * 2,
-                                   static_cast<uint64_t>(a.st[2]) * 2};
-      const uint32_t box[4] = {64, static_cast<uint32_t>(a.per), static_cast<uint32_t>(kTileRows / a.per), 1};
-      if (int s = make_map_16bit(&m.q, a.q, bf16_type, 4, dims, strides, box)) return s;
-    }
-    if (int s = expand(a.c, bf16_type, scratch, scratch + t.side_bytes, a.batch, t.rows, a.lengths, a.error_flag, st)) return s;
+    if (int s = dense_map(&m.k, scratch, rows, D)) return s;
+    if (int s = dense_map(&m.v, scratch + t.side_bytes, rows, D)) return s;
+    ExpandParams e;
+    e.c = a.c;
+    e.dense[0] = scratch;
+    e.dense[1] = scratch + t.side_bytes;
+    p.units = e.units = reinterpret_cast<Units*>(scratch + 2 * t.side_bytes);
+    e.lengths = a.lengths;
+    e.by_tiles = fast_div(static_cast<uint32_t>(t.rows / kTcTile));
+    e.by_heads = fast_div(static_cast<uint32_t>(a.c.map.kv_heads));
+    e.error_flag = a.error_flag;
+    const unsigned tiles = static_cast<unsigned>(rows / kTcTile);
+    if (int s = bf16_type ? launch_expand<bf16>(e, tiles, st) : launch_expand<f16>(e, tiles, st)) return s;
   }
-  p.part = reinterpret_cast<float*>(scratch + 2 * t.side_bytes);
+  p.part = reinterpret_cast<float*>(scratch + 2 * t.side_bytes + t.unit_bytes);
   p.part_ml = p.part + static_cast<size_t>(t.ctas) * rows_of(D) * D;
+  p.odd = reinterpret_cast<int*>(scratch + 2 * t.side_bytes + t.unit_bytes + t.part_bytes);
   p.error_flag = a.error_flag;
   const tc::TestStall stall = tc::take_test_stall();
   p.wait_ns = stall.wait_ns;

@@ -403,10 +403,8 @@ struct FetchParams {
 // contiguous.  A code becomes a float by a byte permutation into 2^23 + code
 // (conversions run at an eighth of the rate), two values to an instruction from
 // there.
-// EXPAND: as expand() says.
-template <typename T, int BITS, int D, bool EXPAND>
+template <typename T, int BITS, int D>
 __global__ void __launch_bounds__(kThreads) fetch_kernel(const FetchParams p) {
-  if (EXPAND) asm volatile("griddepcontrol.launch_dependents;");
   constexpr int LANES = D / 16;
   constexpr int PER_PASS = kThreads / LANES;
   constexpr int W = BITS / 4;  // words of eight codes
@@ -425,7 +423,6 @@ __global__ void __launch_bounds__(kThreads) fetch_kernel(const FetchParams p) {
     if (row < p.rows) {
       const Row r = row_after(p.split, first, first_row, row - first_row, PER_PASS * kRows);
       const int length = __ldg(p.lengths + r.b);
-      if (EXPAND) skip[u] = (r.i & ~127) >= length;
       if (r.i < length) {
         at[u] = row_of(p.c.map, r.b, r.h, r.i);
         if (at[u] == kNoRow) atomicExch(p.error_flag, PHEW_ERR_INVALID);
@@ -450,14 +447,6 @@ __global__ void __launch_bounds__(kThreads) fetch_kernel(const FetchParams p) {
       const int64_t s_at = static_cast<int64_t>(at[u]) * ng + ((half * (D / 2) + c * 8) >> shift);
       sc[u][half] = static_cast<const T*>(p.c.scales[side])[s_at];
       bi[u][half] = static_cast<const T*>(p.c.biases[side])[s_at];
-      if (EXPAND) {
-        const float s = to_f32(side ? sc[u][half] : static_cast<const T*>(p.c.scales[1])[s_at]);
-        const float z = to_f32(side ? bi[u][half] : static_cast<const T*>(p.c.biases[1])[s_at]);
-        if (!(fabsf(s) < INFINITY && fabsf(z) < INFINITY)) {
-          sc[u][half] = from_f32<T>(0.f);
-          bi[u][half] = from_f32<T>(side ? 0.f : __int_as_float(0x7fc00000));
-        }
-      }
     }
   }
 #pragma unroll
@@ -487,12 +476,6 @@ __global__ void __launch_bounds__(kThreads) fetch_kernel(const FetchParams p) {
           const uint64_t n = add2(two(__uint_as_float(lo), __uint_as_float(hi)), two(-8388608.f, -8388608.f));
           set_pair(out, i, fma2(two(s, s), n, two(z, z)));
         }
-      }
-      if constexpr (EXPAND) {
-        // scale * code + bias of finite parts may pass the type's largest value: held there
-        const bool held = at[u] != kNoRow && fabsf(to_f32(sc[u][half])) < INFINITY && fabsf(to_f32(bi[u][half])) < INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) out.w[i] = held ? hold_pair<std::is_same<T, bf16>::value>(out.w[i]) : out.w[i];
       }
       store8(dst + half * (D / 2), out);
     }
@@ -531,20 +514,10 @@ template <typename T> int update_typed(const UpdateParams& p, cudaStream_t st) {
 template <typename T, int BITS> void launch_fetch(const FetchParams& p, cudaStream_t st) {
   const dim3 grid = grid_for(p.rows, p.c.head_dim);
   switch (p.c.head_dim) {
-    case 64: fetch_kernel<T, BITS, 64, false><<<grid, kThreads, 0, st>>>(p); break;
-    case 128: fetch_kernel<T, BITS, 128, false><<<grid, kThreads, 0, st>>>(p); break;
-    default: fetch_kernel<T, BITS, 256, false><<<grid, kThreads, 0, st>>>(p); break;
+    case 64: fetch_kernel<T, BITS, 64><<<grid, kThreads, 0, st>>>(p); break;
+    case 128: fetch_kernel<T, BITS, 128><<<grid, kThreads, 0, st>>>(p); break;
+    default: fetch_kernel<T, BITS, 256><<<grid, kThreads, 0, st>>>(p); break;
   }
-}
-
-template <typename T> int expand_typed(const FetchParams& p, cudaStream_t st) {
-  const dim3 grid = grid_for(p.rows, p.c.head_dim);
-  switch (p.c.head_dim) {
-    case 64: fetch_kernel<T, 4, 64, true><<<grid, kThreads, 0, st>>>(p); break;
-    case 128: fetch_kernel<T, 4, 128, true><<<grid, kThreads, 0, st>>>(p); break;
-    default: fetch_kernel<T, 4, 256, true><<<grid, kThreads, 0, st>>>(p); break;
-  }
-  return launch_status("kv expand");
 }
 
 template <typename T> int fetch_typed(const FetchParams& p, cudaStream_t st) {
@@ -556,19 +529,6 @@ template <typename T> int fetch_typed(const FetchParams& p, cudaStream_t st) {
 }
 
 }  // namespace
-
-int expand(const Cache& c, bool bf16_type, void* k, void* v, int64_t batch, int64_t rows, const int32_t* lengths,
-           int* error_flag, cudaStream_t st) {
-  FetchParams p;
-  p.c = c;
-  p.dense[0] = k;
-  p.dense[1] = v;
-  p.lengths = lengths;
-  p.split = {fast_div(static_cast<uint32_t>(rows)), fast_div(static_cast<uint32_t>(c.map.kv_heads))};
-  p.rows = static_cast<int>(batch * c.map.kv_heads * rows);
-  p.error_flag = error_flag;
-  return bf16_type ? expand_typed<bf16>(p, st) : expand_typed<f16>(p, st);
-}
 
 int make_cache(const phew_kv_cache* c, const int* table, int64_t table_stride, int64_t columns, int64_t batch,
                const char* who, Cache* out) {

@@ -53,14 +53,16 @@ def bounds(plan, q, counts, scale, causal, tensor_core=False):
 
     Errors are independent from key to key, so norms add in squares.  With w_j a row's softmax weights, s_j and
     n_j a value's scale and codes, v'_j = s_j (n_j - 8), or s_j n_j where bf16 sums hold bare codes, or the
-    values rounded to the type on the tcgen05 path (more than 64 rows, where keys are too):
+    values themselves on the tcgen05 path (more than 64 rows):
       * the output rounded once: u |o|, and below 2^-14, where f16's steps stay 2^-24, half a step for each of a
         group's values: 2^-25 sqrt(group)
-      * weights times scales rounded by at most h of them (2^-11 as one f16 term, 2^-22 as two, u on the tcgen05
-        path): h N, N = sqrt(sum w_j^2 |v'_j|^2); 1.5 of it, the most that two keys can give
+      * weights times scales rounded by at most h of them (2^-11 as one f16 term, 2^-22 as two): h N,
+        N = sqrt(sum w_j^2 |v'_j|^2); 1.5 of it, the most that two keys can give.  On the tcgen05 path weights and
+        values, sqrt(2) of it
       * scores off by e: e N.  Products of bare key codes are cut at 2^-14 of the largest query times a code's
         step: 6 sqrt(D / 3) 2^-14 max|q| max s scale at six sigma; of codes less 8, and in f32's sums and
-        queries of 22 bits, 2^-19 |q| |k| scale by Cauchy and Schwarz
+        queries of 22 bits, 2^-19 |q| |k| scale by Cauchy and Schwarz.  On the tcgen05 path a key's values are
+        rounded by 2^-11 each: 6 / sqrt(3) 2^-11 sqrt(sum q_d^2 k_d^2) scale at six sigma
       * weights in 32 bits: the largest is 2^-8 or more, and 2^(s - m) below fp32's 2^-126 is zero, so keys of less
         than 2^-118 of the largest weight may count as nothing: sum w_j |v_j| over those
       * f16's smallest steps: 2^-23 of the largest weight times scale, for each key: sqrt(keys) of that
@@ -72,14 +74,13 @@ def bounds(plan, q, counts, scale, causal, tensor_core=False):
     out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
     tol = torch.zeros((B, H, L, ng), dtype=torch.float64, device="cuda")
     tile = torch.zeros_like(tol)
-    rounded = (lambda x: x.float().to(DTYPES[plan.dtype]).double()) if tensor_core else (lambda x: x)
-    h = u if tensor_core else 2.0 ** (-22 if plan.dtype == "float32" else -11)
+    h = 2.0 ** -22 if plan.dtype == "float32" else 2.0 ** -11 * (2 ** 0.5 if tensor_core else 1.0)
     bare = plan.dtype == "bfloat16" and not tensor_core
     for b, n in enumerate(plan.lengths):
         c = L if counts is None else counts[b]
         if n == 0 or c == 0:
             continue
-        K, V = rounded(plan.values(0, b)), rounded(plan.values(1, b))
+        K, V = plan.values(0, b), plan.values(1, b)
         cols = plan.table[b, : -(-n // plan.page)].long()
         pick = lambda t: t._t[cols].transpose(0, 1).flatten(1, 2)[:, :n].double()  # noqa: E731
         sk, sv, zv = pick(plan.parts(0)[1]).abs(), pick(plan.parts(1)[1]), pick(plan.parts(1)[2])
@@ -98,9 +99,13 @@ def bounds(plan, q, counts, scale, causal, tensor_core=False):
             N = (w.square() @ lone.square()).sqrt()
             seen = (w > 0).double()
             qk = x.norm(dim=-1, keepdim=True) * (seen * k.norm(dim=-1)).amax(-1, keepdim=True) * abs(scale)
-            cut = 0.0 if plan.dtype == "float32" else (
-                6 * (D / 3) ** 0.5 * 2.0 ** -14 * abs(scale) * x.abs().amax(-1, keepdim=True)
-                * (seen * sk[head // per].amax(-1)).amax(-1, keepdim=True))
+            if plan.dtype == "float32":
+                cut = 0.0
+            elif tensor_core:
+                cut = 2.0 ** -11 * 6 / 3 ** 0.5 * abs(scale) * (seen * (x.square() @ k.square().T)).amax(-1, keepdim=True).sqrt()
+            else:
+                cut = (6 * (D / 3) ** 0.5 * 2.0 ** -14 * abs(scale) * x.abs().amax(-1, keepdim=True)
+                       * (seen * sk[head // per].amax(-1)).amax(-1, keepdim=True))
             e = qk * 2.0 ** -19 + cut
             step = s_v.abs()
             top = torch.stack([(w * step[:, g]).amax(-1) for g in range(ng)], -1)
@@ -169,6 +174,24 @@ def test_long_histories_closely(mx, dtype):
 def test_chunks_closely(mx, dtype, head_dim, group, tokens, heads, causal):
     plan = Plan(mx, [1500, tokens, 0, 131], kv_heads=2, head_dim=head_dim, group=group, dtype=dtype, page=24, seed=tokens)
     attend_closely(mx, plan, rand((4, heads, tokens, head_dim), dtype, 7), [tokens, tokens, 3, 31], causal=causal)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("head_dim,group", [(64, 32), (128, 64), (128, 128), (256, 64)])
+@pytest.mark.parametrize("tokens", [60, 500])  # packed (heads of 256: expanded), expanded
+def test_chunks_to_the_types_own_rounding(mx, dtype, head_dim, group, tokens):
+    """The norm of the whole error of a chunk over normal keys and values.  Independent errors add in squares, each
+    uniform up to its bound, so a third of that in square: the output's rounding, u at the start of a binade and
+    less behind it; weights and values, 2^-11; keys, 2^-11 of sqrt(sum q_d^2 k_d^2) scale = 1 in a score.  5 % for
+    what 10^5 values and more leave to chance."""
+    u = 2.0 ** {"bfloat16": -8, "float16": -11}[dtype]
+    plan = Plan(mx, [3000, 1100], kv_heads=2, head_dim=head_dim, group=group, dtype=dtype, page=64, seed=tokens)
+    q = rand((2, 8, tokens, head_dim), dtype, 17)
+    o = mx.fast.quantized_cache_attention(mx.array(q), plan.cache, mx.array(ints(plan.lengths)),
+                                          block_table=mx.array(plan.table), scale=head_dim ** -0.5, mask="causal")._t
+    want = bounds(plan, q, None, head_dim ** -0.5, True, True)[0]
+    off = float((o.double() - want).norm() / want.norm())
+    assert off <= 1.05 * ((u * u + 3 * 2.0 ** -22) / 3) ** 0.5, f"{off:.3g}"
 
 
 # --- values of very different magnitude ---------------------------------------------------
@@ -266,6 +289,46 @@ def test_values_of_the_whole_range(mx, dtype, heads, tokens, drop, copies):
     plan.cache = mx.fast.QuantizedKVCache(*sides, group_size=64, bits=4)
     q = torch.ones((1, heads, tokens, 128), device="cuda").to(DTYPES[dtype])
     attend_closely(mx, plan, q, scale=0.5, sharp=False, copies=copies)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("tokens", [40, 300])  # packed, expanded; both split along the keys
+@pytest.mark.parametrize("what", ["value", "groups", "keys"])
+@pytest.mark.parametrize("causal", [False, True])
+def test_chunks_over_more_than_f16_holds(mx, dtype, tokens, what, causal):
+    """A key of no weight with a large value, groups of different magnitude, keys next to nothing among others: what
+    a tile of 128 keys cannot hold in f16 units of its own."""
+    plan = Plan(mx, [900, 500], kv_heads=2, dtype=dtype, page=100)
+    large, small = spread(dtype, 36)
+    k, v = plan.dense
+    q = rand((2, 8, tokens, 128), dtype, 16)
+    if what == "value":
+        q = q.abs()
+        at = int(plan.table[0, 4])
+        k[at, :, 50] = -8.0
+        v *= small
+        v[at, :, 50] *= large / small
+    elif what == "groups":
+        v[..., :64] *= large
+        v[..., 64:] *= small
+    else:
+        k[int(plan.table[1, 2]), :, :50] *= 2.0 ** (-24 if dtype == "float16" else -36)
+    sides = [mx.quantize(mx.array(x), group_size=64, bits=4) for x in plan.dense]
+    plan.cache = mx.fast.QuantizedKVCache(*sides, group_size=64, bits=4)
+    attend_closely(mx, plan, q, causal=causal, sharp=False)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("tokens", [40, 300])
+def test_chunks_over_zeros(mx, dtype, tokens):
+    """Tokens of zeros, and heads of the head dimension that are next to nothing, among ordinary ones."""
+    plan = Plan(mx, [900, 500], kv_heads=2, dtype=dtype, page=100)
+    for x in plan.dense:
+        x[:, :, 10:13] = 0.0
+        x[:, 1, :, 64:] *= 2.0 ** -12
+    sides = [mx.quantize(mx.array(x), group_size=64, bits=4) for x in plan.dense]
+    plan.cache = mx.fast.QuantizedKVCache(*sides, group_size=64, bits=4)
+    attend_closely(mx, plan, rand((2, 8, tokens, 128), dtype, 18), causal=True, sharp=False)
 
 
 # --- pages that are none of the cache's ------------------------------------------------------
