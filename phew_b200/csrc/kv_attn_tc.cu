@@ -18,9 +18,9 @@
 // this way, for bf16 too (whose own 8 bits cost 3.2e-3 of an output's norm, 1.7e-3
 // of them its rounding).  Scores, maxima and sums are 32-bit.  Where magnitudes in
 // a tile lie further apart than f16 holds (Reach::odd) its rows are computed again
-// by plain_rows_kernel, in one thread's fp32 arithmetic: slow, for caches that no
-// model writes.  (A launch of its own, 2 us; at the end of this kernel its code
-// cost 10 to 20.)
+// by plain_rows_kernel, in fp32: 27 ms for the chunk below, for caches that no
+// model writes.  (A launch
+// of its own, 2 us; at the end of this kernel its code cost 10 to 20.)
 //
 // Two forms:
 //
@@ -64,7 +64,7 @@
 // and leaves partial sums, joined in a fixed order by the combine kernel.
 //
 // Measured, causal, heads of 128 in bf16: two prompts of 4096 tokens on 32
-// heads, 332 us (828 TFLOP/s); the last 2048 of 8192 tokens on 32 heads over 8,
+// heads, 334 us (823 TFLOP/s); the last 2048 of 8192 tokens on 32 heads over 8,
 // 246 us (977 TFLOP/s).  Errors of an output's norm: 1.7e-3 in bf16, 3.9e-4 in
 // f16 (2.1e-4 its own rounding).
 //
@@ -332,68 +332,6 @@ template <typename S> __device__ __forceinline__ Share share_of(const TcParams& 
   s.n_max = static_cast<int>(static_cast<int64_t>(all) * (s.split + 1) / p.splits) - s.j0;
   for (int t = 0; t < 2; ++t) s.n_t[t] = min(max(need[t] - s.j0, 0), s.n_max);
   return s;
-}
-
-// A row's keys [k0, k1) in fp32, from the cache as it lies, by one thread: where a quarter's magnitudes differ by more
-// than f16 holds.  To `out`, or as a partial to `part` and `ml`.  Every 32 head dimensions go through the keys again,
-// so that no thread needs more memory of its own than registers.
-template <typename T, int D>
-__device__ __forceinline__ void plain_row(const TcParams& p, int b, int h, int head, int tok, int k0, int k1, T* out,
-                                       float* part, float* ml) {
-  const T* q = static_cast<const T*>(p.q) + b * p.st[2] + head * p.st[1] + tok * p.st[0];
-  const int ng = D / p.c.group;
-  float top = 0.f;
-  for (int d = 0; d < D; ++d) top = fmaxf(top, fabsf(to_f32(q[d])));
-  const int qe = query_unit(top);
-  const float up = pow2(-qe);  // (qe is -121 .. 114)
-  for (int d0 = 0; d0 < D; d0 += 32) {
-    float o[32], m = kTcFloor, l = 0.f;
-#pragma unroll
-    for (int d = 0; d < 32; ++d) o[d] = 0.f;
-    for (int key = k0; key < k1; ++key) {
-      const uint32_t at = row_of(p.c.map, b, h, key);
-      float s = 0.f, sv = 0.f, zv = 0.f;  // (a bad page's: zeros; it is reported already)
-      uint32_t word[4] = {};
-      if (at != kNoRow) {
-        const int64_t g0 = static_cast<int64_t>(at) * ng;
-        const uint32_t* k = p.c.codes[0] + static_cast<int64_t>(at) * (D / 8);
-        for (int g = 0; g < ng; ++g) {
-          float dot = 0.f, sum = 0.f;
-          for (int d = g * p.c.group; d < (g + 1) * p.c.group; ++d) {
-            const float x = to_f32(q[d]) * up;
-            dot = fmaf(x, static_cast<float>(k[d >> 3] >> (4 * (d & 7)) & 15), dot);
-            sum += x;
-          }
-          // (2^-24: a large key's bias times the sum stays in range)
-          s = fmaf(to_f32(static_cast<const T*>(p.c.scales[0])[g0 + g]) * 0x1p-24f, dot,
-                   fmaf(to_f32(static_cast<const T*>(p.c.biases[0])[g0 + g]) * 0x1p-24f, sum, s));
-        }
-        s = s * (p.scale_log2 * 0x1p24f) * pow2(qe);
-        sv = to_f32(static_cast<const T*>(p.c.scales[1])[g0 + d0 / p.c.group]);
-        zv = to_f32(static_cast<const T*>(p.c.biases[1])[g0 + d0 / p.c.group]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) word[i] = p.c.codes[1][static_cast<int64_t>(at) * (D / 8) + d0 / 8 + i];
-      }
-      const float m_new = fmaxf(m, s), was = ex2(m - m_new), w = ex2(s - m_new);
-      m = m_new;
-      l = fmaf(l, was, w);
-#pragma unroll
-      for (int d = 0; d < 32; ++d)
-        o[d] = fmaf(w, fmaf(sv, static_cast<float>(word[d >> 3] >> (4 * (d & 7)) & 15), zv), o[d] * was);
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int d = 0; d < 32; ++d) {
-      if (part)
-        part[d0 + d] = o[d];
-      else
-        out[d0 + d] = from_f32<T>(o[d] * inv);
-    }
-    if (part) {
-      ml[0] = m;
-      ml[1] = l;
-    }
-  }
 }
 
 template <typename S, bool BF16, bool DENSE>
@@ -881,23 +819,100 @@ __global__ void __launch_bounds__(tc_threads(DENSE, S::QT), 1)
   if (threadIdx.x == 0) p.odd[blockIdx.x] = s_odd[0] | s_odd[1] << 1;
 }
 
-// Rows that met keys that f16 does not hold, again: CTA by CTA of attn_tc_kernel, a thread to a row.
-template <typename S, bool BF16> __global__ void __launch_bounds__(S::ROWS) plain_rows_kernel(const TcParams p) {
+// Rows that met keys that f16 does not hold, again, in fp32 from the cache as it lies: a query tile of a CTA of
+// attn_tc_kernel to a block, a thread to a row, sixteen keys at a time in shared memory.  Heads of 256 go through the
+// keys twice, for half of their values each.
+constexpr int kPlainKeys = 16;
+template <typename S, bool BF16> __global__ void __launch_bounds__(kTileRows) plain_rows_kernel(const TcParams p) {
   using T = typename std::conditional<BF16, bf16, f16>::type;
-  constexpr int D = S::D;
+  constexpr int D = S::D, DV = D < 128 ? D : 128;
+  __shared__ __align__(16) float s_k[kPlainKeys][D], s_v[kPlainKeys][DV];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int t = threadIdx.x / kTileRows;
+  const int t = blockIdx.y;
   if (!(p.odd[blockIdx.x] >> t & 1)) return;
-  const Share s = share_of<S>(p);
-  const int r = s.row0 + static_cast<int>(threadIdx.x);
+  const Share sh = share_of<S>(p);
+  const int r = sh.row0 + t * kTileRows + static_cast<int>(threadIdx.x);
   const int tok = static_cast<int>(div_by(p.by_per, static_cast<uint32_t>(r)));
-  const int head = s.h * p.per + (r - tok * p.per);
-  const int end = min(seen_end(s.length, s.count, tok, p.causal), (s.j0 + (t ? s.n_t[1] : s.n_t[0])) * kTcTile);
-  if (end <= 0) return;
-  const int64_t slot = ((static_cast<int64_t>(s.bh) * p.blocks + s.rb) * p.splits + s.split) * S::ROWS + threadIdx.x;
-  T* out = static_cast<T*>(p.o) + ((static_cast<int64_t>(s.b) * p.heads + head) * p.tokens + tok) * D;
-  plain_row<T, D>(p, s.b, s.h, head, tok, s.j0 * kTcTile, end, out, p.splits > 1 ? p.part + slot * D : nullptr,
-                  p.part_ml + slot * 2);
+  const int head = sh.h * p.per + (r - tok * p.per);
+  const int first = sh.j0 * kTcTile, last = min(sh.length, first + (t ? sh.n_t[1] : sh.n_t[0]) * kTcTile);
+  const int end = min(seen_end(sh.length, sh.count, tok, p.causal), last);  // 0 for a row without a query
+  const T* q = static_cast<const T*>(p.q) + sh.b * p.st[2] + head * p.st[1] + tok * p.st[0];
+  float top = 0.f;
+  if (end > 0)
+    for (int d = 0; d < D; ++d) top = fmaxf(top, fabsf(to_f32(q[d])));
+  const int qe = query_unit(top);
+  const float up = pow2(-qe);  // (qe is -121 .. 114)
+  const int ng = D / p.c.group;
+  for (int d0 = 0; d0 < D; d0 += DV) {
+    float o[DV], m = kTcFloor, l = 0.f;
+#pragma unroll
+    for (int d = 0; d < DV; ++d) o[d] = 0.f;
+    for (int key0 = first; key0 < last; key0 += kPlainKeys) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < 2 * kPlainKeys * (D / 8); i += kTileRows) {
+        const int side = i / (kPlainKeys * (D / 8)), k = i / (D / 8) % kPlainKeys, w = i % (D / 8);
+        if (side && (w * 8 < d0 || w * 8 >= d0 + DV)) continue;
+        const uint32_t at = key0 + k < last ? row_of(p.c.map, sh.b, sh.h, key0 + k) : kNoRow;
+        uint32_t word = 0;
+        float sc = 0.f, bi = 0.f;  // (a bad page's: zeros; it is reported already)
+        if (at != kNoRow) {
+          const int64_t g = static_cast<int64_t>(at) * ng + w * 8 / p.c.group;
+          word = p.c.codes[side][static_cast<int64_t>(at) * (D / 8) + w];
+          sc = to_f32(static_cast<const T*>(p.c.scales[side])[g]);
+          bi = to_f32(static_cast<const T*>(p.c.biases[side])[g]);
+        }
+        float* dst = side ? &s_v[k][w * 8 - d0] : &s_k[k][w * 8];
+        // (keys times 2^-24: with a query of 2^15 the largest stay in range)
+        const float by = side ? 1.f : 0x1p-24f;
+        for (int x = 0; x < 8; ++x) dst[x] = fmaf(sc * by, static_cast<float>(word >> (4 * x) & 15), bi * by);
+      }
+      __syncthreads();
+      if (key0 >= end) continue;
+      float s[kPlainKeys];
+#pragma unroll
+      for (int k = 0; k < kPlainKeys; ++k) s[k] = 0.f;
+      for (int d = 0; d < D; d += 4) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = to_f32(q[d + i]) * up;
+#pragma unroll
+        for (int k = 0; k < kPlainKeys; ++k) {
+          const float4 y = *reinterpret_cast<const float4*>(&s_k[k][d]);
+          s[k] = fmaf(x[0], y.x, fmaf(x[1], y.y, fmaf(x[2], y.z, fmaf(x[3], y.w, s[k]))));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kPlainKeys; ++k) {
+        if (key0 + k >= end) break;
+        const float x = s[k] * (p.scale_log2 * 0x1p24f) * pow2(qe);
+        const float m_new = fmaxf(m, x), was = ex2(m - m_new), w = ex2(x - m_new);
+        m = m_new;
+        l = fmaf(l, was, w);
+#pragma unroll
+        for (int d = 0; d < DV; d += 4) {
+          const float4 y = *reinterpret_cast<const float4*>(&s_v[k][d]);
+          o[d] = fmaf(w, y.x, o[d] * was);
+          o[d + 1] = fmaf(w, y.y, o[d + 1] * was);
+          o[d + 2] = fmaf(w, y.z, o[d + 2] * was);
+          o[d + 3] = fmaf(w, y.w, o[d + 3] * was);
+        }
+      }
+    }
+    if (end <= first) continue;
+    const int64_t slot = ((static_cast<int64_t>(sh.bh) * p.blocks + sh.rb) * p.splits + sh.split) * S::ROWS + t * kTileRows + threadIdx.x;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (p.splits > 1) {
+      float* part = p.part + slot * D + d0;
+#pragma unroll
+      for (int d = 0; d < DV; ++d) part[d] = o[d];
+      p.part_ml[slot * 2] = m;
+      p.part_ml[slot * 2 + 1] = l;
+    } else {
+      T* out = static_cast<T*>(p.o) + ((static_cast<int64_t>(sh.b) * p.heads + head) * p.tokens + tok) * D + d0;
+#pragma unroll
+      for (int d = 0; d < DV; ++d) out[d] = from_f32<T>(o[d] * inv);
+    }
+  }
 }
 
 // Joins the splits of a row: one warp per row, splits in their order.
@@ -1114,8 +1129,8 @@ int launch_tc(const Maps& m, const TcParams& p, unsigned grid, cudaStream_t st) 
   PHEW_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_tc_kernel<S, BF16, DENSE>, m.k, m.v, p));
   if (int s = launch_status("kv attn_tc_kernel")) return s;
   cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(S::ROWS);
+  cfg.gridDim = dim3(grid, S::QT);
+  cfg.blockDim = dim3(kTileRows);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
