@@ -19,8 +19,8 @@
 // of them its rounding).  Scores, maxima and sums are 32-bit.  Where magnitudes in
 // a tile lie further apart than f16 holds (Reach::odd) its rows are computed again
 // by plain_rows_kernel, in fp32: 27 ms for the chunk below, for caches that no
-// model writes.  (A launch
-// of its own, 2 us; at the end of this kernel its code cost 10 to 20.)
+// model writes.  (A launch of its own, 2 us; at the end of this kernel its code
+// cost 10 to 20.)
 //
 // Two forms:
 //
@@ -1061,15 +1061,18 @@ template <typename T> int launch_expand(const ExpandParams& p, unsigned tiles, c
 // whether the cache is expanded first.
 // Query rows to a cache head above which the kernel is taken: up to there the mma.sync kernel's passes of 16 rows
 // (8 of heads of 256) over the cache cost less than a tile of 128 that is mostly empty.  Measured, mma.sync against
-// this kernel, 8 cache heads of 8192 keys / 16 x 8 of 2048 / 8 of 65536: at 48 rows 22 : 31, 49 : 57, 81 : 106 us,
-// at 64 rows 24 : 31, 61 : 57, 103 : 106, at 96 rows 30 : 32, 84 : 57, 146 : 107.  Heads of 256, 8 of 8192 keys /
-// 8 x 8 of 2048: at 64 rows 44 : 55, 77 : 82, at 96 rows 58 : 56, 105 : 84.
+// this kernel, 8 cache heads of 8192 keys / 16 x 8 of 2048 / 8 of 65536: at 48 rows 24 : 34, 54 : 60, 87 : 114 us,
+// at 64 rows 26 : 34, 66 : 60, 110 : 114, at 96 rows 33 : 34, 91 : 61, 156 : 115.  Heads of 256, 8 of 8192 keys /
+// 8 x 8 of 2048: at 64 rows 45 : 55, 78 : 78, at 96 rows 59 : 55, 109 : 79.
 constexpr int64_t kTcAbove = 64;
-// Row blocks from which one expansion beats one per CTA.  Expanded against packed, the same three caches: 2 blocks
-// 44 : 45, 126 : 123, 216 : 209 us, 3 blocks 50 : 56, 162 : 180, 274 : 306, 4 blocks 59 : 69, 198 : 234, 357 : 428.
+// Row blocks from which one expansion beats one per CTA.  Expanded against packed, the same three caches: 1 block
+// 37 : 38, 75 : 65, 138 : 133 us, 2 blocks 44 : 48, 117 : 127, 190 : 226, 3 blocks 50 : 61, 158 : 194, 248 : 322.
 // Heads of 256 are always expanded.
-constexpr int64_t kExpandBlocks = 3;
-constexpr int64_t kExpandBytes = int64_t(1) << 30;  // scratch that a call may take for it
+constexpr int64_t kExpandBlocks = 2;
+// Scratch that a call may take for it, a bound on memory and not on time.  Beyond, packed against expanded, 8 sequences of
+// 8 heads of 128 behind tables for 65536 tokens (2 GiB), 2048 rows: 65536 keys each 6880 : 4643 us, 8192 869 : 641,
+// 2048 243 : 252; heads of 256 behind 32768 tokens, on the mma.sync kernel: 32768 keys 32349 : 5345, 2048 2163 : 416.
+constexpr int64_t kExpandBytes = int64_t(1) << 30;
 
 int rows_of(int head_dim) { return head_dim <= 128 ? TcShape<128, 128>::ROWS : TcShape<256, 128>::ROWS; }
 
