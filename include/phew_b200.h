@@ -325,8 +325,7 @@ int phew_quantize(const void* w, void* wq, void* scales, void* biases, int64_t r
  * outside a sequence's pages or a table entry that is no page of the cache
  * is not accessed: it sets error_flag[0] to PHEW_ERR_INVALID, and its keys
  * and values count as zeros (a length past a sequence's pages ends at them).
- * error_flag is
- * two device ints; a pipeline wait of phew_kv_attention that runs out sets
+ * error_flag is two device ints; a pipeline wait of phew_kv_attention that runs out sets
  * error_flag[1] to PHEW_ERR_TIMEOUT. */
 typedef struct phew_kv_cache {
   void* k_codes;
@@ -379,7 +378,12 @@ size_t phew_kv_attention_workspace(const phew_kv_cache* cache, int64_t batch, in
  * lengths[b] keys and counts[b] query tokens (NULL = all).  causal = 1: the
  * last query token sits at the last key, token i sees keys
  * j <= lengths[b] - counts[b] + i.  Rows that see no key, and rows behind
- * counts[b], are zero.  Scores, softmax statistics and sums are fp32.
+ * counts[b], are zero.  Scores, softmax statistics and sums are fp32.  Up to 64
+ * query rows (tokens * heads / kv_heads) to a cache head, and in fp32 always,
+ * the codes enter the products exactly and weights times value scales are
+ * rounded to 11 bits (fp32: 22, as the queries); above, keys, values and
+ * weights are rounded to 11 bits each.  Which kernels run, and the scratch (at
+ * most about 1 GiB), goes by columns * page_size and not by the lengths.
  * `workspace`: caller-owned scratch of phew_kv_attention_workspace bytes,
  * 16-byte aligned; calls that may overlap need one each.
  * Replaces mx.fast.quantized_scaled_dot_product_attention

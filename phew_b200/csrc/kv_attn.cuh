@@ -36,8 +36,9 @@
 //    one.  The factors lie in shared memory and are looked at again only when a
 //    row's maximum moves, or a scale itself would pass f16's range under one of
 //    them (one comparison a tile; a segment's first tile always: 0.5 us of a
-//    short call, 1.8 with two row tiles).  f32 queries and weights are two f16 terms (22 bits), and its
-//    sums leave the tensor core, which cuts what it adds off, every 16 keys;
+//    short call, 1.5 with two row tiles).  f32 queries and weights are two f16
+//    terms (22 bits), and its sums leave the tensor core, which cuts what it
+//    adds off, every 16 keys;
 //  * a word's eight codes stay with the thread that loads it: the order of
 //    the head dimension inside a product is free, so queries are arranged to
 //    match and nothing is shuffled; weights move from the score fragment
@@ -54,8 +55,8 @@
 // sums (maximum, sum, output) that the combine kernel joins in a fixed order.
 //
 // Measured: 64 sequences of up to 8192 keys, 32 heads of 128 over 8, bf16:
-// 80 us, 3.8 TB/s of the bytes that must be read (0.59 of a copy).  Three warps
-// to a scheduler (168 registers) issue every other cycle: 613 instructions to
+// 82 us, 3.8 TB/s of the bytes that must be read (0.57 of a copy).  Three warps
+// to a scheduler (168 registers) issue every other cycle: 663 instructions to
 // a tile, waits on one another's results between them.  Four (128 registers)
 // spill, or read the queries from shared memory, for the same time.
 #pragma once

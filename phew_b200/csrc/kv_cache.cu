@@ -304,7 +304,7 @@ __device__ __forceinline__ void codes8(const Eight<T>& x, const Affine& a, uint3
 
 // Bound by HBM (update of 4 x 32 heads x 8192 tokens of 128 bf16 values with
 // the values written back: 1.22 GB in 225 us, 5.4 TB/s, 0.83 of the copy rate)
-// and by issue slots (0.74 of them).  A thread takes sixteen neighbouring
+// and by issue slots (0.69 of them).  A thread takes sixteen neighbouring
 // values of a row, so that its address and the group's scale are worked out once
 // for them; a group is G / 16 neighbouring lanes.  (Eight of either half of the
 // row make every access of a warp contiguous: 4 % faster for f32 with its values

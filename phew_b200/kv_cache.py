@@ -332,6 +332,19 @@ def quantized_cache_attention(q, cache: QuantizedKVCache, lengths, *, block_tabl
     behind ``counts``, are zero.  A block table entry that is no page of the
     cache stands for keys and values of zero, a length past a sequence's pages
     ends at them; both are reported by ``ops.check_device_errors``.
+
+    Scores, softmax statistics and sums are 32-bit.  With up to 64 query rows
+    (tokens x heads / kv_heads) to a cache head, and always in float32, the
+    codes enter the products as they are and weights times value scales are
+    rounded to 11 bits (22 in float32, queries too); with more, keys, values
+    and weights are rounded to 11 bits each.  Errors of an output's norm are then
+    1.7e-3 in bfloat16 (its own rounding), 3e-4 and 4e-4 in float16 (2.1e-4).
+
+    Above 64 rows the call takes scratch from torch's allocator, up to 1 GiB,
+    and which kernels it runs goes by the tokens that the block table could
+    hold, not by the lengths: a table as wide as the longest sequence needs is
+    the fastest, and heads of 256 whose table passes the scratch (2 x batch x
+    kv_heads x tokens x 512 bytes) are several times slower.
     """
     if mask is not None and not (isinstance(mask, str) and mask == "causal"):
         raise ValueError(f"quantized_cache_attention: mask must be None or 'causal', got {mask!r}")
