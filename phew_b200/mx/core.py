@@ -758,10 +758,10 @@ def settle_readers(tensors) -> None:
     written = [_storage_range(t) for t in tensors]
     for key, ref in list(_deferred.items()):
         a = ref()
-        if a is None or not a.pending:
-            _deferred.pop(key, None)  # dead or computed: nothing to settle any more
+        op = None if a is None else a._op
+        if op is None:
+            _deferred.pop(key, None)  # dead or computed (by another thread, maybe): nothing to settle any more
             continue
-        op = a._op
         for x in ((op[2],) if op[0] == _ROW_REDUCE else op[1]):
             if not isinstance(x, array) or (isinstance(x, _Lazy) and x.pending):
                 continue
