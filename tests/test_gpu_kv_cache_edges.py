@@ -1,6 +1,6 @@
 """Quantised key/value cache where it can go wrong beyond its sizes: calls
-inside mx.compile, values of very different magnitude, bad pages, calls in
-which nothing is asked."""
+inside mx.compile and captures, errors by row and group, values of very
+different magnitude, bad pages, what is no number, two calls at once."""
 
 from __future__ import annotations
 
@@ -502,3 +502,52 @@ def test_caches_made_by_threads_report_to_one_flag(mx, monkeypatch):
         t.join()
     flag = kv_cache._error_flags[plan.cache.device.index]
     assert len(caches) == 8 and all(c._flag == flag.data_ptr() for c in caches) and not flag.any()
+
+
+# --- two at once -----------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("tokens", [40, 300])  # packed, expanded; both split along the keys
+@pytest.mark.parametrize("odd", [False, True])
+def test_chunks_on_two_streams(mx, tokens, odd):
+    """Each call has its scratch, and the launches behind it wait for their own; over a tile that f16 does not hold
+    in one of the caches too."""
+    plans = [Plan(mx, [1500, 700], kv_heads=2, page=64, seed=i) for i in range(2)]
+    if odd:
+        plans[1].cache.values[1]._t[int(plans[1].table[0, 3]), :, 5] = 2.0 ** 40
+    qs = [mx.array(rand((2, 8, tokens, 128), "bfloat16", 20 + i)) for i in range(2)]
+    n = [mx.array(ints(p.lengths)) for p in plans]
+    tables = [mx.array(p.table) for p in plans]
+    run = lambda i: mx.fast.quantized_cache_attention(  # noqa: E731
+        qs[i], plans[i].cache, n[i], block_table=tables[i], scale=128 ** -0.5, mask="causal")._t
+    want = [run(i).clone() for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                outs[i].append(run(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.isfinite(want[i]).all() and all(torch.equal(o, want[i]) for o in outs[i])
+
+
+def test_chunk_replays_over_other_contents(mx):
+    """A captured chunk whose cache comes to hold what f16 does not, and no longer does."""
+    plan = Plan(mx, [700], kv_heads=2, page=64)
+    q, table, n = mx.array(rand((1, 8, 300, 128), "bfloat16", 21)), mx.array(plan.table), mx.array(ints([700]))
+    run = lambda: mx.fast.quantized_cache_attention(q, plan.cache, n, block_table=table, scale=0.1, mask="causal")._t  # noqa: E731
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = run()
+    scales = plan.cache.values[1]._t
+    old = scales.clone()
+    for factor in (1.0, 2.0 ** 40, 1.0, 2.0 ** 40):
+        scales.copy_(old)
+        scales[int(plan.table[0, 2]), :, 7] *= factor
+        graph.replay()
+        want, tol, _ = bounds(plan, q._t, None, 0.1, True, True)
+        assert bool((groups_err(o, want, 64) <= tol).all())
