@@ -65,8 +65,9 @@
 //
 // Measured, causal, heads of 128 in bf16: two prompts of 4096 tokens on 32
 // heads, 334 us (823 TFLOP/s); the last 2048 of 8192 tokens on 32 heads over 8,
-// 246 us (977 TFLOP/s).  Errors of an output's norm: 1.7e-3 in bf16, 3.9e-4 in
-// f16 (2.1e-4 its own rounding).
+// 247 us (974 TFLOP/s).  Errors of an output's norm: 1.7e-3 in bf16, 4.6e-4 in
+// f16 (2.1e-4 its own rounding; 2.9e-4 with keys and values as two terms each,
+// at 462 us instead of 257 for that chunk in f16).
 //
 // Every wait is bounded; one that runs out sets error_flag[1] and the CTA
 // winds down with its TMEM freed.
