@@ -338,7 +338,8 @@ def quantized_cache_attention(q, cache: QuantizedKVCache, lengths, *, block_tabl
     codes enter the products as they are and weights times value scales are
     rounded to 11 bits (22 in float32, queries too); with more, keys, values
     and weights are rounded to 11 bits each.  Errors of an output's norm are then
-    1.7e-3 in bfloat16 (its own rounding), 3e-4 and 4e-4 in float16 (2.1e-4).
+    1.7e-3 in bfloat16 (its own rounding); in float16 (2.1e-4) 3e-4, above 64
+    rows 4e-4 to 5e-4.
 
     Above 64 rows the call takes scratch from torch's allocator, up to 1 GiB,
     and which kernels it runs goes by the tokens that the block table could
